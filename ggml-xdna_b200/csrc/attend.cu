@@ -1,0 +1,674 @@
+// Attention of new tokens over the paged cache (zest_kv_attend).
+//
+// The rows of one kv head are its new tokens' query heads, token by token:
+// row r of a sequence is token r / G, head r % G of the group (G = heads /
+// kv_heads). All of them read the same keys and values, so a tile of rows
+// costs one read of the cache whatever G is.
+//
+// One pass over the keys with the running maximum m and sum l of a softmax in
+// base 2 (the scale times log2 e folded into one multiply-add):
+//   m' = max(m, s_j),  o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j,  l' alike.
+//
+// A long row of keys is cut into chunks that different blocks take (the grid's
+// x), each leaving its unnormalised o, m and l in the workspace, joined in
+// order by kv_combine_kernel; with one chunk the result is written at once.
+#include "zest_kv.cuh"
+
+#include <algorithm>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+namespace zest {
+
+namespace {
+
+constexpr uint64_t WAIT_LIMIT_NS = 1000000000ull;  // 1 s
+constexpr int ROWS = 16;                           // query rows of a tile of the few-rows kernel
+constexpr int KEYS = 64;                           // keys of a stage
+
+struct attend_args {
+    zest_kv_batch b;
+    const uint16_t *q;
+    int64_t ldq, pages;
+    const uint16_t *v;  // this layer's values, for the rows that see a NaN or infinity others do not
+    int64_t page_stride, token_stride, head_stride;
+    int heads, group, d, page_size, causal;
+    int64_t window;
+    float scale_log2;
+    uint16_t *out;
+    int64_t ldo;
+    float *y;
+    int64_t ldy;
+    uint16_t *a_next;
+    int64_t lda;
+    int64_t chunk;      // keys a block takes, a multiple of 64; splits chunks at most
+    int splits;
+    float2 *ml;         // [splits][T * heads]: m and l
+    float *part;        // [splits][T * heads][DP]: o
+    unsigned *err;
+};
+
+// The keys that rows of tokens [t_lo, t_hi] see: any of them [lo, hi), all of them [clo, chi).
+struct key_span {
+    int lo, hi, clo, chi;
+};
+
+__device__ __forceinline__ int row_lo(const attend_args &A, const kv_seq &s, int t) {
+    return A.causal && A.window ? (int) max((int64_t) 0, (int64_t) s.kv - s.n + t - A.window + 1) : 0;
+}
+
+__device__ __forceinline__ int row_hi(const attend_args &A, const kv_seq &s, int t) {
+    return A.causal ? max(0, s.kv - s.n + t + 1) : s.kv;
+}
+
+__device__ __forceinline__ key_span span_of(const attend_args &A, const kv_seq &s, int t_lo, int t_hi) {
+    return { row_lo(A, s, t_lo), row_hi(A, s, t_hi), row_lo(A, s, t_hi), row_hi(A, s, t_lo) };
+}
+
+// Eight results of one row, from column c on: as asked for in the cache's
+// type, in f32, and as the next matmul's operand.
+template <bool F16>
+__device__ __forceinline__ void store8(const attend_args &A, int64_t t, int head, int c, const float (&o)[8]) {
+    const int64_t col = (int64_t) head * A.d + c;
+    if (A.out) {
+        uint4 w;
+        w.x = kv_bits2<F16>(o[0], o[1]);
+        w.y = kv_bits2<F16>(o[2], o[3]);
+        w.z = kv_bits2<F16>(o[4], o[5]);
+        w.w = kv_bits2<F16>(o[6], o[7]);
+        *reinterpret_cast<uint4 *>(A.out + t * A.ldo + col) = w;
+    }
+    if (A.y) {
+        float4 *y = reinterpret_cast<float4 *>(A.y + t * A.ldy + col);
+        y[0] = make_float4(o[0], o[1], o[2], o[3]);
+        y[1] = make_float4(o[4], o[5], o[6], o[7]);
+    }
+    if (A.a_next) {
+        uint8_t enc[9];
+        uint32_t bf[4];
+        encode_block(o, enc, bf);
+        *reinterpret_cast<uint4 *>(A.a_next + t * A.lda + col) = make_uint4(bf[0], bf[1], bf[2], bf[3]);
+    }
+}
+
+// A NaN or infinite value that some rows of a tile see and others do not is
+// taken as zero in the tile's product (0 times it would reach every row) and
+// added here to the rows that see it: keys [lo, hi) of the row's own range.
+template <bool F16>
+__device__ void add_not_finite(const attend_args &A, int s, int kv_head, int c, int lo, int hi, float (&o)[8]) {
+    for (int j = lo; j < hi; j++) {
+        const int64_t page = A.b.table[s * A.b.table_stride + j / A.page_size];
+        if (page < 0 || page >= A.pages) continue;
+        const uint16_t *v =
+            A.v + page * A.page_stride + j % A.page_size * A.token_stride + kv_head * A.head_stride + c;
+        for (int i = 0; i < 8; i++) {
+            const float x = kv_value<F16>(v[i]);
+            if (!(fabsf(x) <= 3.4028234e38f)) o[i] += x;
+        }
+    }
+}
+
+// --- m16n8k16 on a warp (few rows: the cache's bytes bound it, not the MMAs) ---
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                     "{%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                     "{%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+__device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+// 2^x by the hardware's approximation (relative error about 2^-22).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Both halves' exponents all ones, per half: NaN or infinite.
+template <bool F16>
+__device__ __forceinline__ bool bad_half(uint32_t h) {
+    const uint32_t m = F16 ? 0x7c00u : 0x7f80u;
+    return (h & m) == m;
+}
+
+// A stage's bytes, and as many stages as keep about 64 KB in flight on an SM.
+template <int DP>
+struct few_rows {
+    static constexpr int HALF = KEYS * DP * 2;  // K or V of a stage
+    static constexpr int STAGE = 2 * HALF;
+    static constexpr int STAGES = DP == 64 ? 4 : 3;
+    static constexpr int SMEM = 1024 + STAGES * STAGE;
+};
+
+constexpr int FEW_THREADS = 160;  // four warps of products, one that copies
+
+// A block: up to 16 rows of one kv head of one sequence over one chunk of
+// keys. Warp 4 brings 64 keys a stage by TMA, page by page (K and V as
+// 64-column blocks, 128-byte swizzle); warps 0-3 take 16 keys of a stage
+// each, with a running m, l and o of their own, joined at the end.
+template <int DP, bool F16>
+__global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                    const __grid_constant__ CUtensorMap tv,
+                                                                    const __grid_constant__ attend_args A) {
+    using C = few_rows<DP>;
+    extern __shared__ uint8_t dyn[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
+    __shared__ uint64_t full[C::STAGES], empty[C::STAGES];
+    __shared__ int stop, not_finite;
+    __shared__ float m_sh[4][ROWS], l_sh[4][ROWS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seq = blockIdx.z, split = blockIdx.x;
+    const int row_tiles = gridDim.y / (A.heads / A.group);
+    const int kv_head = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
+
+    const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
+    if (!s.ok) {
+        if (threadIdx.x == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+        return;
+    }
+    const int64_t rows = (int64_t) s.n * A.group, r0 = (int64_t) tile * ROWS;
+    if (r0 >= rows) return;
+    const key_span sp = span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + ROWS, rows) - 1) / A.group));
+    // this block's keys: from the first of the span's 64-key block on, by chunks
+    const int64_t from = (int64_t) sp.lo / KEYS * KEYS + split * A.chunk;
+    const int64_t to = min((int64_t) sp.hi, from + A.chunk);
+    const int steps = to > from ? (int) ((to - from + KEYS - 1) / KEYS) : 0;
+    if (steps == 0 && split > 0) return;  // kv_combine_kernel counts the chunks as this does
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 4);
+        }
+        stop = 0;
+        not_finite = 0;
+        fence_barrier_init();
+    }
+    __syncthreads();
+
+    if (warp == 4) {
+        // boxes of min(page, 64) keys by 64 columns; a lane brings one of them
+        const int box = min(A.page_size, KEYS), boxes = KEYS / box, blocks = DP / 64;
+        const int which = lane / boxes, kb = lane % boxes;  // K's column blocks, then V's
+        const bool mine = which < 2 * blocks;
+        const int col = which % blocks * 64;
+        const bool is_v = which >= blocks;
+        auto page_of = [&](int i) {
+            const int64_t key = from + (int64_t) i * KEYS + kb * box;
+            if (!mine || i >= steps || key >= to) return (int) A.pages;  // outside the tensor: zeros
+            const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
+            if (p < 0 || p >= A.pages) {
+                atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+                return (int) A.pages;
+            }
+            return p;
+        };
+        int page = page_of(0), i = 0;
+        for (; i < steps; i++) {
+            const int st = i % C::STAGES;
+            const int next = page_of(i + 1);
+            const bool ok = i < C::STAGES ||
+                            mbar_wait_bounded(&empty[st], (i / C::STAGES - 1) & 1, (volatile int *) &stop, WAIT_LIMIT_NS);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) {
+                    stop = 1;
+                    atomicOr(A.err, ERR_TIMEOUT);
+                }
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], C::STAGE);
+            __syncwarp();
+            if (mine) {
+                const int64_t key = from + (int64_t) i * KEYS + kb * box;
+                uint8_t *dst = ring + st * C::STAGE + (is_v ? C::HALF : 0) + col / 64 * (KEYS * 128) + kb * box * 128;
+                tma_load_4d(dst, is_v ? &tv : &tk, &full[st], col, (int) (key % A.page_size), kv_head, page);
+            }
+            page = next;
+        }
+        // after a wait that ran out, the copies in flight still land
+        if (i < steps)
+            for (int k = max(0, i - C::STAGES); k < i; k++)
+                mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
+        __syncthreads();
+        return;
+    }
+
+    // this lane's two rows of the tile, and what they see
+    const int g = lane >> 2, tq = lane & 3;
+    int lo[2], hi[2];
+    const uint16_t *qp[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int64_t r = r0 + g + 8 * e;
+        lo[e] = hi[e] = 0;
+        qp[e] = nullptr;
+        if (r < rows) {
+            const int t = (int) (r / A.group);
+            lo[e] = row_lo(A, s, t);
+            hi[e] = row_hi(A, s, t);
+            qp[e] = A.q + (s.q0 + (int64_t) t) * A.ldq + (int64_t) (kv_head * A.group + r % A.group) * A.d;
+        }
+    }
+    uint32_t qf[DP / 16][4];
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ks++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int c = ks * 16 + (e >> 1) * 8 + tq * 2;
+            qf[ks][e] = qp[e & 1] && c < A.d ? *reinterpret_cast<const uint32_t *>(qp[e & 1] + c) : 0;
+        }
+    float o[DP / 8][4];
+#pragma unroll
+    for (int j = 0; j < DP / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[2] = { -INFINITY, -INFINITY }, l[2] = { 0.0f, 0.0f };
+    bool bad = false, timeout = false;
+
+    for (int i = 0; i < steps; i++) {
+        const int st = i % C::STAGES;
+        if (!mbar_wait_bounded(&full[st], (i / C::STAGES) & 1, (volatile int *) &stop, WAIT_LIMIT_NS)) {
+            timeout = true;
+        }
+        if (__any_sync(0xffffffffu, timeout)) {
+            if (lane == 0) {
+                stop = 1;
+                atomicOr(A.err, ERR_TIMEOUT);
+            }
+            timeout = true;
+            break;
+        }
+        const uint32_t kb = smem_u32(ring + st * C::STAGE), vb = kb + C::HALF;
+        const int k0 = warp * 16;  // this warp's keys of the stage
+        const int64_t key0 = from + (int64_t) i * KEYS + k0;
+        float sc[2][4] = {};
+        {
+            const int key = k0 + (lane >> 4) * 8 + (lane & 7), odd = (lane >> 3) & 1;
+            const uint32_t row = kb + key * 128;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ks++) {
+                uint32_t b[4];
+                const int unit = (ks * 2 + odd) & 7;
+                ldmatrix_x4(b, row + (ks / 4) * (KEYS * 128) + ((unit ^ (key & 7)) << 4));
+                mma16816<F16>(sc[0], qf[ks], b[0], b[1]);
+                mma16816<F16>(sc[1], qf[ks], b[2], b[3]);
+            }
+        }
+        // does every row see every key of this warp's?
+        const bool masked = key0 < sp.clo || key0 + 16 > min((int64_t) sp.chi, to) || r0 + ROWS > rows;
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int64_t key = key0 + n * 8 + tq * 2 + (e & 1);
+                    if (key < lo[e >> 1] || key >= hi[e >> 1] || key >= to) sc[n][e] = -INFINITY;
+                }
+        }
+        float f[2];
+        bool moved = false;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float mx = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx = fmaxf(m[e], mx * A.scale_log2);
+            f[e] = mx == m[e] ? 1.0f : exp2_fast(m[e] - mx);  // m = -inf: 0
+            moved |= mx != m[e];
+            m[e] = mx;
+        }
+        uint32_t p[4];
+        {
+            float ps[2][4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float base = m[e >> 1] == -INFINITY ? 0.0f : m[e >> 1];
+#pragma unroll
+                for (int n = 0; n < 2; n++) ps[n][e] = exp2_fast(__fmaf_rn(sc[n][e], A.scale_log2, -base));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                l[e] = l[e] * f[e] + ((ps[0][2 * e] + ps[0][2 * e + 1]) + (ps[1][2 * e] + ps[1][2 * e + 1]));
+            p[0] = kv_bits2<F16>(ps[0][0], ps[0][1]);
+            p[1] = kv_bits2<F16>(ps[0][2], ps[0][3]);
+            p[2] = kv_bits2<F16>(ps[1][0], ps[1][1]);
+            p[3] = kv_bits2<F16>(ps[1][2], ps[1][3]);
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int j = 0; j < DP / 8; j++) {
+                o[j][0] *= f[0];
+                o[j][1] *= f[0];
+                o[j][2] *= f[1];
+                o[j][3] *= f[1];
+            }
+        }
+        {
+            const int key = k0 + ((lane >> 3) & 1) * 8 + (lane & 7), right = lane >> 4;
+            const uint32_t row = vb + key * 128;
+#pragma unroll
+            for (int j = 0; j < DP / 8; j += 2) {
+                uint32_t b[4];
+                const int unit = (j + right) & 7;
+                ldmatrix_x4_t(b, row + (j / 8) * (KEYS * 128) + ((unit ^ (key & 7)) << 4));
+                if (masked) {
+                    // a key that not every row sees: its NaN and infinities apart (add_not_finite)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int64_t k = key0 + (e & 1) * 8 + tq * 2 + h;
+                            const uint32_t half = (b[e] >> (16 * h)) & 0xffffu;
+                            if ((k < sp.clo || k >= sp.chi || k >= to) && bad_half<F16>(half)) {
+                                b[e] &= h ? 0x0000ffffu : 0xffff0000u;
+                                bad |= k < to;
+                            }
+                        }
+                }
+                mma16816<F16>(o[j], p, b[0], b[1]);
+                mma16816<F16>(o[j + 1], p, b[2], b[3]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    if (__any_sync(0xffffffffu, bad) && lane == 0) not_finite = 1;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+    // every stage has been read: the ring holds the four warps' o now
+    __syncthreads();
+    constexpr int LD = DP + 4;
+    float *os = reinterpret_cast<float *>(ring);
+    static_assert(4 * ROWS * LD * 4 <= C::STAGES * C::STAGE, "the joined rows fit the ring");
+#pragma unroll
+    for (int j = 0; j < DP / 8; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            *reinterpret_cast<float2 *>(os + (warp * ROWS + g + 8 * e) * LD + j * 8 + tq * 2) =
+                make_float2(o[j][2 * e], o[j][2 * e + 1]);
+    if (tq == 0)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            m_sh[warp][g + 8 * e] = m[e];
+            l_sh[warp][g + 8 * e] = l[e];
+        }
+    named_barrier(1, 128);
+    if (stop) return;  // a wait ran out: the rows stay as they were
+    const int row = threadIdx.x >> 3;
+    const int64_t r = r0 + row;
+    if (r >= rows) return;
+    float mx = -INFINITY, w[4], sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) mx = fmaxf(mx, m_sh[k][row]);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        w[k] = m_sh[k][row] == -INFINITY ? 0.0f : exp2_fast(m_sh[k][row] - mx);
+        sum += w[k] * l_sh[k][row];
+    }
+    const int t = (int) (r / A.group), head = kv_head * A.group + (int) (r % A.group);
+    const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
+    const float inv = A.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < DP / 64; i++) {
+        const int c = (threadIdx.x & 7) * 8 + 64 * i;
+        if (c >= A.d) break;
+        float x[8] = {};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(os[(k * ROWS + row) * LD + c + e], w[k], x[e]);
+        if (not_finite) {
+            const int a = (int) max((int64_t) row_lo(A, s, t), from), z = (int) min((int64_t) row_hi(A, s, t), to);
+            add_not_finite<F16>(A, seq, kv_head, c, a, min(z, sp.clo), x);
+            add_not_finite<F16>(A, seq, kv_head, c, max(a, max(sp.chi, sp.clo)), z, x);
+        }
+        if (A.splits > 1) {
+            float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c);
+            dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+            dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= inv;
+            store8<F16>(A, tok, head, c, x);
+        }
+    }
+    if (A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
+}
+
+// The chunks' parts of each row joined in order: the weights 2^(m_i - m) once
+// per row and thread, then eight columns a thread.
+template <int DP, bool F16>
+__global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__ attend_args A, int tile_rows) {
+    constexpr int PER_ROW = DP / 8, ROWS_B = 128 / PER_ROW;
+    const int seq = blockIdx.z, kv_head = blockIdx.y;
+    const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
+    if (!s.ok) return;
+    const int64_t rows = (int64_t) s.n * A.group;
+    const int64_t r = (int64_t) blockIdx.x * ROWS_B + threadIdx.x / PER_ROW;
+    const int c = threadIdx.x % PER_ROW * 8;
+    if (r >= rows || c >= A.d) return;
+    // the chunks of the row's tile, counted as its blocks counted them
+    const int64_t r0 = r / tile_rows * tile_rows;
+    const key_span sp =
+        span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + tile_rows, rows) - 1) / A.group));
+    const int64_t span = sp.hi - (int64_t) sp.lo / KEYS * KEYS;
+    const int n = span > 0 ? (int) ((span + A.chunk - 1) / A.chunk) : 1;
+    const int t = (int) (r / A.group), head = kv_head * A.group + (int) (r % A.group);
+    const int64_t tok = s.q0 + (int64_t) t, stride = A.b.T * A.heads, slot = tok * A.heads + head;
+    float mx = -INFINITY;
+    for (int i = 0; i < n; i++) mx = fmaxf(mx, A.ml[i * stride + slot].x);
+    float sum = 0.0f, x[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < n; i++) {
+        const float2 ml = A.ml[i * stride + slot];
+        const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mx);
+        const float4 *p = reinterpret_cast<const float4 *>(A.part + (i * stride + slot) * DP + c);
+        const float4 a = p[0], b = p[1];
+        sum += w * ml.y;
+        const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(v[e], w, x[e]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] *= inv;
+    store8<F16>(A, tok, head, c, x);
+}
+
+// --- host ------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// One layer's pool as (value, token of a page, kv head, page), in boxes of 64
+// values by min(page, 64) tokens. Columns past d and pages past the pool read
+// zeros.
+bool pool_tmap(CUtensorMap *m, const zest_kv_cache *kv, const void *base) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    // a dimension of one entry is never stepped over: any valid stride does
+    const int64_t hs = kv->kv_heads > 1 ? kv->head_stride : 8 * 32, ps = kv->pages > 1 ? kv->page_stride : 8 * 32;
+    cuuint64_t dims[4] = { (cuuint64_t) kv->d, (cuuint64_t) kv->page_size, (cuuint64_t) kv->kv_heads,
+                           (cuuint64_t) kv->pages };
+    cuuint64_t strides[3] = { (cuuint64_t) kv->token_stride * 2, (cuuint64_t) hs * 2, (cuuint64_t) ps * 2 };
+    cuuint32_t box[4] = { 64, (cuuint32_t) std::min(kv->page_size, KEYS), 1, 1 };
+    cuuint32_t estr[4] = { 1, 1, 1, 1 };
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How a call runs: its row tiles, and the chunks its keys are cut into.
+struct attend_plan {
+    int dp, tile_rows, splits;
+    int64_t row_tiles, chunk, ws_ml, ws_part;
+};
+
+// The keys are cut so that the blocks fill the GPU: one batch of resident
+// blocks where every sequence is as long as the next (one sequence), about
+// four where lengths differ, for balance; never below 256 keys a chunk.
+attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
+    attend_plan p;
+    p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
+    const int64_t group = at->heads / kv->kv_heads;
+    p.tile_rows = ROWS;
+    p.row_tiles = std::max<int64_t>(1, up(b->max_q * group, p.tile_rows));
+    const int64_t units = std::max<int64_t>(1, b->n_seqs * (int64_t) kv->kv_heads * p.row_tiles);
+    const int64_t per_sm = p.dp == 64 ? 3 : p.dp == 128 ? 2 : 1;
+    int64_t span = b->max_kv;
+    if (at->causal && at->window)  // which may start inside a block of keys
+        span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
+    const int64_t want = 148 * per_sm * (b->n_seqs > 1 ? 4 : 1);
+    const int64_t splits = std::max<int64_t>(1, want / units);
+    p.chunk = std::max<int64_t>(256, up(up(span, splits), KEYS) * KEYS);
+    p.splits = (int) std::max<int64_t>(1, up(span, p.chunk));
+    p.ws_ml = p.ws_part = 0;
+    if (p.splits > 1) {
+        p.ws_ml = up((int64_t) p.splits * b->T * at->heads * 8, 256) * 256;
+        p.ws_part = (int64_t) p.splits * b->T * at->heads * p.dp * 4;
+    }
+    return p;
+}
+
+const char *attend_fault(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
+    if (!at) return "nothing to attend with";
+    if (at->heads < 1 || at->heads % kv->kv_heads || at->heads / kv->kv_heads > 128)
+        return "heads are a multiple of the kv heads, at most 128 times";
+    if (!(at->scale > 0.0f) || std::isinf(at->scale)) return "scale is not positive";
+    if (at->window < 0 || (at->window > 0 && !at->causal)) return "a window is positive and causal";
+    if (up(b->max_q * (at->heads / kv->kv_heads), ROWS) * kv->kv_heads > 65535)
+        return "too many new tokens of one sequence";
+    return nullptr;
+}
+
+template <int DP, bool F16>
+int launch_few(const CUtensorMap &tk, const CUtensorMap &tv, const attend_args &a, const attend_plan &p, int kv_heads,
+               cudaStream_t st) {
+    using C = few_rows<DP>;
+    // per device: set with each device's first launch
+    static uint64_t ready = 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return set_error("zest_kv_attend: no CUDA device");
+    if (dev >= 64 || !(__atomic_load_n(&ready, __ATOMIC_RELAXED) >> dev & 1)) {
+        if (cudaFuncSetAttribute(kv_attend_few_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 C::SMEM) != cudaSuccess)
+            return check_launch("zest_kv_attend");
+        if (dev < 64) __atomic_fetch_or(&ready, 1ull << dev, __ATOMIC_RELAXED);
+    }
+    const dim3 grid(p.splits, (unsigned) (p.row_tiles * kv_heads), a.b.n_seqs);
+    kv_attend_few_kernel<DP, F16><<<grid, FEW_THREADS, C::SMEM, st>>>(tk, tv, a);
+    if (check_launch("zest_kv_attend")) return -1;
+    if (p.splits == 1) return 0;
+    const int rows_b = 128 / (DP / 8);
+    const dim3 cg((unsigned) up(a.b.max_q * a.group, rows_b), kv_heads, a.b.n_seqs);
+    kv_combine_kernel<DP, F16><<<cg, 128, 0, st>>>(a, p.tile_rows);
+    return check_launch("zest_kv_attend");
+}
+
+}  // namespace
+
+}  // namespace zest
+
+using namespace zest;
+
+extern "C" {
+
+int64_t zest_kv_attend_workspace(const zest_kv_cache *kv, const zest_kv_batch *batch, const zest_kv_attn *at) {
+    const char *call = "zest_kv_attend_workspace";
+    if (const char *why = kv_cache_fault(kv, 0)) return kv_refuse(call, why);
+    if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
+    if (const char *why = attend_fault(kv, batch, at)) return kv_refuse(call, why);
+    const attend_plan p = plan_attend(kv, batch, at);
+    return p.ws_ml + p.ws_part;
+}
+
+int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *batch, const zest_kv_attn *at,
+                   void *workspace, size_t workspace_bytes, unsigned *err, void *stream) {
+    const char *call = "zest_kv_attend";
+    if (const char *why = kv_cache_fault(kv, layer)) return kv_refuse(call, why);
+    if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
+    if (const char *why = attend_fault(kv, batch, at)) return kv_refuse(call, why);
+    if (!err) return kv_refuse(call, "no device error word");
+    const int64_t wide = (int64_t) at->heads * kv->d;
+    auto rows = [&](const void *p, int64_t ld, int64_t unit) { return ld >= wide && ld % unit == 0 && !((uintptr_t) p & 15); };
+    if (!at->q || !rows(at->q, at->ldq, 8)) return kv_refuse(call, "q rows cover the heads and are 16-byte aligned");
+    if (!at->out && !at->y && !at->a_next) return kv_refuse(call, "no output");
+    if ((at->out && !rows(at->out, at->ldo, 8)) || (at->y && !rows(at->y, at->ldy, 4)) ||
+        (at->a_next && !rows(at->a_next, at->lda, 8)))
+        return kv_refuse(call, "output rows cover the heads and are 16-byte aligned");
+    const attend_plan p = plan_attend(kv, batch, at);
+    const int64_t need = p.ws_ml + p.ws_part;
+    if (need > 0 && (!workspace || ((uintptr_t) workspace & 15) || (int64_t) workspace_bytes < need))
+        return kv_refuse(call, "the workspace is smaller than zest_kv_attend_workspace says, or not 16-byte aligned");
+    if (batch->T == 0 || batch->n_seqs == 0 || batch->max_q == 0) return 0;
+    const int64_t off = kv->layers > 1 ? layer * kv->layer_stride : 0;
+    CUtensorMap tk, tv;
+    if (!pool_tmap(&tk, kv, (const uint16_t *) kv->k + off) || !pool_tmap(&tv, kv, (const uint16_t *) kv->v + off))
+        return kv_refuse(call, "the pools' strides make no tensor map");
+    attend_args a;
+    a.b = *batch;
+    a.q = (const uint16_t *) at->q;
+    a.ldq = at->ldq;
+    a.pages = kv->pages;
+    a.v = (const uint16_t *) kv->v + off;
+    a.page_stride = kv->pages > 1 ? kv->page_stride : 0;
+    a.token_stride = kv->token_stride;
+    a.head_stride = kv->kv_heads > 1 ? kv->head_stride : 0;
+    a.heads = at->heads;
+    a.group = at->heads / kv->kv_heads;
+    a.d = kv->d;
+    a.page_size = kv->page_size;
+    a.causal = at->causal != 0;
+    a.window = at->window;
+    a.scale_log2 = at->scale * 1.44269504088896340736f;
+    a.out = (uint16_t *) at->out;
+    a.ldo = at->ldo;
+    a.y = at->y;
+    a.ldy = at->ldy;
+    a.a_next = at->a_next;
+    a.lda = at->lda;
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    a.ml = (float2 *) workspace;
+    a.part = (float *) ((uint8_t *) workspace + p.ws_ml);
+    a.err = err;
+    cudaStream_t st = (cudaStream_t) stream;
+    const bool f16 = kv->type == ZEST_TYPE_F16;
+    switch (p.dp) {
+        case 64: return f16 ? launch_few<64, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<64, false>(tk, tv, a, p, kv->kv_heads, st);
+        case 128: return f16 ? launch_few<128, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<128, false>(tk, tv, a, p, kv->kv_heads, st);
+        default: return f16 ? launch_few<256, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<256, false>(tk, tv, a, p, kv->kv_heads, st);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,690 @@
+// The paged key/value cache's own operations: a step's keys and values
+// written to their pages (zest_kv_append), and the bookkeeping between steps
+// (zest_kv_grow, _fork, _free, _compact), all on the device: a serving loop
+// needs no copy of the tables on the host.
+#include "zest_kv.cuh"
+
+#include <algorithm>
+#include <cstdio>
+
+namespace zest {
+
+int kv_refuse(const char *call, const char *why) {
+    char msg[256];
+    snprintf(msg, sizeof msg, "%s: %s", call, why);
+    return set_error(msg);
+}
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+
+constexpr int AP_WARPS = 8, AP_MAX_D = 256;
+
+// The last sequence whose first row is t or before it, by a search that 32
+// lanes make together: each step cuts the range by 32 with one load. -1: none.
+__device__ __forceinline__ int kv_find_seq(const zest_kv_batch &b, int t, int lane) {
+    int lo = 0, hi = b.n_seqs;
+    while (true) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, at < hi && b.q_start[at] <= t);
+        if (!m) return -1;  // only ever in the first step: later ranges start at a sequence that holds
+        lo += (31 - __clz(m)) * step;
+        hi = min(hi, lo + step);
+        if (step == 1) return lo;
+    }
+}
+
+struct append_args {
+    zest_kv_batch b;
+    zest_kv_new in;
+    uint16_t *k, *v;  // this layer
+    int64_t page_stride, token_stride, head_stride, pages;
+    int page_size, kv_heads, d, q_heads;
+    unsigned *err;
+};
+
+// A warp takes every (head row) of its share of a token: 4 values a lane and
+// 128 columns, so a head of 128 is one 16-byte load a lane. The row's sum of
+// squares by an xor tree, the norm and weight, the rotation with the partner
+// values read back from shared memory (NeoX pairs lie n_dims / 2 apart),
+// one rounding, 8-byte stores. Sums and rotations in f32 with explicitly
+// rounded products, as zest_norm_rope's.
+template <bool F16>
+__global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_constant__ append_args A) {
+    __shared__ float4 buf[AP_WARPS][AP_MAX_D / 4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = A.d;
+    float *row = reinterpret_cast<float *>(buf[warp]);
+    const int rows = A.q_heads + 2 * A.kv_heads;
+    const bool neox = A.in.mode == ZEST_ROPE_NEOX;
+    const int n_dims = A.in.rope ? A.in.n_dims : 0, half = n_dims / 2;
+    for (int64_t t = blockIdx.x; t < A.b.T; t += gridDim.x) {
+        const int s = kv_find_seq(A.b, (int) t, lane);
+        if (s < 0) continue;
+        const kv_seq sq = kv_seq_of(A.b, A.page_size, s);
+        const int64_t i = t - sq.q0;
+        if (!sq.ok) {
+            if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+            continue;
+        }
+        if (i >= sq.n) continue;  // behind the last sequence
+        const int64_t pos = (int64_t) sq.kv - sq.n + i;
+        int64_t at = -1;  // the token's place in the pools, in values
+        if (pos < 0) {
+            if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+        } else {
+            const int64_t page = A.b.table[s * A.b.table_stride + pos / A.page_size];
+            if (page < 0 || page >= A.pages) {
+                if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+            } else {
+                at = page * A.page_stride + pos % A.page_size * A.token_stride;
+            }
+        }
+        for (int r = blockIdx.y * AP_WARPS + warp; r < rows; r += gridDim.y * AP_WARPS) {
+            const bool is_q = r < A.q_heads, is_k = !is_q && r < A.q_heads + A.kv_heads;
+            if (!is_q && at < 0) break;
+            const float *x;
+            uint16_t *dst;
+            if (is_q) {
+                x = A.in.q + t * A.in.ldq + (int64_t) r * d;
+                dst = reinterpret_cast<uint16_t *>(A.in.q_out) + t * A.in.ldqo + (int64_t) r * d;
+            } else if (is_k) {
+                const int h = r - A.q_heads;
+                x = A.in.k + t * A.in.ldk + (int64_t) h * d;
+                dst = A.k + at + h * A.head_stride;
+            } else {
+                const int h = r - A.q_heads - A.kv_heads;
+                x = A.in.v + t * A.in.ldv + (int64_t) h * d;
+                dst = A.v + at + h * A.head_stride;
+            }
+            float v[2][4];
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int j = 4 * lane + 128 * c;
+                const float4 f = j < d ? *reinterpret_cast<const float4 *>(x + j) : make_float4(0, 0, 0, 0);
+                v[c][0] = f.x, v[c][1] = f.y, v[c][2] = f.z, v[c][3] = f.w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) ss = __fmaf_rn(v[c][e], v[c][e], ss);
+            }
+            if (is_q || is_k) {
+                if (A.in.eps >= 0.0f) {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float sc = 1.0f / sqrtf(ss / (float) d + A.in.eps);
+                    const float *w = is_q ? A.in.q_norm : A.in.k_norm;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int j = 4 * lane + 128 * c;
+                        const float4 f = w && j < d ? *reinterpret_cast<const float4 *>(w + j) : make_float4(1, 1, 1, 1);
+                        const float wv[4] = { f.x, f.y, f.z, f.w };
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[c][e] = __fmul_rn(__fmul_rn(v[c][e], sc), wv[e]);
+                    }
+                }
+                if (n_dims) {
+                    const float *cs = A.in.rope + t * n_dims;
+                    if (neox) {
+                        __syncwarp();
+#pragma unroll
+                        for (int c = 0; c < 2; c++)
+                            if (4 * lane + 128 * c < d)
+                                buf[warp][lane + 32 * c] = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float o[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int j = 4 * lane + 128 * c + e;
+                            o[e] = v[c][e];
+                            if (j < n_dims && j < d) {
+                                const bool first = neox ? j < half : (j & 1) == 0;
+                                const int p = neox ? (first ? j : j - half) : j >> 1;
+                                const float other = neox ? row[first ? j + half : j - half] : v[c][e ^ 1];
+                                const float x0 = first ? v[c][e] : other, x1 = first ? other : v[c][e];
+                                const float co = cs[2 * p], si = cs[2 * p + 1];
+                                o[e] = first ? __fsub_rn(__fmul_rn(x0, co), __fmul_rn(x1, si))
+                                             : __fadd_rn(__fmul_rn(x0, si), __fmul_rn(x1, co));
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[c][e] = o[e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int j = 4 * lane + 128 * c;
+                if (j < d) {
+                    uint2 w;
+                    w.x = kv_bits<F16>(v[c][0]) | (uint32_t) kv_bits<F16>(v[c][1]) << 16;
+                    w.y = kv_bits<F16>(v[c][2]) | (uint32_t) kv_bits<F16>(v[c][3]) << 16;
+                    *reinterpret_cast<uint2 *>(dst + j) = w;
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// pages
+// ---------------------------------------------------------------------------
+
+// The tables' part of each page operation is one block's work: ranks of free
+// and live pages by block scans over refs, 8 pages a thread and step, so a
+// pool of 8,192 pages is one step. Bound by latency, not bytes: the scan of
+// 13,000 counts and the rows of 32 sequences take a few microseconds.
+constexpr int PG_THREADS = 1024, PG_PER = 8, PG_STEP = PG_THREADS * PG_PER;
+
+struct pages_shared {
+    int warp[32];
+    int total;
+    int bad;
+    int off[ZEST_KV_MAX_SEQS + 1];   // before each sequence: pages taken by the earlier ones
+    int held[ZEST_KV_MAX_SEQS];      // its pages before the call (grow); its fresh page (fork)
+    int who[ZEST_KV_MAX_SEQS];
+};
+
+// This thread's exclusive prefix over the block of v; total: all of it.
+__device__ __forceinline__ int block_scan(int v, pages_shared &sh, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) sh.warp[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int w = sh.warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        sh.warp[lane] = w;
+    }
+    __syncthreads();
+    const int before = x - v + (warp ? sh.warp[warp - 1] : 0);
+    total = sh.warp[31];
+    __syncthreads();
+    return before;
+}
+
+// The free (or, live = true, held) pages in [from, pages) in rising order:
+// f(rank, page, its count) for each with rank < limit. Every thread calls it;
+// returns how many there are up to the step where the limit was passed.
+template <typename F>
+__device__ __forceinline__ int64_t each_page(const int32_t *refs, int64_t from, int64_t pages, bool live,
+                                             int64_t limit, pages_shared &sh, F f) {
+    int64_t seen = 0;
+    for (int64_t base = from; base < pages && seen < limit; base += PG_STEP) {
+        const int64_t p0 = base + (int64_t) threadIdx.x * PG_PER;
+        int r[PG_PER], mine = 0;
+#pragma unroll
+        for (int i = 0; i < PG_PER; i++) {
+            r[i] = p0 + i < pages ? refs[p0 + i] : (live ? 0 : 1);
+            mine += (r[i] != 0) == live;
+        }
+        int total;
+        int64_t rank = seen + block_scan(mine, sh, total);
+#pragma unroll
+        for (int i = 0; i < PG_PER; i++)
+            if ((r[i] != 0) == live) {
+                if (rank < limit) f(rank, p0 + i, r[i]);
+                rank++;
+            }
+        seen += total;
+    }
+    return seen;
+}
+
+struct pages_args {
+    zest_kv_tables in, out;
+    int64_t pages;
+    int page_size, n;
+    const int32_t *a, *b;  // seq and add; src and dst
+    int32_t *ws;           // moves: count, then (from, to) pairs; compact: [1 + 2 * pages] then the map
+    unsigned *err;
+};
+
+// out := in, by one block (in and out may be the same).
+__device__ void copy_tables(const pages_args &A) {
+    if (A.in.refs != A.out.refs)
+        for (int64_t i = threadIdx.x; i < A.pages; i += blockDim.x) A.out.refs[i] = A.in.refs[i];
+    if (A.in.table != A.out.table)
+        for (int64_t i = threadIdx.x; i < A.in.seqs * A.in.table_stride; i += blockDim.x)
+            A.out.table[i] = A.in.table[i];
+    if (A.in.len != A.out.len)
+        for (int64_t i = threadIdx.x; i < A.in.seqs; i += blockDim.x) A.out.len[i] = A.in.len[i];
+    __syncthreads();
+}
+
+// The same by many blocks, ahead of the operation's own, for tables that one
+// block would take longer over than a launch costs (above 64 Ki entries).
+__global__ void __launch_bounds__(256) kv_copy_tables_kernel(const __grid_constant__ pages_args A) {
+    const int64_t at = blockIdx.x * (int64_t) blockDim.x + threadIdx.x, step = (int64_t) gridDim.x * blockDim.x;
+    if (A.in.refs != A.out.refs)
+        for (int64_t i = at; i < A.pages; i += step) A.out.refs[i] = A.in.refs[i];
+    if (A.in.table != A.out.table)
+        for (int64_t i = at; i < A.in.seqs * A.in.table_stride; i += step) A.out.table[i] = A.in.table[i];
+    if (A.in.len != A.out.len)
+        for (int64_t i = at; i < A.in.seqs; i += step) A.out.len[i] = A.in.len[i];
+}
+
+// Raises sh.bad (bits) where a sequence number is out of range or, with
+// `once`, appears twice among the first n of sh.who.
+__device__ void check_who(const pages_args &A, const int32_t *who, bool once, pages_shared &sh) {
+    if (threadIdx.x == 0) sh.bad = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.n; i += blockDim.x) sh.who[i] = who[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < A.n; i += blockDim.x) {
+        bool bad = sh.who[i] < 0 || sh.who[i] >= A.in.seqs;
+        if (once)
+            for (int j = 0; j < i && !bad; j++) bad = sh.who[j] == sh.who[i];
+        if (bad) atomicOr(&sh.bad, (int) ZEST_ERR_BAD_SEQ);
+    }
+    __syncthreads();
+}
+
+// The bits found so far; true: stop, out stays what copy_tables made it.
+__device__ __forceinline__ bool give_up(const pages_args &A, pages_shared &sh) {
+    __syncthreads();
+    const int bad = sh.bad;
+    __syncthreads();
+    if (bad && threadIdx.x == 0) {
+        atomicOr(A.err, (unsigned) bad);
+        if (A.ws) A.ws[0] = 0;
+    }
+    return bad != 0;
+}
+
+__global__ void __launch_bounds__(PG_THREADS) kv_grow_kernel(const __grid_constant__ pages_args A) {
+    __shared__ pages_shared sh;
+    copy_tables(A);
+    check_who(A, A.a, true, sh);
+    if (give_up(A, sh)) return;
+    int need = 0, now = 0;
+    const int i = threadIdx.x;
+    if (i < A.n) {
+        const int64_t len = A.out.len[sh.who[i]], add = A.b[i], ps = A.page_size;
+        const int64_t held = (len + ps - 1) / ps, want = (len + add + ps - 1) / ps;
+        if (len < 0 || add < 0 || len + add > 0x7fffffff || want > A.in.table_stride)
+            atomicOr(&sh.bad, (int) ZEST_ERR_BAD_SEQ);
+        else {
+            need = (int) (want - held);
+            now = (int) (len + add);
+            sh.held[i] = (int) held;
+        }
+    }
+    if (give_up(A, sh)) return;
+    // a thousand sequences of at most 2^31 tokens: the sum of needs may pass 32 bits, so it is bounded first
+    int total;
+    const int before = block_scan(min(need, (1 << 20)), sh, total);
+    const bool huge = __syncthreads_or(need > (1 << 20));
+    if (i < A.n) sh.off[i] = before;
+    if (threadIdx.x == 0) sh.off[A.n] = total;
+    __syncthreads();
+    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t, int) {});
+    if (threadIdx.x == 0 && (huge || there < total)) atomicOr(&sh.bad, (int) ZEST_ERR_NO_PAGES);
+    if (give_up(A, sh)) return;
+    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page, int) {
+        int lo = 0, hi = A.n;  // the sequence with off[lo] <= rank < off[lo + 1]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (sh.off[mid] <= rank) lo = mid;
+            else hi = mid;
+        }
+        A.out.table[sh.who[lo] * A.out.table_stride + sh.held[lo] + rank - sh.off[lo]] = (int32_t) page;
+        A.out.refs[page] = 1;
+    });
+    if (i < A.n) A.out.len[sh.who[i]] = now;
+}
+
+__global__ void __launch_bounds__(PG_THREADS) kv_free_kernel(const __grid_constant__ pages_args A) {
+    __shared__ pages_shared sh;
+    copy_tables(A);
+    check_who(A, A.a, false, sh);
+    if (give_up(A, sh)) return;
+    const int64_t w = A.out.table_stride, n = A.n * w;
+    for (int64_t e = threadIdx.x; e < n; e += blockDim.x) {
+        // taken out by exchange: of a sequence named twice, one finds the page
+        const int page = atomicExch(&A.out.table[sh.who[e / w] * w + e % w], -1);
+        if (page < 0) continue;
+        if (page >= A.pages || atomicSub(&A.out.refs[page], 1) <= 0) {
+            if (page < A.pages) atomicAdd(&A.out.refs[page], 1);
+            atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+        }
+    }
+    for (int i = threadIdx.x; i < A.n; i += blockDim.x) A.out.len[sh.who[i]] = 0;
+}
+
+__global__ void __launch_bounds__(PG_THREADS) kv_fork_kernel(const __grid_constant__ pages_args A) {
+    __shared__ pages_shared sh;
+    copy_tables(A);
+    check_who(A, A.b, true, sh);  // dst, left in sh.who
+    const int i = threadIdx.x, ps = A.page_size;
+    int len = 0, src = 0, part = 0;
+    if (i < A.n && !sh.bad) {
+        src = A.a[i];
+        const bool in_range = src >= 0 && src < A.in.seqs;
+        len = in_range ? A.out.len[src] : 0;
+        if (!in_range || len < 0 || (len + (int64_t) ps - 1) / ps > A.in.table_stride || A.out.len[sh.who[i]] != 0) {
+            atomicOr(&sh.bad, (int) ZEST_ERR_BAD_SEQ);
+            len = 0;
+        }
+        part = len % ps != 0;
+    }
+    if (give_up(A, sh)) return;
+    int total;
+    const int before = block_scan(part, sh, total);
+    if (i < A.n) sh.off[i] = before;
+    if (threadIdx.x == 0) sh.off[A.n] = total;
+    __syncthreads();
+    // every page that will be shared or copied has to be one; a warp a pair
+    const int64_t w = A.out.table_stride;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int k = warp; k < A.n; k += PG_THREADS / 32) {
+        const int64_t from = A.a[k], pages = (A.out.len[from] + (int64_t) ps - 1) / ps;
+        for (int64_t j = lane; j < pages; j += 32) {
+            const int page = A.out.table[from * w + j];
+            if (page < 0 || page >= A.pages) atomicOr(&sh.bad, (int) ZEST_ERR_BAD_PAGE);
+        }
+    }
+    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t, int) {});
+    if (threadIdx.x == 0 && there < total) atomicOr(&sh.bad, (int) ZEST_ERR_NO_PAGES);
+    if (give_up(A, sh)) return;
+    // the rank-th free page goes to the rank-th pair with a part page: by rank, then by pair
+    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page, int) {
+        sh.held[rank] = (int) page;
+    });
+    __syncthreads();
+    if (i < A.n && part) {
+        const int fresh = sh.held[sh.off[i]];
+        A.ws[1 + 2 * sh.off[i]] = A.out.table[src * w + len / ps];
+        A.ws[2 + 2 * sh.off[i]] = fresh;
+        A.out.refs[fresh] = 1;
+    }
+    if (threadIdx.x == 0) A.ws[0] = total;
+    __syncthreads();
+    for (int k = warp; k < A.n; k += PG_THREADS / 32) {
+        const int64_t from = A.a[k], to = sh.who[k], l = A.out.len[from], whole = l / ps;
+        if (from == to) continue;  // an empty sequence copied onto itself
+        for (int64_t j = lane; j < w; j += 32) {
+            int page = -1;
+            if (j < whole) {
+                page = A.out.table[from * w + j];
+                atomicAdd(&A.out.refs[page], 1);
+            } else if (j == whole && l % ps) {
+                page = sh.held[sh.off[k]];
+            }
+            A.out.table[to * w + j] = page;
+        }
+    }
+    __syncthreads();
+    if (i < A.n) A.out.len[sh.who[i]] = len;
+}
+
+// ws: count of moves, (from, to) pairs, and behind 1 + 2 * pages the new
+// number of each page. The table is rewritten by the copying kernel, whose
+// many blocks suit its size.
+__global__ void __launch_bounds__(PG_THREADS) kv_compact_kernel(const __grid_constant__ pages_args A) {
+    __shared__ pages_shared sh;
+    if (A.in.refs != A.out.refs)
+        for (int64_t i = threadIdx.x; i < A.pages; i += blockDim.x) A.out.refs[i] = A.in.refs[i];
+    if (A.in.len != A.out.len)
+        for (int64_t i = threadIdx.x; i < A.in.seqs; i += blockDim.x) A.out.len[i] = A.in.len[i];
+    int32_t *map = A.ws + 1 + 2 * A.pages;
+    const int64_t all = A.pages;
+    for (int64_t i = threadIdx.x; i < all; i += blockDim.x) map[i] = (int32_t) i;
+    __syncthreads();
+    const int64_t live = each_page(A.out.refs, 0, all, true, all, sh, [](int64_t, int64_t, int) {});
+    const int64_t holes = each_page(A.out.refs, 0, live, false, all, sh, [&](int64_t rank, int64_t page, int) {
+        A.ws[2 + 2 * rank] = (int32_t) page;
+    });
+    __syncthreads();
+    each_page(A.out.refs, live, all, true, all, sh, [&](int64_t rank, int64_t page, int count) {
+        const int to = A.ws[2 + 2 * rank];
+        A.ws[1 + 2 * rank] = (int32_t) page;
+        map[page] = to;
+        A.out.refs[to] = count;
+        A.out.refs[page] = 0;
+    });
+    if (threadIdx.x == 0) A.ws[0] = (int32_t) holes;
+}
+
+struct move_args {
+    const int32_t *ws;
+    uint16_t *pool[2];
+    int64_t layers, layer_stride, page_stride, token_stride, head_stride, pages;
+    int page_size, kv_heads, d;
+    int flat;                     // a page's values lie in one run
+    int64_t pieces;               // of a page
+    const int32_t *table_in;      // compact: its entries renumbered by the map (null: none)
+    int32_t *table_out;
+    int64_t entries;
+    unsigned *err;
+};
+
+constexpr int MV_THREADS = 256, MV_PIECE = MV_THREADS * 4;  // 16-byte vectors: 16 KB
+
+// Each move's page in each layer, K and V, in pieces of 16 KB: four 16-byte
+// loads a thread in flight before the first store. Reads and writes each
+// byte once; no page is both read and written. Bound by HBM (3.0 + 3.0 TB/s).
+__global__ void __launch_bounds__(MV_THREADS) kv_move_kernel(const __grid_constant__ move_args A) {
+    const int64_t moves = A.ws[0], units = moves * A.layers * 2 * A.pieces;
+    const int64_t vecs = (int64_t) A.page_size * A.kv_heads * (A.d / 8);
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t piece = u % A.pieces, q = u / A.pieces, kv = q & 1, r = q >> 1;
+        const int64_t layer = r % A.layers, m = r / A.layers;
+        uint16_t *pool = A.pool[kv] + layer * A.layer_stride;
+        const uint16_t *src = pool + A.ws[1 + 2 * m] * A.page_stride;
+        uint16_t *dst = pool + A.ws[2 + 2 * m] * A.page_stride;
+        uint4 x[4];
+        int64_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t v = piece * MV_PIECE + i * MV_THREADS + threadIdx.x;
+            at[i] = -1;
+            if (v < vecs) {
+                if (A.flat) {
+                    at[i] = v * 8;
+                } else {
+                    const int dv = A.d / 8, c = (int) (v % dv), h = (int) (v / dv % A.kv_heads);
+                    at[i] = v / dv / A.kv_heads * A.token_stride + h * A.head_stride + c * 8;
+                }
+                x[i] = *reinterpret_cast<const uint4 *>(src + at[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (at[i] >= 0) *reinterpret_cast<uint4 *>(dst + at[i]) = x[i];
+    }
+    if (A.table_in) {
+        const int32_t *map = A.ws + 1 + 2 * A.pages;
+        for (int64_t e = blockIdx.x * (int64_t) MV_THREADS + threadIdx.x; e < A.entries;
+             e += (int64_t) gridDim.x * MV_THREADS) {
+            const int p = A.table_in[e];
+            if (p >= A.pages) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+            A.table_out[e] = p >= 0 && p < A.pages ? map[p] : p;
+        }
+    }
+}
+
+int launch_moves(const zest_kv_cache *kv, const int32_t *ws, int64_t most, const int32_t *table_in,
+                 int32_t *table_out, int64_t entries, unsigned *err, cudaStream_t st, const char *what) {
+    move_args m;
+    m.ws = ws;
+    m.pool[0] = (uint16_t *) kv->k;
+    m.pool[1] = (uint16_t *) kv->v;
+    m.layers = kv->layers;
+    m.layer_stride = kv->layers > 1 ? kv->layer_stride : 0;
+    m.page_stride = kv->pages > 1 ? kv->page_stride : 0;
+    m.token_stride = kv->token_stride;
+    m.head_stride = kv->kv_heads > 1 ? kv->head_stride : 0;
+    m.pages = kv->pages;
+    m.page_size = kv->page_size;
+    m.kv_heads = kv->kv_heads;
+    m.d = kv->d;
+    const int64_t d = kv->d, ps = kv->page_size, kh = kv->kv_heads;
+    m.flat = (kv->token_stride == kh * d && (kh == 1 || kv->head_stride == d)) ||
+             (kv->token_stride == d && (kh == 1 || kv->head_stride == ps * d));
+    m.pieces = (ps * kh * (d / 8) + MV_PIECE - 1) / MV_PIECE;
+    m.table_in = table_in;
+    m.table_out = table_out;
+    m.entries = entries;
+    m.err = err;
+    const int64_t units = std::max<int64_t>(most * m.layers * 2 * m.pieces, (entries + MV_THREADS - 1) / MV_THREADS);
+    kv_move_kernel<<<(int) std::min<int64_t>(std::max<int64_t>(units, 1), 148 * 8), MV_THREADS, 0, st>>>(m);
+    return check_launch(what);
+}
+
+const char *tables_fault(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out) {
+    if (const char *why = kv_cache_fault(kv, 0)) return why;
+    if (!in || !out || !in->refs || !in->table || !in->len || !out->refs || !out->table || !out->len)
+        return "no tables";
+    if (in->seqs < 1 || in->seqs > 0x7fffffff || in->table_stride < 1 || in->table_stride > 0x7fffffff)
+        return "no sequences, or no room for pages";
+    if (out->seqs != in->seqs || out->table_stride != in->table_stride) return "in and out differ in size";
+    return nullptr;
+}
+
+// The checks that the operations on n named sequences share.
+const char *named_fault(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                        const int32_t *a, const int32_t *b, const unsigned *err) {
+    if (const char *why = tables_fault(kv, in, out)) return why;
+    if (n < 0 || n > ZEST_KV_MAX_SEQS) return "0 to 1024 sequences a call";
+    if (n > 0 && (!a || !b)) return "no sequence numbers";
+    if (!err) return "no device error word";
+    return nullptr;
+}
+
+pages_args args_of(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                   const int32_t *a, const int32_t *b, void *ws, unsigned *err) {
+    return { *in, *out, kv->pages, kv->page_size, n, a, b, (int32_t *) ws, err };
+}
+
+// Large tables copied by many blocks first; the operation then works in place.
+int copy_first(pages_args &a, cudaStream_t st, const char *call) {
+    const int64_t n = a.in.seqs * (a.in.table_stride + 1) + a.pages;
+    if (n <= (1 << 16) || (a.in.refs == a.out.refs && a.in.table == a.out.table && a.in.len == a.out.len)) return 0;
+    kv_copy_tables_kernel<<<(int) std::min<int64_t>((n + 1023) / 1024, 148 * 8), 256, 0, st>>>(a);
+    a.in = a.out;
+    return check_launch(call);
+}
+
+}  // namespace
+
+}  // namespace zest
+
+using namespace zest;
+
+extern "C" {
+
+int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *batch, const zest_kv_new *in,
+                   unsigned *err, void *stream) {
+    const char *call = "zest_kv_append";
+    if (const char *why = kv_cache_fault(kv, layer)) return kv_refuse(call, why);
+    if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
+    if (!in || !err) return kv_refuse(call, "no new rows, or no device error word");
+    const int64_t d = kv->d, wide = kv->kv_heads * d;
+    auto rows = [](const float *p, int64_t ld, int64_t n) { return p && ld >= n && ld % 4 == 0 && !((uintptr_t) p & 15); };
+    if (batch->T > 0 && (!rows(in->k, in->ldk, wide) || !rows(in->v, in->ldv, wide)))
+        return kv_refuse(call, "k and v rows cover the heads and are 16-byte aligned");
+    if (in->q) {
+        if (in->heads < 1 || in->heads > 65535 || !rows(in->q, in->ldq, in->heads * d) || !in->q_out ||
+            ((uintptr_t) in->q_out & 15) || in->ldqo < in->heads * d || in->ldqo % 8)
+            return kv_refuse(call, "q rows cover the heads, and q and q_out are 16-byte aligned");
+    }
+    if (in->eps != in->eps || std::isinf(in->eps)) return kv_refuse(call, "eps is not a number");
+    if (((uintptr_t) in->q_norm & 15) || ((uintptr_t) in->k_norm & 15))
+        return kv_refuse(call, "norm weights are not 16-byte aligned");
+    if (in->rope) {
+        if (in->mode != ZEST_ROPE_NORMAL && in->mode != ZEST_ROPE_NEOX) return kv_refuse(call, "unsupported rope mode");
+        if (in->n_dims <= 0 || in->n_dims % 2 || in->n_dims > d) return kv_refuse(call, "n_dims even and within d");
+    }
+    if (batch->T == 0 || batch->n_seqs == 0) return 0;
+    append_args a;
+    a.b = *batch;
+    a.in = *in;
+    const int64_t at = kv->layers > 1 ? layer * kv->layer_stride : 0;
+    a.k = (uint16_t *) kv->k + at;
+    a.v = (uint16_t *) kv->v + at;
+    a.page_stride = kv->pages > 1 ? kv->page_stride : 0;
+    a.token_stride = kv->token_stride;
+    a.head_stride = kv->kv_heads > 1 ? kv->head_stride : 0;
+    a.pages = kv->pages;
+    a.page_size = kv->page_size;
+    a.kv_heads = kv->kv_heads;
+    a.d = kv->d;
+    a.q_heads = in->q ? in->heads : 0;
+    a.err = err;
+    // few tokens: a token's heads over several blocks, so that a step of a
+    // few rows is one row a warp; many: a block a token, which finds its
+    // sequence and page once
+    const int groups = (a.q_heads + 2 * a.kv_heads + AP_WARPS - 1) / AP_WARPS;
+    const int gx = (int) std::min<int64_t>(batch->T, 148 * 8);
+    const int gy = (int) std::min<int64_t>(groups, std::max<int64_t>(1, 148 * 8 / gx));
+    if (kv->type == ZEST_TYPE_F16)
+        kv_append_kernel<true><<<dim3(gx, gy), AP_WARPS * 32, 0, (cudaStream_t) stream>>>(a);
+    else kv_append_kernel<false><<<dim3(gx, gy), AP_WARPS * 32, 0, (cudaStream_t) stream>>>(a);
+    return check_launch(call);
+}
+
+int64_t zest_kv_pages_workspace(const zest_kv_cache *kv) {
+    if (const char *why = kv_cache_fault(kv, 0)) return kv_refuse("zest_kv_pages_workspace", why);
+    // fork: at most a move a pair; compact: at most half the pages move, and the map
+    return 4 * (std::max<int64_t>(1 + 3 * kv->pages, 1 + 2 * ZEST_KV_MAX_SEQS) + 3);
+}
+
+int zest_kv_grow(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *seq, const int32_t *add, unsigned *err, void *stream) {
+    if (const char *why = named_fault(kv, in, out, n, seq, add, err)) return kv_refuse("zest_kv_grow", why);
+    pages_args a = args_of(kv, in, out, n, seq, add, nullptr, err);
+    if (copy_first(a, (cudaStream_t) stream, "zest_kv_grow")) return -1;
+    kv_grow_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(a);
+    return check_launch("zest_kv_grow");
+}
+
+int zest_kv_free(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *seq, unsigned *err, void *stream) {
+    if (const char *why = named_fault(kv, in, out, n, seq, seq, err)) return kv_refuse("zest_kv_free", why);
+    pages_args a = args_of(kv, in, out, n, seq, seq, nullptr, err);
+    if (copy_first(a, (cudaStream_t) stream, "zest_kv_free")) return -1;
+    kv_free_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(a);
+    return check_launch("zest_kv_free");
+}
+
+int zest_kv_fork(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *src, const int32_t *dst, void *workspace, unsigned *err, void *stream) {
+    if (const char *why = named_fault(kv, in, out, n, src, dst, err)) return kv_refuse("zest_kv_fork", why);
+    if (!workspace || ((uintptr_t) workspace & 15)) return kv_refuse("zest_kv_fork", "no 16-byte aligned workspace");
+    pages_args a = args_of(kv, in, out, n, src, dst, workspace, err);
+    if (copy_first(a, (cudaStream_t) stream, "zest_kv_fork")) return -1;
+    kv_fork_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(a);
+    if (check_launch("zest_kv_fork")) return -1;
+    if (n == 0) return 0;
+    return launch_moves(kv, (const int32_t *) workspace, n, nullptr, nullptr, 0, err, (cudaStream_t) stream,
+                        "zest_kv_fork");
+}
+
+int zest_kv_compact(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, void *workspace,
+                    unsigned *err, void *stream) {
+    if (const char *why = tables_fault(kv, in, out)) return kv_refuse("zest_kv_compact", why);
+    if (!err) return kv_refuse("zest_kv_compact", "no device error word");
+    if (!workspace || ((uintptr_t) workspace & 15)) return kv_refuse("zest_kv_compact", "no 16-byte aligned workspace");
+    kv_compact_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(
+        args_of(kv, in, out, 0, nullptr, nullptr, workspace, err));
+    if (check_launch("zest_kv_compact")) return -1;
+    return launch_moves(kv, (const int32_t *) workspace, kv->pages / 2, in->table, out->table,
+                        in->seqs * in->table_stride, err, (cudaStream_t) stream, "zest_kv_compact");
+}
+
+}  // extern "C"

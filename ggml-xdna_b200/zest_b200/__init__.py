@@ -17,8 +17,10 @@ LIB_PATH = PKG_DIR / "libzest_b200.so"
 BACKEND_PATH = PKG_DIR / "libggml-zest.so"
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_IQ3_S = 0, 1, 8, 12, 14, 21
+TYPE_BF16 = 30  # with TYPE_F16: the types of a key/value cache
 MODE_F32, MODE_BF16, MODE_SWIGLU = 0, 1, 2
-ERR_NOT_FINITE, ERR_TIMEOUT = 1, 2
+ERR_NOT_FINITE, ERR_TIMEOUT, ERR_BAD_PAGE, ERR_BAD_SEQ, ERR_NO_PAGES = 1, 2, 4, 8, 16
+KV_MAX_SEQS = 1024  # ZEST_KV_MAX_SEQS: sequences of one page operation
 GLU_REGLU, GLU_GEGLU, GLU_SWIGLU, GLU_GEGLU_ERF, GLU_GEGLU_QUICK = 0, 1, 2, 4, 5
 ROPE_NORMAL, ROPE_NEOX = 0, 2
 BLOCK_BYTES = 9
@@ -60,6 +62,38 @@ class MmOut(ctypes.Structure):
     _fields_ = [("y", _vp), ("residual", _vp), ("a_next", _vp)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    """zest_kv_cache: the pools of a paged key/value cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", _int), ("page_size", _int), ("kv_heads", _int), ("d", _int),
+                ("layers", _i64), ("pages", _i64), ("layer_stride", _i64), ("page_stride", _i64),
+                ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class KvBatchDesc(ctypes.Structure):
+    """zest_kv_batch: a step's sequences."""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("table", _vp), ("table_stride", _i64), ("T", _i64),
+                ("max_q", _i64), ("max_kv", _i64), ("n_seqs", _int)]
+
+
+class KvNew(ctypes.Structure):
+    """zest_kv_new: what zest_kv_append takes of a step."""
+    _fields_ = [("k", _vp), ("v", _vp), ("ldk", _i64), ("ldv", _i64), ("q", _vp), ("ldq", _i64), ("q_out", _vp),
+                ("ldqo", _i64), ("heads", _int), ("eps", ctypes.c_float), ("q_norm", _vp), ("k_norm", _vp),
+                ("rope", _vp), ("n_dims", _int), ("mode", _int)]
+
+
+class KvAttn(ctypes.Structure):
+    """zest_kv_attn: what zest_kv_attend reads and writes."""
+    _fields_ = [("q", _vp), ("ldq", _i64), ("heads", _int), ("causal", _int), ("window", _i64),
+                ("scale", ctypes.c_float), ("out", _vp), ("ldo", _i64), ("y", _vp), ("ldy", _i64), ("a_next", _vp),
+                ("lda", _i64)]
+
+
+class KvTablesDesc(ctypes.Structure):
+    """zest_kv_tables: who holds which page."""
+    _fields_ = [("refs", _vp), ("table", _vp), ("len", _vp), ("seqs", _i64), ("table_stride", _i64)]
+
+
 class Times(ctypes.Structure):
     _fields_ = [("encode_ms", ctypes.c_double), ("gemm_ms", ctypes.c_double), ("copy_ms", ctypes.c_double),
                 ("pack_ms", ctypes.c_double), ("calls", _int)]
@@ -97,6 +131,14 @@ def lib() -> ctypes.CDLL:
         "zest_glu": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
         "zest_rope_table": (_int, [_vp, _i64, _int, _int, ctypes.POINTER(ctypes.c_float), _vp, _vp, _vp]),
         "zest_rope": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp]),
+        "zest_kv_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp]),
+        "zest_kv_attend": (_int, [_vp, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp, _vp]),
+        "zest_kv_attend_workspace": (_i64, [_vp, _vp, _vp]),
+        "zest_kv_grow": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp]),
+        "zest_kv_fork": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp]),
+        "zest_kv_free": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp]),
+        "zest_kv_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+        "zest_kv_pages_workspace": (_i64, [_vp]),
         "zest_usable": (_int, [_int, ctypes.c_char_p, ctypes.c_size_t]),
         "zest_open": (_vp, [_int]),
         "zest_close": (None, [_vp]),
@@ -133,6 +175,8 @@ def exported_symbols() -> list[str]:
                         "zest_gemm_segs", "zest_plan_gemm", "zest_mul_mat_noalloc",
                         "zest_rms_norm", "zest_mul_row", "zest_add", "zest_scale", "zest_glu", "zest_rope_table",
                         "zest_rope", "zest_pack_rms_norm", "zest_norm_rope", "zest_widen_bf16",
+                        "zest_kv_append", "zest_kv_attend", "zest_kv_attend_workspace", "zest_kv_grow",
+                        "zest_kv_fork", "zest_kv_free", "zest_kv_compact", "zest_kv_pages_workspace",
                         "zest_usable", "zest_open",
                         "zest_close", "zest_set_out16", "zest_has_weight", "zest_add_weight", "zest_add_fused",
                         "zest_add_weight_values",
@@ -266,6 +310,233 @@ def plan_gemm(M: int, K: int, Ns, sms: int = 0) -> dict:
     out = GemmPlan()
     _check(lib().zest_plan_gemm(M, K, n, (_i64 * n)(*Ns), sms, ctypes.byref(out)), "zest_plan_gemm")
     return {name: getattr(out, name) for name, _ in GemmPlan._fields_}
+
+
+# --- the paged key/value cache ------------------------------------------------
+
+
+def _kv_stream(device: int):
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+class _on_device:
+    """The tensors' device current for one call (nothing to do where it already is)."""
+
+    __slots__ = ("device", "before")
+
+    def __init__(self, device: int):
+        self.device = device
+
+    def __enter__(self):
+        import torch
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.device:
+            torch._C._cuda_setDevice(self.device)
+
+    def __exit__(self, *_):
+        import torch
+        if self.before != self.device:
+            torch._C._cuda_setDevice(self.before)
+
+
+def _dev_ptr(t, dtype, device: int, what: str):
+    """A tensor's address after the checks that the C ABI cannot make."""
+    if t.dtype != dtype or t.get_device() != device:
+        raise ZestError(f"{what}: a {dtype} tensor on the cache's device is wanted, not {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _packed(t, dtype, device: int, n: int, what: str):
+    if not t.is_contiguous() or t.numel() < n:
+        raise ZestError(f"{what}: {n} contiguous values are wanted")
+    return _dev_ptr(t, dtype, device, what)
+
+
+def _heads_rows(t, dtype, device: int, T: int, heads: int, d: int, what: str):
+    """(address, row stride) of [T][heads][d] or [T][heads * d] rows whose values lie side by side."""
+    ok = t.shape[0] >= T and t.stride(-1) == 1 and (
+        t.shape[1:] == (heads * d,) or (t.shape[1:] == (heads, d) and (heads == 1 or t.stride(1) == d)))
+    if not ok:
+        raise ZestError(f"{what}: {T} rows of {heads} heads of {d}, each row in one run, are wanted")
+    return _dev_ptr(t, dtype, device, what), t.stride(0) if t.shape[0] > 1 else pad_to(heads * d, 8)
+
+
+def _heads_of(t, d: int) -> int:
+    return t.shape[1] if t.dim() == 3 else t.shape[-1] // d
+
+
+def _own_err(err, device: int):
+    import torch
+    return torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}") if err is None else err
+
+
+def _raise_err(err, given, what: str):
+    if given is None:
+        e = int(err.item())
+        if e:
+            raise ZestError(f"{what} raised device error bits {e:#x}")
+
+
+class KvCache:
+    """zest_kv_cache over two tensors [layers][pages][page_size][kv_heads][d], bf16 or f16. They may
+    be views in which heads come before tokens; the last dimension's values lie side by side."""
+
+    def __init__(self, k, v):
+        import torch
+        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.stride(4) != 1 or not k.is_cuda or \
+                k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or v.device != k.device:
+            raise ZestError("KvCache: two 5-D bf16 or f16 cuda tensors of the same shape and strides are wanted")
+        self.k, self.v, self.device = k, v, k.get_device()
+        layers, pages, page, heads, d = k.shape
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), TYPE_BF16 if k.dtype == torch.bfloat16 else TYPE_F16,
+                                page, heads, d, layers, pages, *k.stride()[:4])
+        self.ref = ctypes.addressof(self.desc)
+
+
+class KvBatch:
+    """zest_kv_batch over int32 tensors: q_start [n + 1], kv_len [n], table [n][pages of the longest].
+    max_q and max_kv bound the sequences' new and cached tokens (the launch is shaped by them)."""
+
+    def __init__(self, q_start, kv_len, table, T: int, max_q: int, max_kv: int):
+        import torch
+        n, device = kv_len.shape[0], kv_len.get_device()
+        if table.dim() != 2 or table.shape[0] < n or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ZestError("KvBatch: a table row for each sequence is wanted")
+        self.tensors = (q_start, kv_len, table)
+        # a row is as wide as its shape says; rows further apart are read at their stride
+        if table.shape[0] > 1 and table.stride(0) != table.shape[1]:
+            raise ZestError("KvBatch: table rows that follow one another are wanted")
+        self.desc = KvBatchDesc(_packed(q_start, torch.int32, device, n + 1, "q_start"),
+                                _packed(kv_len, torch.int32, device, n, "kv_len"),
+                                _dev_ptr(table, torch.int32, device, "table"), table.shape[1], T, max_q, max_kv, n)
+        self.device = device
+        self.ref = ctypes.addressof(self.desc)
+
+
+class KvTables:
+    """zest_kv_tables over int32 tensors: refs [pages], table [seqs][pages of the longest], len [seqs]."""
+
+    def __init__(self, refs, table, lens):
+        import torch
+        device = refs.get_device()
+        self.tensors, self.device = (refs, table, lens), device
+        self.desc = KvTablesDesc(_packed(refs, torch.int32, device, 1, "refs"),
+                                 _packed(table, torch.int32, device, 1, "table"),
+                                 _packed(lens, torch.int32, device, table.shape[0], "len"), *table.shape)
+        self.ref = ctypes.addressof(self.desc)
+
+
+def kv_append(cache: KvCache, layer: int, batch: KvBatch, k, v, q=None, q_out=None, k_norm=None, q_norm=None,
+              eps: float = -1.0, rope=None, mode: int = ROPE_NEOX, err=None):
+    """zest_kv_append: a step's f32 k and v [T][kv_heads][d] into their pages (k, and q into q_out, normed per head
+    when eps >= 0 and rotated by `rope`, a zest_rope_table [T][n_dims])."""
+    import torch
+    f32, c, dev, T = torch.float32, cache.desc, cache.device, batch.desc.T
+    if batch.device != dev:
+        raise ZestError("kv_append: the batch lies on another device than the cache")
+    kp, ldk = _heads_rows(k, f32, dev, T, c.kv_heads, c.d, "k")
+    vp, ldv = _heads_rows(v, f32, dev, T, c.kv_heads, c.d, "v")
+    qp, ldq, op, ldo, heads = None, 0, None, 0, 0
+    if q is not None:
+        if q_out is None:
+            raise ZestError("kv_append: q needs q_out")
+        heads = _heads_of(q_out, c.d)
+        qp, ldq = _heads_rows(q, f32, dev, T, heads, c.d, "q")
+        op, ldo = _heads_rows(q_out, cache.k.dtype, dev, T, heads, c.d, "q_out")
+    w = [None if x is None else _packed(x, f32, dev, c.d, "norm weight") for x in (q_norm, k_norm)]
+    rp, n_dims = None, 0
+    if rope is not None:
+        n_dims = rope.shape[1]
+        rp = _packed(rope, f32, dev, T * n_dims, "rope")
+    given, err = err, _own_err(err, dev)
+    a = KvNew(kp, vp, ldk, ldv, qp, ldq, op, ldo, heads, eps, w[0], w[1], rp, n_dims, mode)
+    with _on_device(dev):
+        _check(lib().zest_kv_append(cache.ref, layer, batch.ref, ctypes.addressof(a),
+                                    _dev_ptr(err, torch.int32, dev, "err"), _kv_stream(dev)), "zest_kv_append")
+    _raise_err(err, given, "zest_kv_append")
+
+
+def kv_attend(cache: KvCache, layer: int, batch: KvBatch, q, scale: float | None = None, causal: bool = True,
+              window: int = 0, out=None, y=None, a_next=None, workspace=None, err=None):
+    """zest_kv_attend: the attention of q [T][heads][d] (the cache's type) over one layer. The result goes to out
+    (the cache's type; made when no output is given), y (f32) and/or a_next (the o matmul's operand)."""
+    import torch
+    c, dev, T, dt = cache.desc, cache.device, batch.desc.T, cache.k.dtype
+    if batch.device != dev:
+        raise ZestError("kv_attend: the batch lies on another device than the cache")
+    heads = _heads_of(q, c.d)
+    qp, ldq = _heads_rows(q, dt, dev, T, heads, c.d, "q")
+    made = out is None and y is None and a_next is None
+    if made:
+        out = torch.zeros((T, heads, c.d), dtype=dt, device=q.device)
+    op = yp = ap = None
+    ldo = ldy = lda = 0
+    if out is not None:
+        op, ldo = _heads_rows(out, dt, dev, T, heads, c.d, "out")
+    if y is not None:
+        yp, ldy = _heads_rows(y, torch.float32, dev, T, heads, c.d, "y")
+    if a_next is not None:
+        ap, lda = _heads_rows(a_next, torch.int16, dev, T, heads, c.d, "a_next")
+    a = KvAttn(qp, ldq, heads, causal, window, c.d ** -0.5 if scale is None else scale, op, ldo, yp, ldy, ap, lda)
+    L, ref = lib(), ctypes.addressof(a)
+    with _on_device(dev):
+        need = L.zest_kv_attend_workspace(cache.ref, batch.ref, ref)
+        if need < 0:
+            _check(-1, "zest_kv_attend")
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        given, err = err, _own_err(err, dev)
+        ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        _check(L.zest_kv_attend(cache.ref, layer, batch.ref, ref, ws, size, _dev_ptr(err, torch.int32, dev, "err"),
+                                _kv_stream(dev)), "zest_kv_attend")
+    _raise_err(err, given, "zest_kv_attend")
+    return out if out is not None else y if y is not None else a_next
+
+
+def _kv_pages(call: str, cache: KvCache, tables: KvTables, out, arrays, workspace, err):
+    import torch
+    out = tables if out is None else out
+    dev = cache.device
+    pages = cache.desc.pages
+    for t in (tables, out):
+        if t.device != dev or t.tensors[0].numel() < pages:
+            raise ZestError(f"{call}: tables on the cache's device, with a count for each page, are wanted")
+    n = arrays[0].numel() if arrays else 0
+    ptrs = [_packed(x, torch.int32, dev, n, call) for x in arrays]
+    L = lib()
+    given, err = err, _own_err(err, dev)
+    with _on_device(dev):
+        args = [cache.ref, tables.ref, out.ref] + ([n] if arrays else []) + ptrs
+        if call in ("zest_kv_fork", "zest_kv_compact"):
+            if workspace is None:
+                workspace = torch.empty(L.zest_kv_pages_workspace(cache.ref), dtype=torch.uint8, device=cache.k.device)
+            elif workspace.numel() * workspace.element_size() < L.zest_kv_pages_workspace(cache.ref):
+                raise ZestError(f"{call}: the workspace is smaller than zest_kv_pages_workspace says")
+            args.append(workspace.data_ptr())
+        _check(getattr(L, call)(*args, _dev_ptr(err, torch.int32, dev, "err"), _kv_stream(dev)), call)
+    _raise_err(err, given, call)
+    return out
+
+
+def kv_grow(cache, tables, seq, add, out=None, err=None):
+    """zest_kv_grow: room for add[i] more tokens of sequence seq[i]. Here as below, in place unless `out` is given."""
+    return _kv_pages("zest_kv_grow", cache, tables, out, (seq, add), None, err)
+
+
+def kv_fork(cache, tables, src, dst, out=None, workspace=None, err=None):
+    """zest_kv_fork: the empty sequences dst[i] become copies of src[i]."""
+    return _kv_pages("zest_kv_fork", cache, tables, out, (src, dst), workspace, err)
+
+
+def kv_free(cache, tables, seq, out=None, err=None):
+    """zest_kv_free: the sequences give their pages back."""
+    return _kv_pages("zest_kv_free", cache, tables, out, (seq,), None, err)
+
+
+def kv_compact(cache, tables, out=None, workspace=None, err=None):
+    """zest_kv_compact: the pages in use moved to the front."""
+    return _kv_pages("zest_kv_compact", cache, tables, out, (), workspace, err)
 
 
 # --- the matmul service -------------------------------------------------------

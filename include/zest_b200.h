@@ -280,6 +280,142 @@ int zest_norm_rope(const float *x, int64_t T, int64_t heads, int64_t d, float ep
                    int mode, const float *table, float *y, uint16_t *y_bf16, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * A paged key/value cache and the attention that reads it (device pointers,
+ * on the caller's stream). No counterpart in the reference, which leaves the
+ * attention and its cache to the sibling backend: these are the ops a prompt
+ * chunk needs between the q/k/v matmuls and the o matmul, and a serving loop
+ * between its steps. None of them allocates, waits for the GPU or copies to
+ * the host; all may be captured into a CUDA graph.
+ *
+ * err is a device word that the kernels OR ZEST_ERR_* bits into (the caller
+ * clears it). A sequence or a page that is out of bounds is never read or
+ * written: it raises a bit, and what was asked of it is not done.
+ * ------------------------------------------------------------------------- */
+#define ZEST_TYPE_BF16 30        /* with ZEST_TYPE_F16: the types of a cache (ggml_type ids) */
+#define ZEST_ERR_BAD_PAGE 4u     /* a page number outside the cache where a page was needed */
+#define ZEST_ERR_BAD_SEQ 8u      /* a sequence out of range, longer than its table row or the given maxima, or
+                                    (fork, grow) named twice or not empty */
+#define ZEST_ERR_NO_PAGES 16u    /* too few free pages: nothing was changed */
+
+/* The pools: k and v hold `layers` layers of `pages` pages of `page_size`
+ * tokens of `kv_heads` heads of d values. Value (layer, page, token, head, i)
+ * is at layer * layer_stride + page * page_stride + token * token_stride +
+ * head * head_stride + i, in values: tokens or heads may come first. */
+typedef struct {
+    void *k, *v;                /* 16-byte aligned */
+    int type;                   /* ZEST_TYPE_BF16 or ZEST_TYPE_F16 */
+    int page_size;              /* 16, 32, 64, 128 or 256 */
+    int kv_heads, d;            /* d a multiple of 8, at most 256 */
+    int64_t layers, pages;
+    int64_t layer_stride, page_stride, token_stride, head_stride; /* multiples of 8 */
+} zest_kv_cache;
+
+/* A batch of sequences with new tokens. Sequence s has the rows
+ * [q_start[s], q_start[s+1]) of the step's T rows, holds kv_len[s] tokens
+ * (its new ones included: they are the last), and its token p lies in page
+ * table[s][p / page_size]. Rows outside every sequence are left as they are. */
+typedef struct {
+    const int32_t *q_start;     /* [n_seqs + 1], rising */
+    const int32_t *kv_len;      /* [n_seqs] */
+    const int32_t *table;       /* [n_seqs][table_stride] */
+    int64_t table_stride;
+    int64_t T;
+    int64_t max_q, max_kv;      /* no sequence has more new tokens, or holds more (host-side bounds that the
+                                   launch is shaped by; a longer sequence raises ZEST_ERR_BAD_SEQ) */
+    int n_seqs;                 /* at most 65535 */
+} zest_kv_batch;
+
+/* What zest_kv_append takes of a step: the f32 projections of its T rows. */
+typedef struct {
+    const float *k, *v;         /* [T][ldk], [T][ldv]: kv_heads heads of d; rows 16-byte aligned */
+    int64_t ldk, ldv;
+    const float *q;             /* NULL, or [T][ldq]: heads heads of d, which go to q_out */
+    int64_t ldq;
+    void *q_out;                /* [T][ldqo] in the cache's type */
+    int64_t ldqo;               /* a multiple of 8 */
+    int heads;
+    float eps;                  /* of the per-head RMS_NORM of q and k; < 0: no norm */
+    const float *q_norm, *k_norm; /* its weight rows of d (NULL: none), 16-byte aligned */
+    const float *rope;          /* NULL, or zest_rope_table's [T][n_dims]: q and k are rotated */
+    int n_dims, mode;           /* as zest_rope */
+} zest_kv_new;
+
+/* The new tokens' keys and values into their pages of one layer: k after its
+ * per-head RMS_NORM, weight and ROPE (each optional), v as it is, both rounded
+ * once to the cache's type (nearest even); and the step's queries, normed and
+ * rotated alike, to q_out for zest_kv_attend. One launch. A page that new
+ * tokens are written to belongs to one sequence alone (zest_kv_fork sees to
+ * that). */
+int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *batch, const zest_kv_new *in,
+                   unsigned *err, void *stream);
+
+/* What zest_kv_attend reads and writes. Row t, head h of the result:
+ * sum_j p_j v_j / sum_j p_j with p_j = exp(scale * q.k_j) over the tokens j
+ * that the row sees in kv head h / (heads / kv_heads): j < kv_len; if causal,
+ * j <= pos, the row's own position kv_len - (new tokens) + (its index among
+ * them); if window > 0 (causal only), j > pos - window. A row that sees
+ * nothing is zero. What a row does not see does not reach it, NaN or infinite
+ * values among it. Not causal: the attention to states of another length.
+ * Sums in f32; p is rounded to the cache's type before it meets v. */
+typedef struct {
+    const void *q;              /* [T][ldq], heads heads of d, the cache's type; 16-byte aligned rows */
+    int64_t ldq;                /* a multiple of 8 */
+    int heads;                  /* a multiple of kv_heads, at most 128 times it */
+    int causal;
+    int64_t window;             /* 0: none */
+    float scale;                /* positive */
+    void *out;                  /* NULL, or [T][ldo] in the cache's type */
+    int64_t ldo;                /* a multiple of 8 */
+    float *y;                   /* NULL, or [T][ldy] in f32, ggml's attention output */
+    int64_t ldy;                /* a multiple of 4 */
+    uint16_t *a_next;           /* NULL, or [T][lda]: y's K2 operand, the o matmul's A (the same bits as
+                                   zest_pack_activations of y, rows past T aside) */
+    int64_t lda;                /* a multiple of 8 */
+} zest_kv_attn;
+
+/* The attention of a step's rows over one layer of the cache (append the
+ * step's tokens first). workspace: zest_kv_attend_workspace bytes of device
+ * memory, 16-byte aligned, its contents free before and after; calls that may
+ * overlap take one each. */
+int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *batch, const zest_kv_attn *at,
+                   void *workspace, size_t workspace_bytes, unsigned *err, void *stream);
+/* Bytes of workspace such a call needs (0: none); -1 for a call that
+ * zest_kv_attend refuses for its sizes. Reads sizes only: needs no GPU. */
+int64_t zest_kv_attend_workspace(const zest_kv_cache *kv, const zest_kv_batch *batch, const zest_kv_attn *at);
+
+/* Who holds which page: refs[page] table rows hold it (0: it is free), and
+ * sequence s's len[s] tokens lie in table[s][0..]; unused entries are -1. */
+typedef struct {
+    int32_t *refs;              /* [pages of the cache] */
+    int32_t *table;             /* [seqs][table_stride] */
+    int32_t *len;               /* [seqs] */
+    int64_t seqs, table_stride;
+} zest_kv_tables;
+
+/* The page operations: tables `in` to tables `out` (the same, or disjoint
+ * arrays of the same sizes), n sequences at once (n <= ZEST_KV_MAX_SEQS,
+ * device arrays). Free pages are taken lowest number first, for the sequences
+ * in the order given. On an error bit of theirs nothing changes: `out` is
+ * `in`. workspace: zest_kv_pages_workspace bytes, 16-byte aligned. */
+#define ZEST_KV_MAX_SEQS 1024
+/* Room for add[i] more tokens of sequence seq[i] (each named once). */
+int zest_kv_grow(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *seq, const int32_t *add, unsigned *err, void *stream);
+/* Sequence dst[i] (empty, each named once) becomes a copy of src[i]: whole
+ * pages are shared, a part-filled last page is copied in every layer. */
+int zest_kv_fork(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *src, const int32_t *dst, void *workspace, unsigned *err, void *stream);
+/* Sequences seq[i] give their pages back and are empty (naming one twice
+ * frees it once). */
+int zest_kv_free(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
+                 const int32_t *seq, unsigned *err, void *stream);
+/* The pages in use moved to the front, in every layer: with c pages in use,
+ * the k-th of them numbered c or higher goes to the k-th free one below c. */
+int zest_kv_compact(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, void *workspace,
+                    unsigned *err, void *stream);
+int64_t zest_kv_pages_workspace(const zest_kv_cache *kv);
+
+/* ---------------------------------------------------------------------------
  * 2. The matmul service (xdna_npu)
  * ------------------------------------------------------------------------- */
 

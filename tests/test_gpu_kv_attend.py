@@ -1,0 +1,278 @@
+"""zest_kv_attend against the attention's definition in 64 bits: types, head
+layouts, lengths, page sizes, masks, strides, values that must not reach a
+row, captured and concurrent calls.
+
+Tolerance, per value: the output's own rounding, half a step of the value
+(eps / 2 * |o|); the weights' rounding to the cache's type before they meet
+the values, half a step of each (eps / 2 * sum p |v| / sum p); and f32: the
+scores are d-term f32 sums of products of magnitude |q||k| scale, at most
+d 2^-24 of the largest such sum here (|score| below 2^5: 256 * 2^-24 * 2^5 =
+2^-11 in the worst case and about its square root's share, 2^-15, in fact),
+the exponential and the running sums a few 2^-22: together below 2^-11 of
+sum p |v| / sum p. f16 weights below 2^-14 are held to 2^-25 absolutely,
+relative to a largest weight of 2^-8 to 1."""
+import math
+import random
+
+import pytest
+import torch
+
+import zest_b200 as Z
+from kv_util import attention, laid_out
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+class Case:
+    """A batch of (new tokens, all tokens) over a pool whose pages lie in no order, NaN in everything that no
+    sequence holds."""
+
+    def __init__(self, lens, heads, kv_heads, d, page, dt, seed=0, heads_first=False, spare=2, width=None, layers=1):
+        g = torch.Generator("cuda").manual_seed(seed)
+        self.lens, self.heads, self.kv_heads, self.d, self.page, self.dt = lens, heads, kv_heads, d, page, dt
+        held = [-(-kv // page) for _, kv in lens]
+        pages = sum(held) + spare
+        order = random.Random(seed).sample(range(pages), pages)
+        self.width = width or max([1] + held)
+        self.rows = []
+        for n in held:
+            self.rows.append([order.pop() for _ in range(n)])
+        self.table = i32([r + [-1] * (self.width - len(r)) for r in self.rows])
+        starts = [0]
+        for n, _ in lens:
+            starts.append(starts[-1] + n)
+        self.T = starts[-1]
+        self.starts = starts
+        self.q_start, self.kv_len = i32(starts), i32([kv for _, kv in lens])
+        shape = (layers, pages, kv_heads, page, d) if heads_first else (layers, pages, page, kv_heads, d)
+        pool = lambda: (torch.randn(shape, device="cuda", generator=g) * 1.1).to(dt)
+        self.k, self.v = pool(), pool()
+        if heads_first:
+            self.k, self.v = self.k.transpose(2, 3), self.v.transpose(2, 3)
+        mine = torch.zeros(pages, page, dtype=torch.bool, device="cuda")
+        for row, (_, kv) in zip(self.rows, lens):
+            for j, p in enumerate(row):
+                mine[p, :min(page, kv - j * page)] = True
+        self.k[:, ~mine] = math.nan
+        self.v[:, ~mine] = math.nan
+        self.q = torch.randn(self.T, heads, d, device="cuda", generator=g).to(dt)
+        self.max_q, self.max_kv = max([n for n, _ in lens] + [0]), max([kv for _, kv in lens] + [0])
+        self.cache = Z.KvCache(self.k, self.v)
+        self.batch = Z.KvBatch(self.q_start, self.kv_len, self.table, T=self.T, max_q=self.max_q, max_kv=self.max_kv)
+        self.scale = 1 / math.sqrt(d)
+
+    def want(self, causal=True, window=0, layer=0):
+        o = torch.zeros(self.T, self.heads, self.d, dtype=torch.float64, device="cuda")
+        a, n = torch.zeros_like(o), torch.zeros(self.T, dtype=torch.int64, device="cuda")
+        for s, (new, kv) in enumerate(self.lens):
+            i, j = self.starts[s], self.starts[s + 1]
+            k, v = (laid_out(x[layer], self.rows[s], kv, self.page) for x in (self.k, self.v))
+            o[i:j], a[i:j], n[i:j] = attention(self.q[i:j].double(), k, v, kv - new, self.scale, causal, window)
+        return o, a, n
+
+    def check(self, got, causal=True, window=0, layer=0, eps=None):
+        o, a, n = self.want(causal, window, layer)
+        e = torch.finfo(self.dt).eps / 2
+        out = e if eps is None else eps
+        tol = out * o.abs() + (e + 2 ** -11) * a + 1e-30
+        if self.dt == HF:
+            tol += n[:, None, None] * 2.0 ** -25 * 2 ** 8 * 4 / n.clamp(min=1)[:, None, None].double().sqrt() + 2 ** -25
+        got = got.double().view(o.shape)
+        assert torch.equal(torch.isfinite(got), torch.isfinite(o)), "another set of finite values"
+        fine = torch.isfinite(o)
+        worst = ((got - o).abs() / tol)[fine]
+        assert worst.numel() == 0 or worst.max().item() <= 1.0, f"{worst.max().item():.3g} times the tolerance"
+
+
+FEW = [  # up to 16 rows of a kv head, and a few tiles of them
+    (BF, 128, 32, 8, 64, [(1, 1000)], True, 0),
+    (HF, 128, 32, 8, 16, [(1, 1), (1, 17), (1, 64), (1, 65), (1, 700)], True, 0),
+    (BF, 64, 32, 8, 16, [(1, 5), (2, 300), (4, 4), (3, 90)], True, 0),
+    (HF, 256, 24, 4, 64, [(1, 900), (2, 33)], True, 0),
+    (BF, 128, 8, 8, 32, [(1, 50), (5, 200)], True, 0),          # one query head a kv head
+    (BF, 128, 12, 2, 128, [(1, 513), (2, 1)], True, 0),         # fewer keys than new tokens
+    (HF, 96, 15, 3, 256, [(3, 300), (1, 256)], True, 0),
+    (BF, 8, 2, 1, 16, [(1, 40), (7, 40)], True, 0),
+    (HF, 72, 9, 9, 16, [(1, 129)], False, 0),
+    (BF, 128, 16, 1, 64, [(1, 400)], True, 100),
+    (BF, 80, 6, 2, 16, [(1, 200), (3, 77), (1, 3)], True, 1),
+    (HF, 128, 8, 2, 64, [(1, 4000)], True, 37),
+]
+MANY = [  # chunks of new tokens
+    (BF, 128, 8, 2, 64, [(300, 300)], True, 0),
+    (BF, 128, 8, 2, 64, [(257, 1000)], True, 0),
+    (HF, 128, 4, 4, 16, [(130, 513)], True, 0),
+    (HF, 64, 8, 2, 16, [(100, 400), (1, 90), (0, 50), (33, 33)], True, 0),
+    (BF, 64, 12, 2, 32, [(200, 260)], True, 50),
+    (BF, 256, 6, 1, 64, [(90, 333)], True, 0),
+    (HF, 256, 4, 2, 128, [(140, 140), (70, 200)], True, 0),
+    (BF, 128, 14, 2, 256, [(64, 600)], True, 0),                # 7 query heads a kv head
+    (HF, 112, 10, 2, 64, [(65, 129)], True, 0),
+    (BF, 128, 71, 1, 64, [(20, 200)], True, 0),                 # one kv head for 71
+    (BF, 128, 8, 2, 64, [(150, 40)], True, 0),                  # rows before the first key: zeros
+    (BF, 128, 8, 2, 64, [(150, 0), (40, 0)], True, 0),
+    (HF, 128, 8, 2, 64, [(100, 333), (40, 1)], False, 0),       # to an encoder's states
+    (BF, 200, 4, 2, 16, [(70, 300)], False, 0),
+    (BF, 128, 8, 8, 16, [(300, 2000)], True, 200),
+    (HF, 64, 4, 1, 64, [(513, 700)], True, 3),
+]
+
+
+@pytest.mark.parametrize("dt,d,heads,kv_heads,page,lens,causal,window", FEW + MANY)
+def test_equals_the_definition(dt, d, heads, kv_heads, page, lens, causal, window):
+    c = Case(lens, heads, kv_heads, d, page, dt, seed=d + heads)
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, causal=causal, window=window), causal, window)
+
+
+@pytest.mark.parametrize("lens", [[(1, 3000)], [(1, 5000), (1, 100), (1, 2500)], [(40, 3000)], [(200, 6000)]])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_long_keys_are_cut_and_joined(lens, heads_first):
+    c = Case(lens, 8, 2, 128, 16, BF, seed=5, heads_first=heads_first)
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q))
+    # the launch is shaped by the bounds, the result is not
+    wide = Z.KvBatch(c.q_start, c.kv_len, c.table, T=c.T, max_q=c.max_q + 100, max_kv=c.max_kv * 9)
+    c.check(Z.kv_attend(c.cache, 0, wide, c.q))
+
+
+@pytest.mark.parametrize("lens", [[(1, 200)], [(1, 3000)], [(150, 400)]])
+def test_outputs_and_strides(lens):
+    c = Case(lens, 8, 2, 128, 64, BF, seed=9, layers=3)
+    W = 8 * 128
+    q = torch.full((c.T, W + 24), math.nan, dtype=BF, device="cuda")
+    q[:, :W] = c.q.view(c.T, W)
+    out = torch.full((c.T, W + 40), 7.0, dtype=BF, device="cuda")
+    y = torch.full((c.T, W + 4), 7.0, device="cuda")
+    a = torch.full((c.T, W + 8), 7, dtype=torch.int16, device="cuda")
+    Z.kv_attend(c.cache, 2, c.batch, q[:, :W], out=out[:, :W], y=y[:, :W], a_next=a[:, :W])
+    c.check(y[:, :W], layer=2, eps=2.0 ** -23)
+    assert torch.equal(out[:, :W], y[:, :W].to(BF))
+    _, want = Z.pack_activations(y[:, :W].contiguous(), want_bytes=False)
+    assert torch.equal(a[:, :W], want[:c.T])
+    assert (out[:, W:] == 7).all() and (y[:, W:] == 7).all() and (a[:, W:] == 7).all()
+    again = torch.empty((c.T, W), device="cuda")
+    Z.kv_attend(c.cache, 2, c.batch, q[:, :W], y=again)
+    assert torch.equal(again, y[:, :W])
+
+
+@pytest.mark.parametrize("d,lens,window", [(128, [(5, 100)], 0), (128, [(200, 300)], 0), (64, [(90, 300)], 20),
+                                           (256, [(70, 200)], 0), (128, [(3, 3000)], 0), (256, [(2, 130)], 40)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_a_row_does_not_see_do_not_reach_it(d, lens, window, bad):
+    c = Case(lens, 8, 2, d, 16, BF, seed=3)
+    n, kv = lens[0]
+    at = lambda p: (c.rows[0][p // 16], p % 16)
+    # in the last token's value, one before it, and (seen by the first rows alone) at the window's start
+    for p, head, col in [(kv - 1, 0, 3), (kv - 2, 1, d - 1)] + ([(kv - n - window + 1, 0, 5)] if window else []):
+        c.v[0][at(p)][head, col] = bad
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, window=window), window=window)
+    # a NaN or infinite key reaches the rows that see it alone
+    c = Case(lens, 8, 2, d, 16, BF, seed=4)
+    c.k[0][at(kv - 1)][1, 2] = math.nan
+    got = Z.kv_attend(c.cache, 0, c.batch, c.q, window=window)
+    assert torch.isnan(got[n - 1, 4:]).all()
+    rest = torch.ones(n, 8, dtype=torch.bool, device="cuda")
+    rest[n - 1, 4:] = False
+    assert torch.isfinite(got[rest]).all()
+
+
+def test_masked_lowest_and_infinite_scores():
+    c = Case([(40, 200)], 4, 4, 64, 16, HF, seed=8)
+    c.q[:, 0] = 65504.0  # the type's largest: scores of millions, one key takes all
+    c.q[:, 1] = 0.0      # every key the same
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q))
+
+
+@pytest.mark.parametrize("lens", [[(1, 90), (3, 40)], [(60, 90), (33, 40)]])
+def test_rows_outside_the_sequences_stay(lens):
+    c = Case(lens, 8, 2, 128, 16, BF, seed=2)
+    T = c.T + 150
+    q = torch.full((T, 8, 128), math.nan, dtype=BF, device="cuda")
+    q[3:3 + c.T] = c.q
+    out = torch.full((T, 8, 128), 5.0, dtype=BF, device="cuda")
+    b = Z.KvBatch(c.q_start + 3, c.kv_len, c.table, T=T, max_q=c.max_q, max_kv=c.max_kv)
+    Z.kv_attend(c.cache, 0, b, q, out=out)
+    c.check(out[3:3 + c.T])
+    assert (out[:3] == 5).all() and (out[3 + c.T:] == 5).all()
+
+
+@pytest.mark.parametrize("lens", [[(1, 200), (1, 300), (1, 100)], [(40, 200), (50, 300), (60, 100)]])
+def test_bad_sequences_and_pages_raise_bits(lens):
+    c = Case(lens, 8, 2, 128, 16, BF, seed=6)
+    good = Z.kv_attend(c.cache, 0, c.batch, c.q)
+    mid = slice(c.starts[1], c.starts[2])
+    for change in ("long", "pages", "starts"):
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.full_like(good, 5.0)
+        kv, table, starts = c.kv_len.clone(), c.table.clone(), c.q_start.clone()
+        if change == "long":  # longer than its table row
+            kv[1] = c.width * 16 + 1
+        elif change == "pages":
+            table[1, 2], table[1, 3] = 1 << 30, -7
+        else:
+            starts[2] = starts[1] - 1  # falling: the second sequence, and the third's start
+        b = Z.KvBatch(starts, kv, table, T=c.T, max_q=c.max_q, max_kv=1 << 20)
+        Z.kv_attend(c.cache, 0, b, c.q, out=out, err=err)
+        assert int(err) == (Z.ERR_BAD_PAGE if change == "pages" else Z.ERR_BAD_SEQ)
+        assert torch.equal(out[:c.starts[1]], good[:c.starts[1]])
+        if change == "long":
+            assert (out[mid] == 5).all() and torch.equal(out[c.starts[2]:], good[c.starts[2]:])
+    with pytest.raises(Z.ZestError, match="error bits 0x8"):
+        Z.kv_attend(c.cache, 0, Z.KvBatch(c.q_start, c.kv_len, c.table, T=c.T, max_q=c.max_q, max_kv=150), c.q)
+
+
+def test_captured_replayed_and_beside_another_stream():
+    """Two captured calls with a workspace each, replayed at once on two streams over changing lengths."""
+    cs = [Case([(1, 4000), (1, 900)], 8, 2, 128, 16, BF, seed=11), Case([(33, 4000)], 8, 2, 128, 64, BF, seed=12)]
+    calls = []
+    for c in cs:
+        out = torch.zeros_like(c.q)
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            Z.kv_attend(c.cache, 0, c.batch, c.q, out=out, err=err, workspace=ws)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            Z.kv_attend(c.cache, 0, c.batch, c.q, out=out, err=err, workspace=ws)
+        calls.append((c, out, err, ws, st, g))
+    for shorter in (0, 300, 1500):
+        for c, out, err, ws, st, g in calls:
+            c.kv_len -= shorter * (c.kv_len > 2 * shorter).int()
+            c.lens = list(zip([n for n, _ in c.lens], c.kv_len.tolist()))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for c, out, err, ws, st, g in calls:
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        for c, out, err, ws, st, g in calls:
+            assert int(err) == 0
+            c.check(out)
+
+
+def test_the_same_bits_every_time():
+    c = Case([(1, 3000), (1, 50)], 8, 2, 128, 16, BF, seed=1)
+    first = Z.kv_attend(c.cache, 0, c.batch, c.q)
+    for _ in range(5):
+        assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, c.q), first)
+
+
+@pytest.mark.parametrize("n", [1, 200])
+def test_offsets_past_32_bits(n):
+    """A pool of more than 2^32 values whose sequences lie at its end."""
+    pages, page, kv_heads, d = (1 << 32) // (64 * 8 * 128) + 40, 64, 8, 128
+    k = torch.zeros(1, pages, page, kv_heads, d, dtype=BF, device="cuda")
+    v = torch.zeros_like(k)
+    small = Case([(n, 1500)], 32, kv_heads, d, page, BF, seed=13)
+    rows = [pages - 1 - p for p in range(len(small.rows[0]))]
+    for a, b in zip(small.rows[0], rows):
+        k[0, b], v[0, b] = small.k[0, a], small.v[0, a]
+    batch = Z.KvBatch(small.q_start, small.kv_len, i32([rows]), T=n, max_q=n, max_kv=1500)
+    small.check(Z.kv_attend(Z.KvCache(k, v), 0, batch, small.q))
