@@ -244,10 +244,9 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             }
             page = next;
         }
-        // after a wait that ran out, the copies in flight still land
-        if (i < steps)
-            for (int k = max(0, i - C::STAGES); k < i; k++)
-                mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
+        // the last copies land before the block ends, whatever the others do
+        for (int k = max(0, i - C::STAGES); k < i; k++)
+            mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
         __syncthreads();
         return;
     }
@@ -455,6 +454,417 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     if (A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
 }
 
+// --- many rows: tcgen05 -------------------------------------------------------------
+
+// Shapes by padded head size. Two tiles of 128 query rows share each tile of
+// keys and values (one tile where the head is 256 wide, whose scores then have
+// two buffers): while one tile's rows take their exponentials, the tensor
+// cores work for the other.
+template <int DP>
+struct many_rows {
+    static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
+    static constexpr int NS = DP == 256 ? 2 : 1;    // score buffers of each
+    static constexpr int BN = DP == 256 ? 64 : 128; // keys of a tile
+    static constexpr int STAGES = 2;                // of K, and of V
+    static constexpr int Q_BYTES = 128 * DP * 2;
+    static constexpr int KV_BYTES = BN * DP * 2;
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
+    static constexpr int SOFTMAX = NQ * 128;        // threads
+    static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for the MMAs, K's copies and V's
+    // TMEM columns: O of each query tile, then its scores (P lies over them)
+    static constexpr int O_COL = 0, S_COL = NQ * DP, COLS = 512;
+};
+
+// A rise of the running maximum below this (in powers of two) leaves the
+// weights relative to the old one: they stay within 2^8, and o is not touched.
+constexpr float LAZY = 8.0f;
+
+__device__ __forceinline__ void fma2(float &a, float &b, float m, float c) {
+    asm("{\n\t.reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(m), "f"(c));
+}
+
+// A block: NQ x 128 rows of one kv head of one sequence over one chunk of
+// keys. S = Q K^T into TMEM; each softmax thread owns a row: it takes the
+// row's scores from TMEM, keeps m and l, and leaves the weights P in TMEM over
+// the scores, from where O += P V takes them as its A operand. O stays in TMEM
+// and is touched by the threads only when a row's maximum rises by more than
+// 2^8, and at the end.
+template <int DP, bool F16>
+__global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
+    kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                          const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
+    using C = many_rows<DP>;
+    constexpr int NQ = C::NQ, NS = C::NS, BN = C::BN, ST = C::STAGES;
+    extern __shared__ uint8_t dyn[];
+    uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
+    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + ST * C::KV_BYTES;
+    __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[NQ * NS], p_full[NQ * NS],
+        pv_done, drained;
+    __shared__ uint32_t tmem_sh;
+    __shared__ int stop, not_finite;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seq = blockIdx.z;
+    const int kv_head = blockIdx.y / A.splits, split = blockIdx.y % A.splits;
+    const int tile = gridDim.x - 1 - blockIdx.x;  // the last rows see the most keys: first
+
+    const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
+    if (!s.ok) {
+        if (threadIdx.x == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+        return;
+    }
+    const int per_tile = 128 / A.group;  // whole tokens of a query tile
+    const int t0 = min((int64_t) tile * NQ * per_tile, (int64_t) s.n), t1 = min(t0 + NQ * per_tile, s.n);
+    if (t0 >= t1) return;
+    const int nq = NQ > 1 && t0 + per_tile < t1 ? 2 : 1;  // query tiles that have rows
+    const key_span sp = span_of(A, s, t0, t1 - 1);
+    const int64_t from = (int64_t) sp.lo / KEYS * KEYS + split * A.chunk;
+    const int64_t to = min((int64_t) sp.hi, from + A.chunk);
+    const int n = to > from ? (int) ((to - from + BN - 1) / BN) : 0;
+    if (n == 0 && split > 0) return;
+
+    constexpr int W_MMA = C::SOFTMAX / 32, W_K = W_MMA + 1, W_V = W_MMA + 2;
+    if (threadIdx.x == 0) {
+        mbar_init(&q_full, 1);
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < NQ * NS; i++) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+        }
+        mbar_init(&pv_done, 1);
+        mbar_init(&drained, 1);
+        stop = 0;
+        not_finite = 0;
+        fence_barrier_init();
+    }
+    if (warp == W_MMA) {
+        tmem_alloc(&tmem_sh, C::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_sh;
+    volatile int *const gone = &stop;
+    auto give_up = [&] {
+        stop = 1;
+        atomicOr(A.err, ERR_TIMEOUT);
+    };
+
+    // A row of scores lives in registers: the softmax warps take the others'
+    // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
+    auto fewer = [] {
+        if (NQ > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    };
+    if (warp == W_K || warp == W_V) {
+        fewer();
+        // copies: Q once (K's warp), then a tile a step, a box of
+        // min(page, 64) keys by 64 columns a lane
+        const bool is_v = warp == W_V;
+        const CUtensorMap *map = is_v ? &tv : &tk;
+        uint8_t *sm = is_v ? v_sm : k_sm;
+        uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+        const int box = min(A.page_size, KEYS), boxes = BN / box;
+        const int kb = lane % boxes, col = lane / boxes * 64;
+        const bool mine = col < DP;
+        if (!is_v && n > 0 && lane == 0) {
+            mbar_arrive_expect_tx(&q_full, nq * (DP / 64) * per_tile * A.group * 128);
+            for (int q = 0; q < nq; q++)
+                for (int c = 0; c < DP / 64; c++)
+                    tma_load_3d(q_sm + q * C::Q_BYTES + c * (128 * 128), &tq, &q_full, c * 64, kv_head * A.group,
+                                s.q0 + t0 + q * per_tile);
+        }
+        __syncwarp();
+        auto page_of = [&](int i) {
+            const int64_t key = from + (int64_t) i * BN + kb * box;
+            if (!mine || i >= n || key >= to) return (int) A.pages;  // outside the tensor: zeros
+            const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
+            if (p < 0 || p >= A.pages) {
+                atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+                return (int) A.pages;
+            }
+            return p;
+        };
+        int page = page_of(0), i = 0;
+        for (; i < n; i++) {
+            const int st = i % ST;
+            const int next = page_of(i + 1);
+            const bool ok = i < ST || mbar_wait_bounded(&empty[st], (i / ST - 1) & 1, gone, WAIT_LIMIT_NS);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) give_up();
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
+            __syncwarp();
+            if (mine) {
+                const int64_t key = from + (int64_t) i * BN + kb * box;
+                tma_load_4d(sm + st * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, &full[st], col,
+                            (int) (key % A.page_size), kv_head, page);
+            }
+            page = next;
+        }
+        // the last copies land before the block ends, whatever the others do
+        for (int k = max(0, i - ST); k < i; k++)
+            mbar_wait_bounded(&full[k % ST], (k / ST) & 1, nullptr, WAIT_LIMIT_NS);
+        if (!is_v && n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
+    } else if (warp == W_MMA) {
+        fewer();
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
+            constexpr uint32_t QK = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
+            constexpr uint32_t PV = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
+            auto wait = [&](uint64_t *bar, int phase) {
+                if (mbar_wait_bounded(bar, phase & 1, gone, WAIT_LIMIT_NS)) {
+                    tc_fence_after();
+                    return true;
+                }
+                give_up();
+                return false;
+            };
+            auto s_col = [&](int q, int b) { return tmem + C::S_COL + (q * NS + b) * BN; };
+            auto scores = [&](int q, int i) {
+                const uint8_t *kt = k_sm + i % ST * C::KV_BYTES, *qt = q_sm + q * C::Q_BYTES;
+                const uint32_t d = s_col(q, NS > 1 ? i % NS : 0);
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ks++)
+                    tc_mma_bf16(d, sw128_desc(qt + ks / 4 * (128 * 128) + ks % 4 * 32),
+                                sw128_desc(kt + ks / 4 * (BN * 128) + ks % 4 * 32), QK, ks > 0);
+                tc_commit(&s_full[q * NS + (NS > 1 ? i % NS : 0)]);
+            };
+            auto values = [&](int q, int i) {
+                const uint8_t *vt = v_sm + i % ST * C::KV_BYTES;
+                const uint32_t a = s_col(q, NS > 1 ? i % NS : 0);
+#pragma unroll
+                for (int ks = 0; ks < BN / 16; ks++)
+                    tc_mma_f16_ts(tmem + C::O_COL + q * DP, a + ks * 8, sw128_desc_mn(vt + ks * 16 * 128, BN * 128),
+                                  PV, i > 0 || ks > 0);
+            };
+            bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
+            if (ok) {
+                for (int q = 0; q < nq; q++) scores(q, 0);
+                tc_commit(&k_empty[0]);
+            }
+            for (int i = 0; ok && i < n; i++) {
+                const bool more = i + 1 < n;
+                if (NS > 1 && more) {  // the other buffer: its weights went into the product before
+                    if (!(ok = wait(&k_full[(i + 1) % ST], (i + 1) / ST))) break;
+                    scores(0, i + 1);
+                    tc_commit(&k_empty[(i + 1) % ST]);
+                }
+                if (!(ok = wait(&v_full[i % ST], i / ST))) break;
+                for (int q = 0; ok && q < nq; q++) {
+                    if (!(ok = wait(&p_full[q * NS + (NS > 1 ? i % NS : 0)], i / NS))) break;
+                    values(q, i);
+                    if (q == nq - 1) tc_commit(&v_empty[i % ST]);
+                    if (NS > 1 || i == n - 1) {
+                        if (q == nq - 1) tc_commit(&pv_done);
+                    }
+                    if (NS == 1 && more) {
+                        if (q == 0 && !(ok = wait(&k_full[(i + 1) % ST], (i + 1) / ST))) break;
+                        scores(q, i + 1);
+                        if (q == nq - 1) tc_commit(&k_empty[(i + 1) % ST]);
+                    }
+                }
+            }
+            if (!ok) {  // what was issued still ends before TMEM goes
+                tc_commit(&drained);
+                mbar_wait_bounded(&drained, 0, nullptr, WAIT_LIMIT_NS);
+            }
+        }
+        __syncwarp();
+    } else if (warp > W_MMA) {
+        fewer();
+    } else {
+        if (NQ > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int q = warp / 4, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t) (warp % 4 * 32) << 16;
+        const uint32_t o_at = tmem + lanes + C::O_COL + q * DP;
+        const int tq0 = t0 + q * per_tile, tq1 = min(tq0 + per_tile, t1);
+        const int t = tq0 + row / A.group;
+        const bool valid = row < per_tile * A.group && t < t1;
+        const int lo = valid ? row_lo(A, s, t) : 0, hi = valid ? row_hi(A, s, t) : 0;
+        const key_span mine = span_of(A, s, tq0, tq1 - 1);
+        float m = -INFINITY, l = 0.0f;
+        bool ok = q < nq;
+        for (int i = 0; i < n && q < nq; i++) {
+            const int b = NS > 1 ? i % NS : 0;
+            ok = mbar_wait_bounded(&s_full[q * NS + b], (i / NS) & 1, gone, WAIT_LIMIT_NS);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) give_up();
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t s_at = tmem + lanes + C::S_COL + (q * NS + b) * BN;
+            uint32_t x[BN / 32][32];
+#pragma unroll
+            for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(s_at + c * 32, x[c]);
+#pragma unroll
+            for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
+            const int64_t key0 = from + (int64_t) i * BN;
+            if (key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to)) {
+                const int a = (int) (max((int64_t) lo, key0) - key0), z = (int) (min((int64_t) hi, to) - key0);
+#pragma unroll
+                for (int c = 0; c < BN / 32; c++)
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if (c * 32 + e < a || c * 32 + e >= z) x[c][e] = 0xff800000u;
+            }
+            if (key0 < sp.clo || key0 + BN > min((int64_t) sp.chi, to)) {
+                // keys that not every row of the block sees: their NaN and
+                // infinities out of the tile of values (add_not_finite)
+                if (!__all_sync(0xffffffffu,
+                                mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1, gone, WAIT_LIMIT_NS))) {
+                    if (lane == 0) give_up();
+                    ok = false;
+                    break;
+                }
+                bool found = false;
+                uint8_t *vt = v_sm + i % ST * C::KV_BYTES;
+                for (int e = row; e < C::KV_BYTES / 16; e += 128) {
+                    const int64_t key = key0 + e / 8 % BN;
+                    if (key >= sp.clo && key < min((int64_t) sp.chi, to)) continue;
+                    uint4 w = *reinterpret_cast<uint4 *>(vt + e * 16);
+                    uint32_t h[4] = { w.x, w.y, w.z, w.w };
+                    bool bad = false;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (bad_half<F16>(h[k])) h[k] &= 0xffff0000u, bad = true;
+                        if (bad_half<F16>(h[k] >> 16)) h[k] &= 0x0000ffffu, bad = true;
+                    }
+                    if (bad) {
+                        *reinterpret_cast<uint4 *>(vt + e * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                        found |= key < to;
+                    }
+                }
+                if (found) not_finite = 1;
+                fence_proxy_async_shared();
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < BN / 32; c++)
+#pragma unroll
+                for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(x[c][e]));
+            mx = fmaxf(m, mx * A.scale_log2);
+            if (i == 0) {
+                m = mx;
+            } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
+                // o relative to the new maxima; every product before is done
+                // (one score buffer: this tile's scores were issued after it)
+                if (NS > 1) {
+                    ok = mbar_wait_bounded(&pv_done, (i - 1) & 1, gone, WAIT_LIMIT_NS);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        if (lane == 0) give_up();
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                const float f = mx == m ? 1.0f : exp2_fast(m - mx);
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(o_at + c * 32, o);
+                    tmem_ld_wait(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st_32x32b_x32(o_at + c * 32, o);
+                }
+                l *= f;
+                m = mx;
+            }
+            const float base = m == -INFINITY ? 0.0f : -m;
+            float sum[4] = {};
+#pragma unroll
+            for (int h = 0; h < BN / 64; h++) {
+                uint32_t p[32];
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    float u = __uint_as_float(x[2 * h + e / 16][2 * e % 32]);
+                    float w = __uint_as_float(x[2 * h + e / 16][2 * e % 32 + 1]);
+                    fma2(u, w, A.scale_log2, base);
+                    u = exp2_fast(u);
+                    w = exp2_fast(w);
+                    sum[e & 1] += u;
+                    sum[2 + (e & 1)] += w;
+                    p[e] = kv_bits2<F16>(u, w);
+                }
+                tmem_st_32x32b_x32(s_at + h * 32, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[q * NS + b]);
+        }
+        // the last product
+        if (ok && n > 0) {
+            // by phases: the one before it may not have ended either
+            if (NS > 1 && n > 1) mbar_wait_bounded(&pv_done, (n - 2) & 1, gone, WAIT_LIMIT_NS);
+            ok = mbar_wait_bounded(&pv_done, NS > 1 ? (n - 1) & 1 : 0, gone, WAIT_LIMIT_NS);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) give_up();
+                ok = false;
+            }
+            tc_fence_after();
+        }
+        if (ok) {
+            const int head = kv_head * A.group + row % A.group;
+            const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
+            const float inv = A.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const int fa = (int) max((int64_t) lo, from), fz = (int) min((int64_t) hi, to);
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(o_at + c, o);
+                    tmem_ld_wait(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0;
+                }
+                if (!valid) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (c + e >= A.d) break;
+                    float r[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) r[k] = __uint_as_float(o[e + k]);
+                    if (not_finite) {
+                        add_not_finite<F16>(A, seq, kv_head, c + e, fa, min(fz, sp.clo), r);
+                        add_not_finite<F16>(A, seq, kv_head, c + e, max(fa, max(sp.chi, sp.clo)), fz, r);
+                    }
+                    if (A.splits > 1) {
+                        float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c + e);
+                        dst[0] = make_float4(r[0], r[1], r[2], r[3]);
+                        dst[1] = make_float4(r[4], r[5], r[6], r[7]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) r[k] *= inv;
+                        store8<F16>(A, tok, head, c + e, r);
+                    }
+                }
+            }
+            if (A.splits > 1 && valid) A.ml[slot] = make_float2(m, l);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::COLS);
+    }
+}
+
 // The chunks' parts of each row joined in order: the weights 2^(m_i - m) once
 // per row and thread, then eight columns a thread.
 template <int DP, bool F16>
@@ -531,9 +941,13 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // How a call runs: its row tiles, and the chunks its keys are cut into.
 struct attend_plan {
     int dp, tile_rows, splits;
+    bool many;
     int64_t row_tiles, chunk, ws_ml, ws_part;
 };
 
+// Up to 16 rows of a kv head go to the few-rows kernel: the cache's bytes
+// bound it, and its smaller blocks keep more of them in flight. More rows go
+// to the tensor-core tiles.
 // The keys are cut so that the blocks fill the GPU: one batch of resident
 // blocks where every sequence is as long as the next (one sequence), about
 // four where lengths differ, for balance; never below 256 keys a chunk.
@@ -541,16 +955,17 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
     attend_plan p;
     p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
     const int64_t group = at->heads / kv->kv_heads;
-    p.tile_rows = ROWS;
+    p.many = b->max_q * group > ROWS;
+    p.tile_rows = p.many ? (int) ((p.dp == 256 ? 1 : 2) * (128 / group) * group) : ROWS;
     p.row_tiles = std::max<int64_t>(1, up(b->max_q * group, p.tile_rows));
     const int64_t units = std::max<int64_t>(1, b->n_seqs * (int64_t) kv->kv_heads * p.row_tiles);
-    const int64_t per_sm = p.dp == 64 ? 3 : p.dp == 128 ? 2 : 1;
+    const int64_t per_sm = p.many ? 1 : p.dp == 64 ? 3 : p.dp == 128 ? 2 : 1;
     int64_t span = b->max_kv;
     if (at->causal && at->window)  // which may start inside a block of keys
         span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
     const int64_t want = 148 * per_sm * (b->n_seqs > 1 ? 4 : 1);
     const int64_t splits = std::max<int64_t>(1, want / units);
-    p.chunk = std::max<int64_t>(256, up(up(span, splits), KEYS) * KEYS);
+    p.chunk = std::max<int64_t>(p.many ? 512 : 256, up(up(span, splits), 2 * KEYS) * 2 * KEYS);
     p.splits = (int) std::max<int64_t>(1, up(span, p.chunk));
     p.ws_ml = p.ws_part = 0;
     if (p.splits > 1) {
@@ -566,33 +981,59 @@ const char *attend_fault(const zest_kv_cache *kv, const zest_kv_batch *b, const 
         return "heads are a multiple of the kv heads, at most 128 times";
     if (!(at->scale > 0.0f) || std::isinf(at->scale)) return "scale is not positive";
     if (at->window < 0 || (at->window > 0 && !at->causal)) return "a window is positive and causal";
-    if (up(b->max_q * (at->heads / kv->kv_heads), ROWS) * kv->kv_heads > 65535)
-        return "too many new tokens of one sequence";
+    if (plan_attend(kv, b, at).splits * (int64_t) kv->kv_heads > 65535) return "too many heads for the keys";
     return nullptr;
 }
 
-template <int DP, bool F16>
-int launch_few(const CUtensorMap &tk, const CUtensorMap &tv, const attend_args &a, const attend_plan &p, int kv_heads,
-               cudaStream_t st) {
-    using C = few_rows<DP>;
-    // per device: set with each device's first launch
-    static uint64_t ready = 0;
+// A step's queries as (value, head, token), in boxes of 64 values of a group
+// of heads and as many whole tokens as 128 rows hold.
+bool query_tmap(CUtensorMap *m, const attend_args &a) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = { (cuuint64_t) a.d, (cuuint64_t) a.heads, (cuuint64_t) a.b.T };
+    cuuint64_t strides[2] = { (cuuint64_t) a.d * 2, (cuuint64_t) a.ldq * 2 };
+    cuuint32_t box[3] = { 64, (cuuint32_t) a.group, (cuuint32_t) (128 / a.group) };
+    cuuint32_t estr[3] = { 1, 1, 1 };
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<uint16_t *>(a.q), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A kernel's dynamic shared memory allowed, on each device before its first launch there.
+template <typename K>
+bool allow_smem(K kernel, int bytes, uint64_t &ready) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return set_error("zest_kv_attend: no CUDA device");
-    if (dev >= 64 || !(__atomic_load_n(&ready, __ATOMIC_RELAXED) >> dev & 1)) {
-        if (cudaFuncSetAttribute(kv_attend_few_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 C::SMEM) != cudaSuccess)
-            return check_launch("zest_kv_attend");
-        if (dev < 64) __atomic_fetch_or(&ready, 1ull << dev, __ATOMIC_RELAXED);
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (dev < 64 && (__atomic_load_n(&ready, __ATOMIC_RELAXED) >> dev & 1)) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    if (dev < 64) __atomic_fetch_or(&ready, 1ull << dev, __ATOMIC_RELAXED);
+    return true;
+}
+
+template <int DP, bool F16>
+int launch_attend(const zest_kv_cache *kv, const CUtensorMap &tk, const CUtensorMap &tv, const attend_args &a,
+                  const attend_plan &p, cudaStream_t st) {
+    const char *call = "zest_kv_attend";
+    static uint64_t few_ready = 0, many_ready = 0;
+    if (p.many) {
+        using C = many_rows<DP>;
+        CUtensorMap tq;
+        if (!query_tmap(&tq, a)) return kv_refuse(call, "the queries' strides make no tensor map");
+        if (!allow_smem(kv_attend_many_kernel<DP, F16>, C::SMEM, many_ready)) return check_launch(call);
+        const dim3 grid((unsigned) p.row_tiles, (unsigned) (kv->kv_heads * p.splits), a.b.n_seqs);
+        kv_attend_many_kernel<DP, F16><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, a);
+    } else {
+        using C = few_rows<DP>;
+        if (!allow_smem(kv_attend_few_kernel<DP, F16>, C::SMEM, few_ready)) return check_launch(call);
+        const dim3 grid(p.splits, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
+        kv_attend_few_kernel<DP, F16><<<grid, FEW_THREADS, C::SMEM, st>>>(tk, tv, a);
     }
-    const dim3 grid(p.splits, (unsigned) (p.row_tiles * kv_heads), a.b.n_seqs);
-    kv_attend_few_kernel<DP, F16><<<grid, FEW_THREADS, C::SMEM, st>>>(tk, tv, a);
-    if (check_launch("zest_kv_attend")) return -1;
+    if (check_launch(call)) return -1;
     if (p.splits == 1) return 0;
     const int rows_b = 128 / (DP / 8);
-    const dim3 cg((unsigned) up(a.b.max_q * a.group, rows_b), kv_heads, a.b.n_seqs);
+    const dim3 cg((unsigned) up(a.b.max_q * a.group, rows_b), kv->kv_heads, a.b.n_seqs);
     kv_combine_kernel<DP, F16><<<cg, 128, 0, st>>>(a, p.tile_rows);
-    return check_launch("zest_kv_attend");
+    return check_launch(call);
 }
 
 }  // namespace
@@ -665,9 +1106,9 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     cudaStream_t st = (cudaStream_t) stream;
     const bool f16 = kv->type == ZEST_TYPE_F16;
     switch (p.dp) {
-        case 64: return f16 ? launch_few<64, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<64, false>(tk, tv, a, p, kv->kv_heads, st);
-        case 128: return f16 ? launch_few<128, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<128, false>(tk, tv, a, p, kv->kv_heads, st);
-        default: return f16 ? launch_few<256, true>(tk, tv, a, p, kv->kv_heads, st) : launch_few<256, false>(tk, tv, a, p, kv->kv_heads, st);
+        case 64: return f16 ? launch_attend<64, true>(kv, tk, tv, a, p, st) : launch_attend<64, false>(kv, tk, tv, a, p, st);
+        case 128: return f16 ? launch_attend<128, true>(kv, tk, tv, a, p, st) : launch_attend<128, false>(kv, tk, tv, a, p, st);
+        default: return f16 ? launch_attend<256, true>(kv, tk, tv, a, p, st) : launch_attend<256, false>(kv, tk, tv, a, p, st);
     }
 }
 

@@ -424,6 +424,36 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  : "memory");
 }
 
+// 32 lanes x 32 consecutive 32-bit columns written: thread i's registers to lane (base + i).
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+          "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16: A's rows are lanes, two 16-bit
+// values along K in each 32-bit column.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // --- CTA pairs (a cluster of 2 sharing one tcgen05 MMA) -----------------------
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -571,6 +601,15 @@ __device__ __forceinline__ uint64_t sw128_desc(const void *tile) {
            | ((1024ull >> 4) << 32)      // stride byte offset: next 8-row atom
            | (1ull << 46)                // descriptor version (sm_100)
            | (2ull << 61);               // SWIZZLE_128B
+}
+
+// The same for an MN-major 16-bit operand (rows along K, 64 values of N in a
+// 128-byte row): atoms of 8 rows 1 KB apart along K, the next 64 values of N
+// `block` bytes on.
+__device__ __forceinline__ uint64_t sw128_desc_mn(const void *tile, uint32_t block) {
+    const uint64_t addr = smem_u32(tile);
+    return ((addr & 0x3ffffu) >> 4) | ((uint64_t) ((block & 0x3ffffu) >> 4) << 16) | ((1024ull >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
 }
 
 }  // namespace zest
