@@ -9,9 +9,11 @@
 // base 2 (the scale times log2 e folded into one multiply-add):
 //   m' = max(m, s_j),  o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j,  l' alike.
 //
-// A long row of keys is cut into chunks that different blocks take (the grid's
-// x), each leaving its unnormalised o, m and l in the workspace, joined in
-// order by kv_combine_kernel; with one chunk the result is written at once.
+// A long row of keys is cut into chunks that different blocks take. Few rows
+// in at most 8 chunks: the blocks are one cluster and join their o, m and l
+// through each other's shared memory. More chunks, or many rows: each leaves
+// its unnormalised o, m and l in the workspace, joined in order by
+// kv_combine_kernel. With one chunk the result is written at once.
 #include "zest_kv.cuh"
 
 #include <algorithm>
@@ -43,6 +45,7 @@ struct attend_args {
     int64_t lda;
     int64_t chunk;      // keys a block takes, a multiple of 64; splits chunks at most
     int splits;
+    int join;           // the chunks' blocks are a cluster (few rows): each sequence in equal chunks
     float2 *ml;         // [splits][T * heads]: m and l
     float *part;        // [splits][T * heads][DP]: o
     unsigned *err;
@@ -189,10 +192,13 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     if (r0 >= rows) return;
     const key_span sp = span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + ROWS, rows) - 1) / A.group));
     // this block's keys: from the first of the span's 64-key block on, by chunks
-    const int64_t from = (int64_t) sp.lo / KEYS * KEYS + split * A.chunk;
-    const int64_t to = min((int64_t) sp.hi, from + A.chunk);
+    const int64_t first = (int64_t) sp.lo / KEYS * KEYS;
+    const int64_t chunk =
+        A.join ? ((max((int64_t) sp.hi - first, (int64_t) 1) + KEYS - 1) / KEYS + A.splits - 1) / A.splits * KEYS
+               : A.chunk;
+    const int64_t from = first + split * chunk, to = min((int64_t) sp.hi, from + chunk);
     const int steps = to > from ? (int) ((to - from + KEYS - 1) / KEYS) : 0;
-    if (steps == 0 && split > 0) return;  // kv_combine_kernel counts the chunks as this does
+    if (steps == 0 && split > 0 && !A.join) return;  // kv_combine_kernel counts the chunks as this does
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
@@ -248,6 +254,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         for (int k = max(0, i - C::STAGES); k < i; k++)
             mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
         __syncthreads();
+        if (A.join) {
+            cluster_sync();
+            cluster_sync();
+        }
         return;
     }
 
@@ -311,7 +321,8 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             }
         }
         // does every row see every key of this warp's?
-        const bool masked = key0 < sp.clo || key0 + 16 > min((int64_t) sp.chi, to) || r0 + ROWS > rows;
+        // (rows past the last hold zero queries, and their results go nowhere)
+        const bool masked = key0 < sp.clo || key0 + 16 > min((int64_t) sp.chi, to);
         if (masked) {
 #pragma unroll
             for (int n = 0; n < 2; n++)
@@ -412,10 +423,8 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             l_sh[warp][g + 8 * e] = l[e];
         }
     named_barrier(1, 128);
-    if (stop) return;  // a wait ran out: the rows stay as they were
     const int row = threadIdx.x >> 3;
     const int64_t r = r0 + row;
-    if (r >= rows) return;
     float mx = -INFINITY, w[4], sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; k++) mx = fmaxf(mx, m_sh[k][row]);
@@ -426,32 +435,89 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     }
     const int t = (int) (r / A.group), head = kv_head * A.group + (int) (r % A.group);
     const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
-    const float inv = A.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const bool live = r < rows && !stop;  // a wait that ran out leaves the rows as they were
 #pragma unroll
     for (int i = 0; i < DP / 64; i++) {
         const int c = (threadIdx.x & 7) * 8 + 64 * i;
-        if (c >= A.d) break;
         float x[8] = {};
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(os[(k * ROWS + row) * LD + c + e], w[k], x[e]);
-        if (not_finite) {
+        if (not_finite && live && c < A.d) {
             const int a = (int) max((int64_t) row_lo(A, s, t), from), z = (int) min((int64_t) row_hi(A, s, t), to);
             add_not_finite<F16>(A, seq, kv_head, c, a, min(z, sp.clo), x);
             add_not_finite<F16>(A, seq, kv_head, c, max(a, max(sp.chi, sp.clo)), z, x);
         }
-        if (A.splits > 1) {
-            float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c);
+        if (A.join) {  // over the first warp's part, which this thread alone reads
+            float4 *dst = reinterpret_cast<float4 *>(os + row * LD + c);
             dst[0] = make_float4(x[0], x[1], x[2], x[3]);
             dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
+        } else if (live && c < A.d) {
+            if (A.splits > 1) {
+                float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c);
+                dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] *= inv;
-            store8<F16>(A, tok, head, c, x);
+                for (int e = 0; e < 8; e++) x[e] *= inv;
+                store8<F16>(A, tok, head, c, x);
+            }
         }
     }
-    if (A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
+    if (!A.join) {
+        if (live && A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
+        return;
+    }
+    // the cluster's chunks joined in order, the rows' columns dealt to its blocks
+    __shared__ float2 ml_sh[ROWS];
+    if ((threadIdx.x & 7) == 0) ml_sh[row] = make_float2(stop ? NAN : mx, sum);
+    cluster_sync();
+    const int live_rows = (int) min((int64_t) ROWS, rows - r0);
+    for (int u = split * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.splits * 128) {
+        const int jr = u / (DP / 8), c = u % (DP / 8) * 8;
+        if (c >= A.d) continue;
+        float2 part[8];
+        float top = -INFINITY, total = 0.0f, x[8] = {};
+        bool whole = true;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < A.splits) {
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                             : "=f"(part[k].x), "=f"(part[k].y)
+                             : "r"(map_to_rank(&ml_sh[jr], k))
+                             : "memory");
+                whole = whole && part[k].x == part[k].x;
+                top = fmaxf(top, part[k].x);
+            }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < A.splits) {
+                const float f = part[k].x == -INFINITY ? 0.0f : exp2_fast(part[k].x - top);
+                total += f * part[k].y;
+                float4 a, b;
+                const uint32_t src = map_to_rank(os + jr * LD + c, k);
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(a.x), "=f"(a.y), "=f"(a.z), "=f"(a.w)
+                             : "r"(src)
+                             : "memory");
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(b.x), "=f"(b.y), "=f"(b.z), "=f"(b.w)
+                             : "r"(src + 16)
+                             : "memory");
+                const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(v[e], f, x[e]);
+            }
+        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= scale;
+        const int64_t jrow = r0 + jr;
+        if (whole)
+            store8<F16>(A, s.q0 + jrow / A.group, kv_head * A.group + (int) (jrow % A.group), c, x);
+    }
+    cluster_sync();  // nobody's shared memory goes while another reads it
 }
 
 // --- many rows: tcgen05 -------------------------------------------------------------
@@ -941,7 +1007,7 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // How a call runs: its row tiles, and the chunks its keys are cut into.
 struct attend_plan {
     int dp, tile_rows, splits;
-    bool many;
+    bool many, join;
     int64_t row_tiles, chunk, ws_ml, ws_part;
 };
 
@@ -950,7 +1016,8 @@ struct attend_plan {
 // to the tensor-core tiles.
 // The keys are cut so that the blocks fill the GPU: one batch of resident
 // blocks where every sequence is as long as the next (one sequence), about
-// four where lengths differ, for balance; never below 256 keys a chunk.
+// four where lengths differ, for balance; never below 128 keys a chunk (512
+// for many rows).
 attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
     attend_plan p;
     p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
@@ -965,10 +1032,11 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
         span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
     const int64_t want = 148 * per_sm * (b->n_seqs > 1 ? 4 : 1);
     const int64_t splits = std::max<int64_t>(1, want / units);
-    p.chunk = std::max<int64_t>(p.many ? 512 : 256, up(up(span, splits), 2 * KEYS) * 2 * KEYS);
+    p.chunk = std::max<int64_t>(p.many ? 512 : 128, up(up(span, splits), 2 * KEYS) * 2 * KEYS);
     p.splits = (int) std::max<int64_t>(1, up(span, p.chunk));
+    p.join = !p.many && p.splits > 1 && p.splits <= 8;
     p.ws_ml = p.ws_part = 0;
-    if (p.splits > 1) {
+    if (p.splits > 1 && !p.join) {
         p.ws_ml = up((int64_t) p.splits * b->T * at->heads * 8, 256) * 256;
         p.ws_part = (int64_t) p.splits * b->T * at->heads * p.dp * 4;
     }
@@ -1025,11 +1093,21 @@ int launch_attend(const zest_kv_cache *kv, const CUtensorMap &tk, const CUtensor
     } else {
         using C = few_rows<DP>;
         if (!allow_smem(kv_attend_few_kernel<DP, F16>, C::SMEM, few_ready)) return check_launch(call);
-        const dim3 grid(p.splits, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
-        kv_attend_few_kernel<DP, F16><<<grid, FEW_THREADS, C::SMEM, st>>>(tk, tv, a);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(p.splits, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
+        cfg.blockDim = dim3(FEW_THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.stream = st;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = p.join ? p.splits : 1;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kv_attend_few_kernel<DP, F16>, tk, tv, a);
     }
     if (check_launch(call)) return -1;
-    if (p.splits == 1) return 0;
+    if (p.splits == 1 || p.join) return 0;
     const int rows_b = 128 / (DP / 8);
     const dim3 cg((unsigned) up(a.b.max_q * a.group, rows_b), kv->kv_heads, a.b.n_seqs);
     kv_combine_kernel<DP, F16><<<cg, 128, 0, st>>>(a, p.tile_rows);
@@ -1100,6 +1178,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.lda = at->lda;
     a.chunk = p.chunk;
     a.splits = p.splits;
+    a.join = p.join;
     a.ml = (float2 *) workspace;
     a.part = (float *) ((uint8_t *) workspace + p.ws_ml);
     a.err = err;

@@ -21,20 +21,39 @@ namespace {
 // append
 // ---------------------------------------------------------------------------
 
-constexpr int AP_WARPS = 8, AP_MAX_D = 256;
+constexpr int AP_WARPS = 8;
 
-// The last sequence whose first row is t or before it, by a search that 32
-// lanes make together: each step cuts the range by 32 with one load. -1: none.
-__device__ __forceinline__ int kv_find_seq(const zest_kv_batch &b, int t, int lane) {
+// The sequence that row t may belong to: the last whose first row is t or
+// before it, by a search that 32 lanes make together (each step cuts the
+// range by 32), its bounds loaded with the last step. index -1: none.
+struct found_seq {
+    int index;
+    kv_seq s;
+};
+
+__device__ __forceinline__ found_seq kv_find_seq(const zest_kv_batch &b, int page_size, int t, int lane) {
     int lo = 0, hi = b.n_seqs;
     while (true) {
-        const int step = (hi - lo + 31) / 32;
-        const int at = lo + lane * step;
-        const unsigned m = __ballot_sync(0xffffffffu, at < hi && b.q_start[at] <= t);
-        if (!m) return -1;  // only ever in the first step: later ranges start at a sequence that holds
-        lo += (31 - __clz(m)) * step;
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        int a = 0, e = 0, kv = 0;
+        if (at < hi) {
+            a = b.q_start[at];
+            if (step == 1) {
+                e = b.q_start[at + 1];
+                kv = b.kv_len[at];
+            }
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, at < hi && a <= t);
+        if (!m) return { -1, {} };  // only ever in the first step: later ranges start at a sequence that holds
+        const int k = 31 - __clz(m);
+        lo += k * step;
         hi = min(hi, lo + step);
-        if (step == 1) return lo;
+        if (step == 1) {
+            a = __shfl_sync(0xffffffffu, a, k);
+            e = __shfl_sync(0xffffffffu, e, k);
+            kv = __shfl_sync(0xffffffffu, kv, k);
+            return { lo, kv_seq_from(b, page_size, a, e, kv) };
+        }
     }
 }
 
@@ -47,125 +66,164 @@ struct append_args {
     unsigned *err;
 };
 
-// A warp takes every (head row) of its share of a token: 4 values a lane and
-// 128 columns, so a head of 128 is one 16-byte load a lane. The row's sum of
-// squares by an xor tree, the norm and weight, the rotation with the partner
-// values read back from shared memory (NeoX pairs lie n_dims / 2 apart),
-// one rounding, 8-byte stores. Sums and rotations in f32 with explicitly
-// rounded products, as zest_norm_rope's.
-template <bool F16>
+constexpr int AP_ROWS = 4;  // head rows of a token that a warp has in flight
+
+// One head row of d values, 4 a lane and 128 columns (NC = 1: d <= 128), after
+// its norm and rotation, rounded and stored. f: this lane's cosines and sines,
+// the same for every head of a token; partner values of a NeoX pair (n_dims / 2
+// apart) come back from shared memory. Sums and rotations in f32 with
+// explicitly rounded products, as zest_norm_rope's.
+template <int NC, bool F16>
+__device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args &A, const float *w, bool turn,
+                                           const float (&co)[NC][4], const float (&si)[NC][4], float4 *buf,
+                                           uint16_t *dst) {
+    const int lane = threadIdx.x & 31, d = A.d;
+    const bool neox = A.in.mode == ZEST_ROPE_NEOX;
+    const int n_dims = A.in.rope ? A.in.n_dims : 0, half = n_dims / 2;
+    if (turn && A.in.eps >= 0.0f) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) ss = __fmaf_rn(v[c][e], v[c][e], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float sc = 1.0f / sqrtf(ss / (float) d + A.in.eps);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int j = 4 * lane + 128 * c;
+            const float4 f = w && j < d ? *reinterpret_cast<const float4 *>(w + j) : make_float4(1, 1, 1, 1);
+            const float wv[4] = { f.x, f.y, f.z, f.w };
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[c][e] = __fmul_rn(__fmul_rn(v[c][e], sc), wv[e]);
+        }
+    }
+    if (turn && n_dims) {
+        if (neox) {
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                if (4 * lane + 128 * c < d) buf[lane + 32 * c] = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
+            __syncwarp();
+        }
+        const float *row = reinterpret_cast<const float *>(buf);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int j0 = 4 * lane + 128 * c;
+            if (j0 >= n_dims) continue;
+            float x[4];
+            if (!neox) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = v[c][e ^ 1];
+            } else if (half % 4 == 0) {  // four values on one side of the middle, their partners side by side too
+                const float4 f = buf[(j0 < half ? j0 + half : j0 - half) / 4];
+                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = j0 + e;
+                    x[e] = j < n_dims ? row[j < half ? j + half : j - half] : 0.0f;
+                }
+            }
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = j0 + e;
+                const bool first = neox ? j < half : (j & 1) == 0;
+                o[e] = first ? __fsub_rn(__fmul_rn(v[c][e], co[c][e]), __fmul_rn(x[e], si[c][e]))
+                             : __fadd_rn(__fmul_rn(x[e], si[c][e]), __fmul_rn(v[c][e], co[c][e]));
+                if (j >= n_dims) o[e] = v[c][e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[c][e] = o[e];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int j = 4 * lane + 128 * c;
+        if (j < d) {
+            uint2 u;
+            u.x = kv_bits<F16>(v[c][0]) | (uint32_t) kv_bits<F16>(v[c][1]) << 16;
+            u.y = kv_bits<F16>(v[c][2]) | (uint32_t) kv_bits<F16>(v[c][3]) << 16;
+            *reinterpret_cast<uint2 *>(dst + j) = u;
+        }
+    }
+}
+
+// A block's share of a token's head rows (q, k, v), up to AP_ROWS a warp, all
+// loaded before anything is known of the token's sequence: the search for it
+// and the page's number are two loads, one after the other, that the rows'
+// loads run beside. Bound by the f32 rows' bytes in and the 16-bit ones out
+// for a chunk, by those loads' latency for a few tokens.
+template <int NC, bool F16>
 __global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_constant__ append_args A) {
-    __shared__ float4 buf[AP_WARPS][AP_MAX_D / 4];
+    __shared__ float4 buf[AP_WARPS][NC * 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = A.d;
-    float *row = reinterpret_cast<float *>(buf[warp]);
-    const int rows = A.q_heads + 2 * A.kv_heads;
+    const int rows = A.q_heads + 2 * A.kv_heads, step = gridDim.y * AP_WARPS;
     const bool neox = A.in.mode == ZEST_ROPE_NEOX;
     const int n_dims = A.in.rope ? A.in.n_dims : 0, half = n_dims / 2;
     for (int64_t t = blockIdx.x; t < A.b.T; t += gridDim.x) {
-        const int s = kv_find_seq(A.b, (int) t, lane);
-        if (s < 0) continue;
-        const kv_seq sq = kv_seq_of(A.b, A.page_size, s);
-        const int64_t i = t - sq.q0;
-        if (!sq.ok) {
-            if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
-            continue;
-        }
-        if (i >= sq.n) continue;  // behind the last sequence
-        const int64_t pos = (int64_t) sq.kv - sq.n + i;
-        int64_t at = -1;  // the token's place in the pools, in values
-        if (pos < 0) {
-            if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
-        } else {
-            const int64_t page = A.b.table[s * A.b.table_stride + pos / A.page_size];
-            if (page < 0 || page >= A.pages) {
-                if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
-            } else {
-                at = page * A.page_stride + pos % A.page_size * A.token_stride;
-            }
-        }
-        for (int r = blockIdx.y * AP_WARPS + warp; r < rows; r += gridDim.y * AP_WARPS) {
-            const bool is_q = r < A.q_heads, is_k = !is_q && r < A.q_heads + A.kv_heads;
-            if (!is_q && at < 0) break;
-            const float *x;
-            uint16_t *dst;
-            if (is_q) {
-                x = A.in.q + t * A.in.ldq + (int64_t) r * d;
-                dst = reinterpret_cast<uint16_t *>(A.in.q_out) + t * A.in.ldqo + (int64_t) r * d;
-            } else if (is_k) {
-                const int h = r - A.q_heads;
-                x = A.in.k + t * A.in.ldk + (int64_t) h * d;
-                dst = A.k + at + h * A.head_stride;
-            } else {
-                const int h = r - A.q_heads - A.kv_heads;
-                x = A.in.v + t * A.in.ldv + (int64_t) h * d;
-                dst = A.v + at + h * A.head_stride;
-            }
-            float v[2][4];
-            float ss = 0.0f;
+        for (int r0 = blockIdx.y * AP_WARPS + warp; r0 < rows; r0 += AP_ROWS * step) {
+            float v[AP_ROWS][NC][4];
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int j = 4 * lane + 128 * c;
-                const float4 f = j < d ? *reinterpret_cast<const float4 *>(x + j) : make_float4(0, 0, 0, 0);
-                v[c][0] = f.x, v[c][1] = f.y, v[c][2] = f.z, v[c][3] = f.w;
+            for (int k = 0; k < AP_ROWS; k++) {
+                const int r = r0 + k * step;
+                const float *x = r < A.q_heads               ? A.in.q + t * A.in.ldq + (int64_t) r * d
+                                 : r < A.q_heads + A.kv_heads ? A.in.k + t * A.in.ldk + (int64_t) (r - A.q_heads) * d
+                                                              : A.in.v + t * A.in.ldv +
+                                                                    (int64_t) (r - A.q_heads - A.kv_heads) * d;
 #pragma unroll
-                for (int e = 0; e < 4; e++) ss = __fmaf_rn(v[c][e], v[c][e], ss);
-            }
-            if (is_q || is_k) {
-                if (A.in.eps >= 0.0f) {
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    const float sc = 1.0f / sqrtf(ss / (float) d + A.in.eps);
-                    const float *w = is_q ? A.in.q_norm : A.in.k_norm;
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int j = 4 * lane + 128 * c;
-                        const float4 f = w && j < d ? *reinterpret_cast<const float4 *>(w + j) : make_float4(1, 1, 1, 1);
-                        const float wv[4] = { f.x, f.y, f.z, f.w };
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v[c][e] = __fmul_rn(__fmul_rn(v[c][e], sc), wv[e]);
-                    }
+                for (int c = 0; c < NC; c++) {
+                    const int j = 4 * lane + 128 * c;
+                    const float4 f =
+                        r < rows && j < d ? *reinterpret_cast<const float4 *>(x + j) : make_float4(0, 0, 0, 0);
+                    v[k][c][0] = f.x, v[k][c][1] = f.y, v[k][c][2] = f.z, v[k][c][3] = f.w;
                 }
-                if (n_dims) {
-                    const float *cs = A.in.rope + t * n_dims;
-                    if (neox) {
-                        __syncwarp();
+            }
+            float co[NC][4] = {}, si[NC][4] = {};
+            if (n_dims) {
+                const float *cs = A.in.rope + t * n_dims;
 #pragma unroll
-                        for (int c = 0; c < 2; c++)
-                            if (4 * lane + 128 * c < d)
-                                buf[warp][lane + 32 * c] = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
-                        __syncwarp();
-                    }
+                for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        float o[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int j = 4 * lane + 128 * c + e;
-                            o[e] = v[c][e];
-                            if (j < n_dims && j < d) {
-                                const bool first = neox ? j < half : (j & 1) == 0;
-                                const int p = neox ? (first ? j : j - half) : j >> 1;
-                                const float other = neox ? row[first ? j + half : j - half] : v[c][e ^ 1];
-                                const float x0 = first ? v[c][e] : other, x1 = first ? other : v[c][e];
-                                const float co = cs[2 * p], si = cs[2 * p + 1];
-                                o[e] = first ? __fsub_rn(__fmul_rn(x0, co), __fmul_rn(x1, si))
-                                             : __fadd_rn(__fmul_rn(x0, si), __fmul_rn(x1, co));
-                            }
+                    for (int e = 0; e < 4; e++) {
+                        const int j = 4 * lane + 128 * c + e, p = neox ? (j < half ? j : j - half) : j >> 1;
+                        if (j < n_dims) {
+                            const float2 f = *reinterpret_cast<const float2 *>(cs + 2 * p);
+                            co[c][e] = f.x;
+                            si[c][e] = f.y;
                         }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v[c][e] = o[e];
                     }
+            }
+            const found_seq at_seq = kv_find_seq(A.b, A.page_size, (int) t, lane);
+            const kv_seq &sq = at_seq.s;
+            if (at_seq.index < 0) break;
+            if (!sq.ok) {
+                if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+                break;
+            }
+            const int64_t i = t - sq.q0, pos = (int64_t) sq.kv - sq.n + i;
+            if (i >= sq.n) break;  // behind the last sequence
+            int64_t at = -1;       // the token's place in the pools, in values
+            if (pos < 0) {
+                if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
+            } else {
+                const int64_t page = A.b.table[at_seq.index * A.b.table_stride + pos / A.page_size];
+                if (page < 0 || page >= A.pages) {
+                    if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+                } else {
+                    at = page * A.page_stride + pos % A.page_size * A.token_stride;
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int j = 4 * lane + 128 * c;
-                if (j < d) {
-                    uint2 w;
-                    w.x = kv_bits<F16>(v[c][0]) | (uint32_t) kv_bits<F16>(v[c][1]) << 16;
-                    w.y = kv_bits<F16>(v[c][2]) | (uint32_t) kv_bits<F16>(v[c][3]) << 16;
-                    *reinterpret_cast<uint2 *>(dst + j) = w;
-                }
+            for (int k = 0; k < AP_ROWS; k++) {
+                const int r = r0 + k * step;
+                if (r >= rows || (r >= A.q_heads && at < 0)) continue;
+                const bool is_q = r < A.q_heads, is_k = !is_q && r < A.q_heads + A.kv_heads;
+                uint16_t *dst = is_q ? reinterpret_cast<uint16_t *>(A.in.q_out) + t * A.in.ldqo + (int64_t) r * d
+                                : is_k ? A.k + at + (r - A.q_heads) * A.head_stride
+                                       : A.v + at + (r - A.q_heads - A.kv_heads) * A.head_stride;
+                append_row<NC, F16>(v[k], A, is_q ? A.in.q_norm : A.in.k_norm, is_q || is_k, co, si, buf[warp], dst);
             }
         }
     }
@@ -595,11 +653,11 @@ int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
     if (!in || !err) return kv_refuse(call, "no new rows, or no device error word");
     const int64_t d = kv->d, wide = kv->kv_heads * d;
-    auto rows = [](const float *p, int64_t ld, int64_t n) { return p && ld >= n && ld % 4 == 0 && !((uintptr_t) p & 15); };
-    if (batch->T > 0 && (!rows(in->k, in->ldk, wide) || !rows(in->v, in->ldv, wide)))
+    auto good = [](const float *p, int64_t ld, int64_t n) { return p && ld >= n && ld % 4 == 0 && !((uintptr_t) p & 15); };
+    if (batch->T > 0 && (!good(in->k, in->ldk, wide) || !good(in->v, in->ldv, wide)))
         return kv_refuse(call, "k and v rows cover the heads and are 16-byte aligned");
     if (in->q) {
-        if (in->heads < 1 || in->heads > 65535 || !rows(in->q, in->ldq, in->heads * d) || !in->q_out ||
+        if (in->heads < 1 || in->heads > 65535 || !good(in->q, in->ldq, in->heads * d) || !in->q_out ||
             ((uintptr_t) in->q_out & 15) || in->ldqo < in->heads * d || in->ldqo % 8)
             return kv_refuse(call, "q rows cover the heads, and q and q_out are 16-byte aligned");
     }
@@ -609,6 +667,7 @@ int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     if (in->rope) {
         if (in->mode != ZEST_ROPE_NORMAL && in->mode != ZEST_ROPE_NEOX) return kv_refuse(call, "unsupported rope mode");
         if (in->n_dims <= 0 || in->n_dims % 2 || in->n_dims > d) return kv_refuse(call, "n_dims even and within d");
+        if ((uintptr_t) in->rope & 7) return kv_refuse(call, "the rope table is not 8-byte aligned");
     }
     if (batch->T == 0 || batch->n_seqs == 0) return 0;
     append_args a;
@@ -626,15 +685,18 @@ int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.d = kv->d;
     a.q_heads = in->q ? in->heads : 0;
     a.err = err;
-    // few tokens: a token's heads over several blocks, so that a step of a
-    // few rows is one row a warp; many: a block a token, which finds its
-    // sequence and page once
-    const int groups = (a.q_heads + 2 * a.kv_heads + AP_WARPS - 1) / AP_WARPS;
-    const int gx = (int) std::min<int64_t>(batch->T, 148 * 8);
-    const int gy = (int) std::min<int64_t>(groups, std::max<int64_t>(1, 148 * 8 / gx));
-    if (kv->type == ZEST_TYPE_F16)
-        kv_append_kernel<true><<<dim3(gx, gy), AP_WARPS * 32, 0, (cudaStream_t) stream>>>(a);
-    else kv_append_kernel<false><<<dim3(gx, gy), AP_WARPS * 32, 0, (cudaStream_t) stream>>>(a);
+    // a token's heads over as many blocks as give a warp AP_ROWS of them; few
+    // tokens: over more, down to one row a warp
+    const int rows = a.q_heads + 2 * a.kv_heads, most = (rows + AP_WARPS - 1) / AP_WARPS;
+    const int least = (rows + AP_WARPS * AP_ROWS - 1) / (AP_WARPS * AP_ROWS);
+    const int gx = (int) std::min<int64_t>(batch->T, 1 << 20);
+    const dim3 grid(gx, (int) std::min<int64_t>(most, std::max<int64_t>(least, 148 * 8 / gx)));
+    cudaStream_t st = (cudaStream_t) stream;
+    const bool f16 = kv->type == ZEST_TYPE_F16;
+    if (d <= 128 && f16) kv_append_kernel<1, true><<<grid, AP_WARPS * 32, 0, st>>>(a);
+    else if (d <= 128) kv_append_kernel<1, false><<<grid, AP_WARPS * 32, 0, st>>>(a);
+    else if (f16) kv_append_kernel<2, true><<<grid, AP_WARPS * 32, 0, st>>>(a);
+    else kv_append_kernel<2, false><<<grid, AP_WARPS * 32, 0, st>>>(a);
     return check_launch(call);
 }
 

@@ -19,15 +19,18 @@ struct kv_seq {
     bool ok;
 };
 
-__device__ __forceinline__ kv_seq kv_seq_of(const zest_kv_batch &b, int page_size, int s) {
+__device__ __forceinline__ kv_seq kv_seq_from(const zest_kv_batch &b, int page_size, int a, int e, int kv) {
     kv_seq r;
-    const int a = b.q_start[s], e = b.q_start[s + 1];
     r.q0 = a;
-    r.kv = b.kv_len[s];
+    r.kv = kv;
     r.ok = a >= 0 && e >= a && e <= b.T && (int64_t) e - a <= b.max_q && r.kv >= 0 && r.kv <= b.max_kv &&
            r.kv <= b.table_stride * page_size;
     r.n = r.ok ? e - a : 0;
     return r;
+}
+
+__device__ __forceinline__ kv_seq kv_seq_of(const zest_kv_batch &b, int page_size, int s) {
+    return kv_seq_from(b, page_size, b.q_start[s], b.q_start[s + 1], b.kv_len[s]);
 }
 
 // The bits of x rounded once (nearest even) to the cache's type. fp16 values

@@ -313,84 +313,87 @@ def plan_gemm(M: int, K: int, Ns, sms: int = 0) -> dict:
 
 
 # --- the paged key/value cache ------------------------------------------------
+#
+# A serving step makes a few of these calls a layer, so the checks that the C
+# ABI cannot make (types, devices, layouts of tensors) are kept to a few
+# attribute reads a tensor.
+
+_torch = None
 
 
-def _kv_stream(device: int):
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-class _on_device:
-    """The tensors' device current for one call (nothing to do where it already is)."""
-
-    __slots__ = ("device", "before")
-
-    def __init__(self, device: int):
-        self.device = device
-
-    def __enter__(self):
+def _tt():
+    global _torch
+    if _torch is None:
         import torch
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.device:
-            torch._C._cuda_setDevice(self.device)
-
-    def __exit__(self, *_):
-        import torch
-        if self.before != self.device:
-            torch._C._cuda_setDevice(self.before)
+        _torch = torch
+    return _torch
 
 
-def _dev_ptr(t, dtype, device: int, what: str):
-    """A tensor's address after the checks that the C ABI cannot make."""
-    if t.dtype != dtype or t.get_device() != device:
-        raise ZestError(f"{what}: a {dtype} tensor on the cache's device is wanted, not {t.dtype} on {t.device}")
+def _bad(what: str, wanted: str, t):
+    raise ZestError(f"{what}: {wanted} wanted, not {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+
+def _flat(t, dtype, device: int, n: int, what: str) -> int:
+    """The address of n or more values in one run."""
+    if t.dtype is not dtype or t.get_device() != device or t.numel() < n or not t.is_contiguous():
+        _bad(what, f"{n} contiguous values of {dtype} on cuda:{device}", t)
     return t.data_ptr()
 
 
-def _packed(t, dtype, device: int, n: int, what: str):
-    if not t.is_contiguous() or t.numel() < n:
-        raise ZestError(f"{what}: {n} contiguous values are wanted")
-    return _dev_ptr(t, dtype, device, what)
-
-
-def _heads_rows(t, dtype, device: int, T: int, heads: int, d: int, what: str):
-    """(address, row stride) of [T][heads][d] or [T][heads * d] rows whose values lie side by side."""
-    ok = t.shape[0] >= T and t.stride(-1) == 1 and (
-        t.shape[1:] == (heads * d,) or (t.shape[1:] == (heads, d) and (heads == 1 or t.stride(1) == d)))
-    if not ok:
-        raise ZestError(f"{what}: {T} rows of {heads} heads of {d}, each row in one run, are wanted")
-    return _dev_ptr(t, dtype, device, what), t.stride(0) if t.shape[0] > 1 else pad_to(heads * d, 8)
+def _rows(t, dtype, device: int, T: int, heads: int, d: int, what: str):
+    """(address, row stride) of [T][heads][d] or [T][heads * d], each row's values in one run."""
+    sh, st = t.shape, t.stride()
+    if t.dtype is not dtype or t.get_device() != device or sh[0] < T or st[-1] != 1 or not (
+            (len(sh) == 2 and sh[1] == heads * d) or
+            (len(sh) == 3 and sh[1] == heads and sh[2] == d and (st[1] == d or heads == 1))):
+        _bad(what, f"{T} rows of {heads} heads of {d} {dtype} values on cuda:{device}, each row in one run,", t)
+    return t.data_ptr(), st[0] if sh[0] > 1 else -(-heads * d // 8) * 8
 
 
 def _heads_of(t, d: int) -> int:
     return t.shape[1] if t.dim() == 3 else t.shape[-1] // d
 
 
-def _own_err(err, device: int):
-    import torch
-    return torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}") if err is None else err
-
-
-def _raise_err(err, given, what: str):
-    if given is None:
-        e = int(err.item())
-        if e:
-            raise ZestError(f"{what} raised device error bits {e:#x}")
+def _kv_call(fn, what: str, device: int, err, *args) -> None:
+    """One call with the device word and the current stream behind its arguments, on the tensors' device. With err
+    None the call gets a word of its own, waits and raises what it finds."""
+    torch = _torch or _tt()
+    own = err is None
+    if own:
+        err = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+    word = _flat(err, torch.int32, device, 1, "err")
+    before = torch._C._cuda_getDevice()
+    if before == device:
+        rc = fn(*args, word, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        torch._C._cuda_setDevice(device)
+        try:
+            rc = fn(*args, word, torch._C._cuda_getCurrentRawStream(device))
+        finally:
+            torch._C._cuda_setDevice(before)
+    if rc:
+        _check(rc, what)
+    if own and (e := int(err.item())):
+        raise ZestError(f"{what} raised device error bits {e:#x}")
 
 
 class KvCache:
     """zest_kv_cache over two tensors [layers][pages][page_size][kv_heads][d], bf16 or f16. They may
     be views in which heads come before tokens; the last dimension's values lie side by side."""
 
+    __slots__ = ("k", "v", "device", "dtype", "heads", "d", "pages", "desc", "ref")
+
     def __init__(self, k, v):
-        import torch
-        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.stride(4) != 1 or not k.is_cuda or \
-                k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype or v.device != k.device:
-            raise ZestError("KvCache: two 5-D bf16 or f16 cuda tensors of the same shape and strides are wanted")
-        self.k, self.v, self.device = k, v, k.get_device()
-        layers, pages, page, heads, d = k.shape
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), TYPE_BF16 if k.dtype == torch.bfloat16 else TYPE_F16,
-                                page, heads, d, layers, pages, *k.stride()[:4])
+        torch = _torch or _tt()
+        sh, st, dt, device = k.shape, k.stride(), k.dtype, k.get_device()
+        kind = TYPE_BF16 if dt is torch.bfloat16 else TYPE_F16 if dt is torch.float16 else None
+        if kind is None or len(sh) != 5 or device < 0 or st[4] != 1 or v.shape != sh or v.stride() != st or \
+                v.dtype is not dt or v.get_device() != device:
+            _bad("KvCache", "two 5-D bf16 or f16 cuda tensors of the same shape and strides", k)
+        self.k, self.v, self.device, self.dtype = k, v, device, dt
+        layers, self.pages, page, self.heads, self.d = sh
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), kind, page, self.heads, self.d, layers, self.pages,
+                                st[0], st[1], st[2], st[3])
         self.ref = ctypes.addressof(self.desc)
 
 
@@ -398,32 +401,30 @@ class KvBatch:
     """zest_kv_batch over int32 tensors: q_start [n + 1], kv_len [n], table [n][pages of the longest].
     max_q and max_kv bound the sequences' new and cached tokens (the launch is shaped by them)."""
 
+    __slots__ = ("tensors", "device", "T", "desc", "ref")
+
     def __init__(self, q_start, kv_len, table, T: int, max_q: int, max_kv: int):
-        import torch
-        n, device = kv_len.shape[0], kv_len.get_device()
-        if table.dim() != 2 or table.shape[0] < n or (table.shape[1] > 1 and table.stride(1) != 1):
-            raise ZestError("KvBatch: a table row for each sequence is wanted")
-        self.tensors = (q_start, kv_len, table)
-        # a row is as wide as its shape says; rows further apart are read at their stride
-        if table.shape[0] > 1 and table.stride(0) != table.shape[1]:
-            raise ZestError("KvBatch: table rows that follow one another are wanted")
-        self.desc = KvBatchDesc(_packed(q_start, torch.int32, device, n + 1, "q_start"),
-                                _packed(kv_len, torch.int32, device, n, "kv_len"),
-                                _dev_ptr(table, torch.int32, device, "table"), table.shape[1], T, max_q, max_kv, n)
-        self.device = device
+        i32 = (_torch or _tt()).int32
+        n, device, sh = kv_len.shape[0], kv_len.get_device(), table.shape
+        if len(sh) != 2 or sh[0] < n:
+            _bad("KvBatch", f"a page table of {n} rows", table)
+        self.tensors, self.device, self.T = (q_start, kv_len, table), device, T
+        self.desc = KvBatchDesc(_flat(q_start, i32, device, n + 1, "q_start"), _flat(kv_len, i32, device, n, "kv_len"),
+                                _flat(table, i32, device, 0, "table"), sh[1], T, max_q, max_kv, n)
         self.ref = ctypes.addressof(self.desc)
 
 
 class KvTables:
     """zest_kv_tables over int32 tensors: refs [pages], table [seqs][pages of the longest], len [seqs]."""
 
+    __slots__ = ("tensors", "device", "pages", "desc", "ref")
+
     def __init__(self, refs, table, lens):
-        import torch
-        device = refs.get_device()
+        i32 = (_torch or _tt()).int32
+        device, (seqs, width), self.pages = refs.get_device(), table.shape, refs.shape[0]
         self.tensors, self.device = (refs, table, lens), device
-        self.desc = KvTablesDesc(_packed(refs, torch.int32, device, 1, "refs"),
-                                 _packed(table, torch.int32, device, 1, "table"),
-                                 _packed(lens, torch.int32, device, table.shape[0], "len"), *table.shape)
+        self.desc = KvTablesDesc(_flat(refs, i32, device, 0, "refs"), _flat(table, i32, device, 0, "table"),
+                                 _flat(lens, i32, device, seqs, "len"), seqs, width)
         self.ref = ctypes.addressof(self.desc)
 
 
@@ -431,112 +432,103 @@ def kv_append(cache: KvCache, layer: int, batch: KvBatch, k, v, q=None, q_out=No
               eps: float = -1.0, rope=None, mode: int = ROPE_NEOX, err=None):
     """zest_kv_append: a step's f32 k and v [T][kv_heads][d] into their pages (k, and q into q_out, normed per head
     when eps >= 0 and rotated by `rope`, a zest_rope_table [T][n_dims])."""
-    import torch
-    f32, c, dev, T = torch.float32, cache.desc, cache.device, batch.desc.T
+    f32, dev, T, d = (_torch or _tt()).float32, cache.device, batch.T, cache.d
     if batch.device != dev:
         raise ZestError("kv_append: the batch lies on another device than the cache")
-    kp, ldk = _heads_rows(k, f32, dev, T, c.kv_heads, c.d, "k")
-    vp, ldv = _heads_rows(v, f32, dev, T, c.kv_heads, c.d, "v")
+    kp, ldk = _rows(k, f32, dev, T, cache.heads, d, "k")
+    vp, ldv = _rows(v, f32, dev, T, cache.heads, d, "v")
     qp, ldq, op, ldo, heads = None, 0, None, 0, 0
     if q is not None:
         if q_out is None:
             raise ZestError("kv_append: q needs q_out")
-        heads = _heads_of(q_out, c.d)
-        qp, ldq = _heads_rows(q, f32, dev, T, heads, c.d, "q")
-        op, ldo = _heads_rows(q_out, cache.k.dtype, dev, T, heads, c.d, "q_out")
-    w = [None if x is None else _packed(x, f32, dev, c.d, "norm weight") for x in (q_norm, k_norm)]
+        heads = _heads_of(q_out, d)
+        qp, ldq = _rows(q, f32, dev, T, heads, d, "q")
+        op, ldo = _rows(q_out, cache.dtype, dev, T, heads, d, "q_out")
+    qw = None if q_norm is None else _flat(q_norm, f32, dev, d, "q_norm")
+    kw = None if k_norm is None else _flat(k_norm, f32, dev, d, "k_norm")
     rp, n_dims = None, 0
     if rope is not None:
         n_dims = rope.shape[1]
-        rp = _packed(rope, f32, dev, T * n_dims, "rope")
-    given, err = err, _own_err(err, dev)
-    a = KvNew(kp, vp, ldk, ldv, qp, ldq, op, ldo, heads, eps, w[0], w[1], rp, n_dims, mode)
-    with _on_device(dev):
-        _check(lib().zest_kv_append(cache.ref, layer, batch.ref, ctypes.addressof(a),
-                                    _dev_ptr(err, torch.int32, dev, "err"), _kv_stream(dev)), "zest_kv_append")
-    _raise_err(err, given, "zest_kv_append")
+        rp = _flat(rope, f32, dev, T * n_dims, "rope")
+    a = KvNew(kp, vp, ldk, ldv, qp, ldq, op, ldo, heads, eps, qw, kw, rp, n_dims, mode)
+    _kv_call((_lib or lib()).zest_kv_append, "zest_kv_append", dev, err, cache.ref, layer, batch.ref,
+             ctypes.addressof(a))
 
 
 def kv_attend(cache: KvCache, layer: int, batch: KvBatch, q, scale: float | None = None, causal: bool = True,
               window: int = 0, out=None, y=None, a_next=None, workspace=None, err=None):
     """zest_kv_attend: the attention of q [T][heads][d] (the cache's type) over one layer. The result goes to out
     (the cache's type; made when no output is given), y (f32) and/or a_next (the o matmul's operand)."""
-    import torch
-    c, dev, T, dt = cache.desc, cache.device, batch.desc.T, cache.k.dtype
+    torch = _torch or _tt()
+    dev, T, dt, d = cache.device, batch.T, cache.dtype, cache.d
     if batch.device != dev:
         raise ZestError("kv_attend: the batch lies on another device than the cache")
-    heads = _heads_of(q, c.d)
-    qp, ldq = _heads_rows(q, dt, dev, T, heads, c.d, "q")
-    made = out is None and y is None and a_next is None
-    if made:
-        out = torch.zeros((T, heads, c.d), dtype=dt, device=q.device)
-    op = yp = ap = None
-    ldo = ldy = lda = 0
-    if out is not None:
-        op, ldo = _heads_rows(out, dt, dev, T, heads, c.d, "out")
-    if y is not None:
-        yp, ldy = _heads_rows(y, torch.float32, dev, T, heads, c.d, "y")
-    if a_next is not None:
-        ap, lda = _heads_rows(a_next, torch.int16, dev, T, heads, c.d, "a_next")
-    a = KvAttn(qp, ldq, heads, causal, window, c.d ** -0.5 if scale is None else scale, op, ldo, yp, ldy, ap, lda)
-    L, ref = lib(), ctypes.addressof(a)
-    with _on_device(dev):
-        need = L.zest_kv_attend_workspace(cache.ref, batch.ref, ref)
-        if need < 0:
-            _check(-1, "zest_kv_attend")
-        if need and workspace is None:
+    heads = _heads_of(q, d)
+    qp, ldq = _rows(q, dt, dev, T, heads, d, "q")
+    if out is None and y is None and a_next is None:
+        out = torch.zeros((T, heads, d), dtype=dt, device=q.device)
+    op, ldo = (None, 0) if out is None else _rows(out, dt, dev, T, heads, d, "out")
+    yp, ldy = (None, 0) if y is None else _rows(y, torch.float32, dev, T, heads, d, "y")
+    ap, lda = (None, 0) if a_next is None else _rows(a_next, torch.int16, dev, T, heads, d, "a_next")
+    a = KvAttn(qp, ldq, heads, causal, window, d ** -0.5 if scale is None else scale, op, ldo, yp, ldy, ap, lda)
+    L, ref = _lib or lib(), ctypes.addressof(a)
+    need = L.zest_kv_attend_workspace(cache.ref, batch.ref, ref)
+    if need < 0:
+        _check(-1, "zest_kv_attend")
+    ws, size = None, 0
+    if need:
+        if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        given, err = err, _own_err(err, dev)
-        ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        _check(L.zest_kv_attend(cache.ref, layer, batch.ref, ref, ws, size, _dev_ptr(err, torch.int32, dev, "err"),
-                                _kv_stream(dev)), "zest_kv_attend")
-    _raise_err(err, given, "zest_kv_attend")
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            _bad("kv_attend", f"a contiguous workspace on cuda:{dev}", workspace)
+        ws, size = workspace.data_ptr(), workspace.nbytes
+    _kv_call(L.zest_kv_attend, "zest_kv_attend", dev, err, cache.ref, layer, batch.ref, ref, ws, size)
     return out if out is not None else y if y is not None else a_next
 
 
-def _kv_pages(call: str, cache: KvCache, tables: KvTables, out, arrays, workspace, err):
-    import torch
-    out = tables if out is None else out
-    dev = cache.device
-    pages = cache.desc.pages
-    for t in (tables, out):
-        if t.device != dev or t.tensors[0].numel() < pages:
-            raise ZestError(f"{call}: tables on the cache's device, with a count for each page, are wanted")
-    n = arrays[0].numel() if arrays else 0
-    ptrs = [_packed(x, torch.int32, dev, n, call) for x in arrays]
-    L = lib()
-    given, err = err, _own_err(err, dev)
-    with _on_device(dev):
-        args = [cache.ref, tables.ref, out.ref] + ([n] if arrays else []) + ptrs
-        if call in ("zest_kv_fork", "zest_kv_compact"):
-            if workspace is None:
-                workspace = torch.empty(L.zest_kv_pages_workspace(cache.ref), dtype=torch.uint8, device=cache.k.device)
-            elif workspace.numel() * workspace.element_size() < L.zest_kv_pages_workspace(cache.ref):
-                raise ZestError(f"{call}: the workspace is smaller than zest_kv_pages_workspace says")
-            args.append(workspace.data_ptr())
-        _check(getattr(L, call)(*args, _dev_ptr(err, torch.int32, dev, "err"), _kv_stream(dev)), call)
-    _raise_err(err, given, call)
+def _kv_pages(call: str, cache: KvCache, tables: KvTables, out, arrays, workspace, err, moves: bool):
+    torch = _torch or _tt()
+    out, dev = tables if out is None else out, cache.device
+    if tables.device != dev or out.device != dev or tables.pages < cache.pages or out.pages < cache.pages:
+        raise ZestError(f"{call}: tables on the cache's device, with a count for each page, are wanted")
+    L = _lib or lib()
+    args = [cache.ref, tables.ref, out.ref]
+    if arrays:
+        n = arrays[0].shape[0]
+        args.append(n)
+        for x in arrays:
+            args.append(_flat(x, torch.int32, dev, n, call))
+    if moves:
+        need = L.zest_kv_pages_workspace(cache.ref)
+        if need < 0:
+            _check(-1, call)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=cache.k.device)
+        elif workspace.nbytes < need or workspace.get_device() != dev or not workspace.is_contiguous():
+            _bad(call, f"a workspace of {need} bytes on cuda:{dev}", workspace)
+        args.append(workspace.data_ptr())
+    _kv_call(getattr(L, call), call, dev, err, *args)
     return out
 
 
 def kv_grow(cache, tables, seq, add, out=None, err=None):
     """zest_kv_grow: room for add[i] more tokens of sequence seq[i]. Here as below, in place unless `out` is given."""
-    return _kv_pages("zest_kv_grow", cache, tables, out, (seq, add), None, err)
+    return _kv_pages("zest_kv_grow", cache, tables, out, (seq, add), None, err, False)
 
 
 def kv_fork(cache, tables, src, dst, out=None, workspace=None, err=None):
     """zest_kv_fork: the empty sequences dst[i] become copies of src[i]."""
-    return _kv_pages("zest_kv_fork", cache, tables, out, (src, dst), workspace, err)
+    return _kv_pages("zest_kv_fork", cache, tables, out, (src, dst), workspace, err, True)
 
 
 def kv_free(cache, tables, seq, out=None, err=None):
     """zest_kv_free: the sequences give their pages back."""
-    return _kv_pages("zest_kv_free", cache, tables, out, (seq,), None, err)
+    return _kv_pages("zest_kv_free", cache, tables, out, (seq,), None, err, False)
 
 
 def kv_compact(cache, tables, out=None, workspace=None, err=None):
     """zest_kv_compact: the pages in use moved to the front."""
-    return _kv_pages("zest_kv_compact", cache, tables, out, (), workspace, err)
+    return _kv_pages("zest_kv_compact", cache, tables, out, (), workspace, err, True)
 
 
 # --- the matmul service -------------------------------------------------------

@@ -336,7 +336,7 @@ typedef struct {
     int heads;
     float eps;                  /* of the per-head RMS_NORM of q and k; < 0: no norm */
     const float *q_norm, *k_norm; /* its weight rows of d (NULL: none), 16-byte aligned */
-    const float *rope;          /* NULL, or zest_rope_table's [T][n_dims]: q and k are rotated */
+    const float *rope;          /* NULL, or zest_rope_table's [T][n_dims], 8-byte aligned: q and k are rotated */
     int n_dims, mode;           /* as zest_rope */
 } zest_kv_new;
 

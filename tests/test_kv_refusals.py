@@ -112,7 +112,7 @@ def test_append():
                       (dict(ldv=1000), "k and v rows"), (dict(ldq=100), "q rows"), (dict(q_out=0), "q rows"),
                       (dict(ldqo=4100), "q rows"), (dict(heads=0), "q rows"), (dict(eps=float("nan")), "eps"),
                       (dict(q_norm=ODD), "norm weights"), (dict(mode=7), "rope mode"), (dict(n_dims=0), "n_dims"),
-                      (dict(n_dims=130), "n_dims"), (dict(n_dims=31), "n_dims")]:
+                      (dict(n_dims=130), "n_dims"), (dict(n_dims=31), "n_dims"), (dict(rope=ODD), "rope table")]:
         refused(append(i=new(**kw)), words)
 
 
