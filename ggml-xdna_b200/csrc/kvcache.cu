@@ -62,21 +62,32 @@ struct append_args {
     zest_kv_new in;
     uint16_t *k, *v;  // this layer
     int64_t page_stride, token_stride, head_stride, pages;
-    int page_size, kv_heads, d, q_heads;
+    int page_size, page_shift, kv_heads, d, q_heads;
+    float inv_d;
     unsigned *err;
 };
 
-constexpr int AP_ROWS = 4;  // head rows of a token that a warp has in flight
+// Head rows of a token that a warp has in flight.
+template <int NC>
+constexpr int AP_ROWS = NC == 1 ? 6 : 3;
+
+// What a token's heads share of the rotation: out = x * co + partner * si for
+// this lane's values (si negative for the first of a pair), and where a quad's
+// partners lie.
+template <int NC>
+struct turn_of {
+    float co[NC][4], si[NC][4];
+};
 
 // One head row of d values, 4 a lane and 128 columns (NC = 1: d <= 128), after
-// its norm and rotation, rounded and stored. f: this lane's cosines and sines,
-// the same for every head of a token; partner values of a NeoX pair (n_dims / 2
-// apart) come back from shared memory. Sums and rotations in f32 with
-// explicitly rounded products, as zest_norm_rope's.
+// its norm (w: this lane's weights) and rotation, rounded and stored. The
+// partners of a NeoX pair (n_dims / 2 apart) come back from shared memory.
+// Sums and rotations in f32 with explicitly rounded products; the scale is
+// 1 / sqrt to 2 units in the last place (rsqrtf): far below the one rounding
+// to 16 bits.
 template <int NC, bool F16>
-__device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args &A, const float *w, bool turn,
-                                           const float (&co)[NC][4], const float (&si)[NC][4], float4 *buf,
-                                           uint16_t *dst) {
+__device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args &A, const float (&w)[NC][4],
+                                           const turn_of<NC> &f, float4 *buf, uint16_t *dst, bool turn) {
     const int lane = threadIdx.x & 31, d = A.d;
     const bool neox = A.in.mode == ZEST_ROPE_NEOX;
     const int n_dims = A.in.rope ? A.in.n_dims : 0, half = n_dims / 2;
@@ -88,15 +99,11 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
             for (int e = 0; e < 4; e++) ss = __fmaf_rn(v[c][e], v[c][e], ss);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float sc = 1.0f / sqrtf(ss / (float) d + A.in.eps);
+        const float sc = rsqrtf(__fmaf_rn(ss, A.inv_d, A.in.eps));
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const int j = 4 * lane + 128 * c;
-            const float4 f = w && j < d ? *reinterpret_cast<const float4 *>(w + j) : make_float4(1, 1, 1, 1);
-            const float wv[4] = { f.x, f.y, f.z, f.w };
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[c][e] = __fmul_rn(__fmul_rn(v[c][e], sc), wv[e]);
-        }
+            for (int e = 0; e < 4; e++) v[c][e] = __fmul_rn(__fmul_rn(v[c][e], sc), w[c][e]);
     }
     if (turn && n_dims) {
         if (neox) {
@@ -116,8 +123,8 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[e] = v[c][e ^ 1];
             } else if (half % 4 == 0) {  // four values on one side of the middle, their partners side by side too
-                const float4 f = buf[(j0 < half ? j0 + half : j0 - half) / 4];
-                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+                const float4 q = buf[(j0 < half ? j0 + half : j0 - half) / 4];
+                x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -127,26 +134,21 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
             }
             float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + e;
-                const bool first = neox ? j < half : (j & 1) == 0;
-                o[e] = first ? __fsub_rn(__fmul_rn(v[c][e], co[c][e]), __fmul_rn(x[e], si[c][e]))
-                             : __fadd_rn(__fmul_rn(x[e], si[c][e]), __fmul_rn(v[c][e], co[c][e]));
-                if (j >= n_dims) o[e] = v[c][e];
+            for (int e = 0; e < 4; e++) o[e] = __fadd_rn(__fmul_rn(v[c][e], f.co[c][e]), __fmul_rn(x[e], f.si[c][e]));
+            v[c][0] = o[0];
+            v[c][1] = o[1];
+            if (j0 + 2 < n_dims) {  // n_dims may end in the middle of a quad
+                v[c][2] = o[2];
+                v[c][3] = o[3];
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[c][e] = o[e];
         }
     }
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int j = 4 * lane + 128 * c;
-        if (j < d) {
-            uint2 u;
-            u.x = kv_bits<F16>(v[c][0]) | (uint32_t) kv_bits<F16>(v[c][1]) << 16;
-            u.y = kv_bits<F16>(v[c][2]) | (uint32_t) kv_bits<F16>(v[c][3]) << 16;
-            *reinterpret_cast<uint2 *>(dst + j) = u;
-        }
+        if (j < d)
+            *reinterpret_cast<uint2 *>(dst + j) =
+                make_uint2(kv_bits2<F16>(v[c][0], v[c][1]), kv_bits2<F16>(v[c][2], v[c][3]));
     }
 }
 
@@ -157,21 +159,21 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
 // for a chunk, by those loads' latency for a few tokens.
 template <int NC, bool F16>
 __global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_constant__ append_args A) {
+    constexpr int N = AP_ROWS<NC>;
     __shared__ float4 buf[AP_WARPS][NC * 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = A.d;
-    const int rows = A.q_heads + 2 * A.kv_heads, step = gridDim.y * AP_WARPS;
+    const int q_rows = A.q_heads, k_rows = q_rows + A.kv_heads, rows = k_rows + A.kv_heads;
+    const int step = gridDim.y * AP_WARPS;
     const bool neox = A.in.mode == ZEST_ROPE_NEOX;
     const int n_dims = A.in.rope ? A.in.n_dims : 0, half = n_dims / 2;
     for (int64_t t = blockIdx.x; t < A.b.T; t += gridDim.x) {
-        for (int r0 = blockIdx.y * AP_WARPS + warp; r0 < rows; r0 += AP_ROWS * step) {
-            float v[AP_ROWS][NC][4];
+        const float *qx = A.in.q + t * A.in.ldq, *kx = A.in.k + t * A.in.ldk, *vx = A.in.v + t * A.in.ldv;
+        for (int r0 = blockIdx.y * AP_WARPS + warp; r0 < rows; r0 += N * step) {
+            float v[N][NC][4];
 #pragma unroll
-            for (int k = 0; k < AP_ROWS; k++) {
+            for (int k = 0; k < N; k++) {
                 const int r = r0 + k * step;
-                const float *x = r < A.q_heads               ? A.in.q + t * A.in.ldq + (int64_t) r * d
-                                 : r < A.q_heads + A.kv_heads ? A.in.k + t * A.in.ldk + (int64_t) (r - A.q_heads) * d
-                                                              : A.in.v + t * A.in.ldv +
-                                                                    (int64_t) (r - A.q_heads - A.kv_heads) * d;
+                const float *x = r < q_rows ? qx + r * d : r < k_rows ? kx + (r - q_rows) * d : vx + (r - k_rows) * d;
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     const int j = 4 * lane + 128 * c;
@@ -180,20 +182,26 @@ __global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_c
                     v[k][c][0] = f.x, v[k][c][1] = f.y, v[k][c][2] = f.z, v[k][c][3] = f.w;
                 }
             }
-            float co[NC][4] = {}, si[NC][4] = {};
-            if (n_dims) {
-                const float *cs = A.in.rope + t * n_dims;
+            turn_of<NC> turn = {};
+            float w[2][NC][4];
 #pragma unroll
-                for (int c = 0; c < NC; c++)
+            for (int c = 0; c < NC; c++) {
+                const int j0 = 4 * lane + 128 * c;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int j = 4 * lane + 128 * c + e, p = neox ? (j < half ? j : j - half) : j >> 1;
-                        if (j < n_dims) {
-                            const float2 f = *reinterpret_cast<const float2 *>(cs + 2 * p);
-                            co[c][e] = f.x;
-                            si[c][e] = f.y;
-                        }
+                for (int e = 0; e < 4; e++) {
+                    const int j = j0 + e, p = neox ? (j < half ? j : j - half) : j >> 1;
+                    if (j < n_dims) {
+                        const float2 f = *reinterpret_cast<const float2 *>(A.in.rope + t * n_dims + 2 * p);
+                        turn.co[c][e] = f.x;
+                        turn.si[c][e] = (neox ? j < half : (j & 1) == 0) ? -f.y : f.y;
                     }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float *src = h ? A.in.k_norm : A.in.q_norm;
+                    const float4 f = src && j0 < d ? *reinterpret_cast<const float4 *>(src + j0) : make_float4(1, 1, 1, 1);
+                    w[h][c][0] = f.x, w[h][c][1] = f.y, w[h][c][2] = f.z, w[h][c][3] = f.w;
+                }
             }
             const found_seq at_seq = kv_find_seq(A.b, A.page_size, (int) t, lane);
             const kv_seq &sq = at_seq.s;
@@ -202,28 +210,30 @@ __global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_c
                 if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
                 break;
             }
-            const int64_t i = t - sq.q0, pos = (int64_t) sq.kv - sq.n + i;
+            const int i = (int) (t - sq.q0), pos = sq.kv - sq.n + i;
             if (i >= sq.n) break;  // behind the last sequence
             int64_t at = -1;       // the token's place in the pools, in values
             if (pos < 0) {
                 if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
             } else {
-                const int64_t page = A.b.table[at_seq.index * A.b.table_stride + pos / A.page_size];
+                const int64_t page = A.b.table[at_seq.index * A.b.table_stride + (pos >> A.page_shift)];
                 if (page < 0 || page >= A.pages) {
                     if (lane == 0) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
                 } else {
-                    at = page * A.page_stride + pos % A.page_size * A.token_stride;
+                    at = page * A.page_stride + (pos & (A.page_size - 1)) * A.token_stride;
                 }
             }
+            uint16_t *qo = reinterpret_cast<uint16_t *>(A.in.q_out) + t * A.in.ldqo;
 #pragma unroll
-            for (int k = 0; k < AP_ROWS; k++) {
+            for (int k = 0; k < N; k++) {
                 const int r = r0 + k * step;
-                if (r >= rows || (r >= A.q_heads && at < 0)) continue;
-                const bool is_q = r < A.q_heads, is_k = !is_q && r < A.q_heads + A.kv_heads;
-                uint16_t *dst = is_q ? reinterpret_cast<uint16_t *>(A.in.q_out) + t * A.in.ldqo + (int64_t) r * d
-                                : is_k ? A.k + at + (r - A.q_heads) * A.head_stride
-                                       : A.v + at + (r - A.q_heads - A.kv_heads) * A.head_stride;
-                append_row<NC, F16>(v[k], A, is_q ? A.in.q_norm : A.in.k_norm, is_q || is_k, co, si, buf[warp], dst);
+                if (r >= rows || (r >= q_rows && at < 0)) continue;
+                if (r < q_rows) append_row<NC, F16>(v[k], A, w[0], turn, buf[warp], qo + r * d, true);
+                else
+                    append_row<NC, F16>(v[k], A, w[1], turn, buf[warp],
+                                        r < k_rows ? A.k + at + (r - q_rows) * A.head_stride
+                                                   : A.v + at + (r - k_rows) * A.head_stride,
+                                        r < k_rows);
             }
         }
     }
@@ -234,10 +244,10 @@ __global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 
 // The tables' part of each page operation is one block's work: ranks of free
-// and live pages by block scans over refs, 8 pages a thread and step, so a
-// pool of 8,192 pages is one step. Bound by latency, not bytes: the scan of
-// 13,000 counts and the rows of 32 sequences take a few microseconds.
-constexpr int PG_THREADS = 1024, PG_PER = 8, PG_STEP = PG_THREADS * PG_PER;
+// and live pages by block scans over refs, 16 pages a thread and step, so a
+// pool of 16,384 pages is one step. Bound by latency, not bytes: one dependent
+// load after another, so loads that do not depend go out together.
+constexpr int PG_THREADS = 1024, PG_PER = 16, PG_STEP = PG_THREADS * PG_PER;
 
 struct pages_shared {
     int warp[32];
@@ -276,28 +286,39 @@ __device__ __forceinline__ int block_scan(int v, pages_shared &sh, int &total) {
 }
 
 // The free (or, live = true, held) pages in [from, pages) in rising order:
-// f(rank, page, its count) for each with rank < limit. Every thread calls it;
-// returns how many there are up to the step where the limit was passed.
+// f(rank, page) for each with rank < limit. Every thread calls it; returns how
+// many there are up to the step where the limit was passed.
 template <typename F>
 __device__ __forceinline__ int64_t each_page(const int32_t *refs, int64_t from, int64_t pages, bool live,
                                              int64_t limit, pages_shared &sh, F f) {
+    const bool vec = ((uintptr_t) refs & 15) == 0;
     int64_t seen = 0;
-    for (int64_t base = from; base < pages && seen < limit; base += PG_STEP) {
+    for (int64_t base = from & ~(int64_t) 3; base < pages && seen < limit; base += PG_STEP) {
         const int64_t p0 = base + (int64_t) threadIdx.x * PG_PER;
-        int r[PG_PER], mine = 0;
+        int4 r[PG_PER / 4];
 #pragma unroll
-        for (int i = 0; i < PG_PER; i++) {
-            r[i] = p0 + i < pages ? refs[p0 + i] : (live ? 0 : 1);
-            mine += (r[i] != 0) == live;
+        for (int i = 0; i < PG_PER / 4; i++) {
+            const int64_t p = p0 + 4 * i;
+            if (vec && p + 4 <= pages) r[i] = *reinterpret_cast<const int4 *>(refs + p);
+            else
+                r[i] = make_int4(p < pages ? refs[p] : 0, p + 1 < pages ? refs[p + 1] : 0,
+                                 p + 2 < pages ? refs[p + 2] : 0, p + 3 < pages ? refs[p + 3] : 0);
         }
-        int total;
-        int64_t rank = seen + block_scan(mine, sh, total);
+        unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < PG_PER; i++)
-            if ((r[i] != 0) == live) {
-                if (rank < limit) f(rank, p0 + i, r[i]);
-                rank++;
-            }
+        for (int i = 0; i < PG_PER / 4; i++)
+            bits |= ((r[i].x != 0) | (r[i].y != 0) << 1 | (r[i].z != 0) << 2 | (r[i].w != 0) << 3) << (4 * i);
+        if (!live) bits = ~bits;
+        // only pages of [from, pages)
+        const int64_t n = min(max(pages - p0, (int64_t) 0), (int64_t) PG_PER), skip = max(from - p0, (int64_t) 0);
+        bits &= (1u << n) - 1u;
+        bits = skip < PG_PER ? bits & ~((1u << skip) - 1u) : 0u;
+        int total;
+        int64_t rank = seen + block_scan(__popc(bits), sh, total);
+        while (bits && rank < limit) {
+            f(rank++, p0 + __ffs(bits) - 1);
+            bits &= bits - 1;
+        }
         seen += total;
     }
     return seen;
@@ -312,16 +333,31 @@ struct pages_args {
     unsigned *err;
 };
 
+// n values copied by one block, four 16-byte loads a thread in flight.
+__device__ __forceinline__ void copy_values(int32_t *dst, const int32_t *src, int64_t n) {
+    if (dst == src) return;
+    int64_t done = 0;
+    if ((((uintptr_t) dst | (uintptr_t) src) & 15) == 0) {
+        const int64_t n4 = n / 4;
+        for (int64_t base = threadIdx.x; base < n4; base += 4 * PG_THREADS) {
+            int4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (base + i * PG_THREADS < n4) x[i] = reinterpret_cast<const int4 *>(src)[base + i * PG_THREADS];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (base + i * PG_THREADS < n4) reinterpret_cast<int4 *>(dst)[base + i * PG_THREADS] = x[i];
+        }
+        done = 4 * n4;
+    }
+    for (int64_t i = done + threadIdx.x; i < n; i += PG_THREADS) dst[i] = src[i];
+}
+
 // out := in, by one block (in and out may be the same).
-__device__ void copy_tables(const pages_args &A) {
-    if (A.in.refs != A.out.refs)
-        for (int64_t i = threadIdx.x; i < A.pages; i += blockDim.x) A.out.refs[i] = A.in.refs[i];
-    if (A.in.table != A.out.table)
-        for (int64_t i = threadIdx.x; i < A.in.seqs * A.in.table_stride; i += blockDim.x)
-            A.out.table[i] = A.in.table[i];
-    if (A.in.len != A.out.len)
-        for (int64_t i = threadIdx.x; i < A.in.seqs; i += blockDim.x) A.out.len[i] = A.in.len[i];
-    __syncthreads();
+__device__ __forceinline__ void copy_tables(const pages_args &A) {
+    copy_values(A.out.refs, A.in.refs, A.pages);
+    copy_values(A.out.table, A.in.table, A.in.seqs * A.in.table_stride);
+    copy_values(A.out.len, A.in.len, A.in.seqs);
 }
 
 // The same by many blocks, ahead of the operation's own, for tables that one
@@ -336,20 +372,22 @@ __global__ void __launch_bounds__(256) kv_copy_tables_kernel(const __grid_consta
         for (int64_t i = at; i < A.in.seqs; i += step) A.out.len[i] = A.in.len[i];
 }
 
-// Raises sh.bad (bits) where a sequence number is out of range or, with
-// `once`, appears twice among the first n of sh.who.
-__device__ void check_who(const pages_args &A, const int32_t *who, bool once, pages_shared &sh) {
-    if (threadIdx.x == 0) sh.bad = 0;
+// out := in, and the sequences named into sh.who; sh.bad gets bits where one
+// is out of range or, with `once`, appears twice. Ends with the block in step
+// and the copies visible to it.
+__device__ __forceinline__ void begin(const pages_args &A, const int32_t *who, bool once, pages_shared &sh) {
+    const int i = threadIdx.x, mine = i < A.n ? who[i] : 0;
+    if (i == 0) sh.bad = 0;
+    if (i < A.n) sh.who[i] = mine;
+    copy_tables(A);
     __syncthreads();
-    for (int i = threadIdx.x; i < A.n; i += blockDim.x) sh.who[i] = who[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < A.n; i += blockDim.x) {
-        bool bad = sh.who[i] < 0 || sh.who[i] >= A.in.seqs;
-        if (once)
-            for (int j = 0; j < i && !bad; j++) bad = sh.who[j] == sh.who[i];
-        if (bad) atomicOr(&sh.bad, (int) ZEST_ERR_BAD_SEQ);
-    }
-    __syncthreads();
+    bool bad = i < A.n && (mine < 0 || mine >= A.in.seqs);
+    if (once)  // every pair, dealt over the block
+        for (int e = i; e < A.n * A.n; e += PG_THREADS) {
+            const int a = e / A.n, b = e % A.n;
+            bad |= a < b && sh.who[a] == sh.who[b];
+        }
+    if (bad) atomicOr(&sh.bad, (int) ZEST_ERR_BAD_SEQ);
 }
 
 // The bits found so far; true: stop, out stays what copy_tables made it.
@@ -366,8 +404,7 @@ __device__ __forceinline__ bool give_up(const pages_args &A, pages_shared &sh) {
 
 __global__ void __launch_bounds__(PG_THREADS) kv_grow_kernel(const __grid_constant__ pages_args A) {
     __shared__ pages_shared sh;
-    copy_tables(A);
-    check_who(A, A.a, true, sh);
+    begin(A, A.a, true, sh);
     if (give_up(A, sh)) return;
     int need = 0, now = 0;
     const int i = threadIdx.x;
@@ -390,10 +427,10 @@ __global__ void __launch_bounds__(PG_THREADS) kv_grow_kernel(const __grid_consta
     if (i < A.n) sh.off[i] = before;
     if (threadIdx.x == 0) sh.off[A.n] = total;
     __syncthreads();
-    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t, int) {});
+    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t) {});
     if (threadIdx.x == 0 && (huge || there < total)) atomicOr(&sh.bad, (int) ZEST_ERR_NO_PAGES);
     if (give_up(A, sh)) return;
-    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page, int) {
+    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page) {
         int lo = 0, hi = A.n;  // the sequence with off[lo] <= rank < off[lo + 1]
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
@@ -408,8 +445,7 @@ __global__ void __launch_bounds__(PG_THREADS) kv_grow_kernel(const __grid_consta
 
 __global__ void __launch_bounds__(PG_THREADS) kv_free_kernel(const __grid_constant__ pages_args A) {
     __shared__ pages_shared sh;
-    copy_tables(A);
-    check_who(A, A.a, false, sh);
+    begin(A, A.a, false, sh);
     if (give_up(A, sh)) return;
     const int64_t w = A.out.table_stride, n = A.n * w;
     for (int64_t e = threadIdx.x; e < n; e += blockDim.x) {
@@ -426,8 +462,8 @@ __global__ void __launch_bounds__(PG_THREADS) kv_free_kernel(const __grid_consta
 
 __global__ void __launch_bounds__(PG_THREADS) kv_fork_kernel(const __grid_constant__ pages_args A) {
     __shared__ pages_shared sh;
-    copy_tables(A);
-    check_who(A, A.b, true, sh);  // dst, left in sh.who
+    begin(A, A.b, true, sh);  // dst, left in sh.who
+    __syncthreads();
     const int i = threadIdx.x, ps = A.page_size;
     int len = 0, src = 0, part = 0;
     if (i < A.n && !sh.bad) {
@@ -456,11 +492,11 @@ __global__ void __launch_bounds__(PG_THREADS) kv_fork_kernel(const __grid_consta
             if (page < 0 || page >= A.pages) atomicOr(&sh.bad, (int) ZEST_ERR_BAD_PAGE);
         }
     }
-    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t, int) {});
+    const int64_t there = each_page(A.out.refs, 0, A.pages, false, total, sh, [](int64_t, int64_t) {});
     if (threadIdx.x == 0 && there < total) atomicOr(&sh.bad, (int) ZEST_ERR_NO_PAGES);
     if (give_up(A, sh)) return;
     // the rank-th free page goes to the rank-th pair with a part page: by rank, then by pair
-    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page, int) {
+    each_page(A.out.refs, 0, A.pages, false, total, sh, [&](int64_t rank, int64_t page) {
         sh.held[rank] = (int) page;
     });
     __syncthreads();
@@ -495,21 +531,19 @@ __global__ void __launch_bounds__(PG_THREADS) kv_fork_kernel(const __grid_consta
 // many blocks suit its size.
 __global__ void __launch_bounds__(PG_THREADS) kv_compact_kernel(const __grid_constant__ pages_args A) {
     __shared__ pages_shared sh;
-    if (A.in.refs != A.out.refs)
-        for (int64_t i = threadIdx.x; i < A.pages; i += blockDim.x) A.out.refs[i] = A.in.refs[i];
-    if (A.in.len != A.out.len)
-        for (int64_t i = threadIdx.x; i < A.in.seqs; i += blockDim.x) A.out.len[i] = A.in.len[i];
+    copy_values(A.out.refs, A.in.refs, A.pages);
+    copy_values(A.out.len, A.in.len, A.in.seqs);
     int32_t *map = A.ws + 1 + 2 * A.pages;
     const int64_t all = A.pages;
     for (int64_t i = threadIdx.x; i < all; i += blockDim.x) map[i] = (int32_t) i;
     __syncthreads();
-    const int64_t live = each_page(A.out.refs, 0, all, true, all, sh, [](int64_t, int64_t, int) {});
-    const int64_t holes = each_page(A.out.refs, 0, live, false, all, sh, [&](int64_t rank, int64_t page, int) {
+    const int64_t live = each_page(A.out.refs, 0, all, true, all, sh, [](int64_t, int64_t) {});
+    const int64_t holes = each_page(A.out.refs, 0, live, false, all, sh, [&](int64_t rank, int64_t page) {
         A.ws[2 + 2 * rank] = (int32_t) page;
     });
     __syncthreads();
-    each_page(A.out.refs, live, all, true, all, sh, [&](int64_t rank, int64_t page, int count) {
-        const int to = A.ws[2 + 2 * rank];
+    each_page(A.out.refs, live, all, true, all, sh, [&](int64_t rank, int64_t page) {
+        const int to = A.ws[2 + 2 * rank], count = A.out.refs[page];
         A.ws[1 + 2 * rank] = (int32_t) page;
         map[page] = to;
         A.out.refs[to] = count;
@@ -683,12 +717,15 @@ int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.page_size = kv->page_size;
     a.kv_heads = kv->kv_heads;
     a.d = kv->d;
+    a.inv_d = 1.0f / (float) kv->d;
+    a.page_shift = 4;
+    while (1 << a.page_shift < kv->page_size) a.page_shift++;
     a.q_heads = in->q ? in->heads : 0;
     a.err = err;
     // a token's heads over as many blocks as give a warp AP_ROWS of them; few
     // tokens: over more, down to one row a warp
     const int rows = a.q_heads + 2 * a.kv_heads, most = (rows + AP_WARPS - 1) / AP_WARPS;
-    const int least = (rows + AP_WARPS * AP_ROWS - 1) / (AP_WARPS * AP_ROWS);
+    const int each = AP_WARPS * (d <= 128 ? AP_ROWS<1> : AP_ROWS<2>), least = (rows + each - 1) / each;
     const int gx = (int) std::min<int64_t>(batch->T, 1 << 20);
     const dim3 grid(gx, (int) std::min<int64_t>(most, std::max<int64_t>(least, 148 * 8 / gx)));
     cudaStream_t st = (cudaStream_t) stream;
