@@ -531,10 +531,11 @@ struct many_rows {
     static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
     static constexpr int NS = DP == 256 ? 2 : 1;    // score buffers of each
     static constexpr int BN = DP == 256 ? 64 : 128; // keys of a tile
-    static constexpr int STAGES = 2;                // of K, and of V
+    static constexpr int HALVES = BN / 64;          // a tile's weights are handed over 64 keys at a time
+    static constexpr int KST = 3, VST = 2;          // stages of K, and of V
     static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + (KST + VST) * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads
     static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for the MMAs, K's copies and V's
     // TMEM columns: O of each query tile, then its scores (P lies over them)
@@ -545,13 +546,95 @@ struct many_rows {
 // weights relative to the old one: they stay within 2^8, and o is not touched.
 constexpr float LAZY = 8.0f;
 
-__device__ __forceinline__ void fma2(float &a, float &b, float m, float c) {
-    asm("{\n\t.reg .b64 x, y, z;\n\t"
-        "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\t"
-        "mov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(a), "+f"(b)
-        : "f"(m), "f"(c));
+// Two f32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^u and 2^w without the exponential unit: x = n + f, n the nearest integer
+// (adding 1.5 * 2^23 leaves it in the low mantissa bits), 2^f by a polynomial
+// of degree 4 on [-1/2, 1/2] whose relative error, fitted to be even
+// (iteratively reweighted least squares), is 2^-18.5; n added to the
+// exponent. Below 2^-126 the result is 2^-126; u, w < 127, no NaN.
+__device__ __forceinline__ void exp2_poly(float &u, float &w) {
+    const float R = 12582912.0f;  // 1.5 * 2^23
+    const uint64_t x = pack2(fmaxf(u, -126.0f), fmaxf(w, -126.0f));
+    const uint64_t t = add2(x, pack2(R, R)), n = add2(t, pack2(-R, -R));
+    const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), x);
+    uint64_t p = pack2(9.5701022e-3f, 9.5701022e-3f);
+    p = fma2(p, f, pack2(5.5917859e-2f, 5.5917859e-2f));
+    p = fma2(p, f, pack2(2.4024744e-1f, 2.4024744e-1f));
+    p = fma2(p, f, pack2(6.9312179e-1f, 6.9312179e-1f));
+    p = fma2(p, f, pack2(9.9999928e-1f, 9.9999928e-1f));
+    float tu, tw;
+    unpack2(t, tu, tw);
+    unpack2(p, u, w);
+    u = __uint_as_float(__float_as_uint(u) + (__float_as_uint(tu) << 23));
+    w = __uint_as_float(__float_as_uint(w) + (__float_as_uint(tw) << 23));
+}
+
+// Waits as mbar_wait_bounded does, reading the clock only now and then: the
+// waits here are short and in the way of the next tile.
+__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile int *gone) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; it++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 63u) == 0) {
+            if (gone && *gone) return false;
+            const uint64_t now = global_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > WAIT_LIMIT_NS) return false;
+        }
+    }
+}
+
+// The weights of 64 keys: x in (bits of scores), 2^(x scale + base) rounded to
+// the cache's type and packed out, their f32 sums into s0 and s1. MIXED: one
+// pair of four by polynomial, so that the exponential unit (16 a clock and SM,
+// as long as the tile's products take) is not what the tile waits for.
+template <bool MIXED, bool F16>
+__device__ __forceinline__ void weights(const uint32_t *x, float scale, float base, uint32_t (&p)[32], uint64_t &s0,
+                                        uint64_t &s1) {
+    const uint64_t m = pack2(scale, scale), c = pack2(base, base);
+#pragma unroll
+    for (int e = 0; e < 32; e++) {
+        float u, w;
+        unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m, c), u, w);
+        if (MIXED && e % 4 == 3) {
+            exp2_poly(u, w);
+        } else {
+            u = exp2_fast(u);
+            w = exp2_fast(w);
+        }
+        if (e & 1) s1 = add2(s1, pack2(u, w));
+        else s0 = add2(s0, pack2(u, w));
+        p[e] = kv_bits2<F16>(u, w);
+    }
 }
 
 // A block: NQ x 128 rows of one kv head of one sequence over one chunk of
@@ -565,12 +648,12 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, NS = C::NS, BN = C::BN, ST = C::STAGES;
+    constexpr int NQ = C::NQ, NS = C::NS, BN = C::BN, KST = C::KST, VST = C::VST, H = C::HALVES;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
-    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + ST * C::KV_BYTES;
-    __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[NQ * NS], p_full[NQ * NS],
-        pv_done, drained;
+    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + KST * C::KV_BYTES;
+    __shared__ uint64_t q_full, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[NQ * NS],
+        p_full[NQ * NS * H], pv_done, drained;
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -596,16 +679,16 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     constexpr int W_MMA = C::SOFTMAX / 32, W_K = W_MMA + 1, W_V = W_MMA + 2;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        for (int i = 0; i < ST; i++) {
+        for (int i = 0; i < KST; i++) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < VST; i++) {
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
         }
-        for (int i = 0; i < NQ * NS; i++) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-        }
+        for (int i = 0; i < NQ * NS; i++) mbar_init(&s_full[i], 1);
+        for (int i = 0; i < NQ * NS * H; i++) mbar_init(&p_full[i], 4);
         mbar_init(&pv_done, 1);
         mbar_init(&drained, 1);
         stop = 0;
@@ -639,6 +722,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const CUtensorMap *map = is_v ? &tv : &tk;
         uint8_t *sm = is_v ? v_sm : k_sm;
         uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+        const int ST = is_v ? VST : KST;
         const int box = min(A.page_size, KEYS), boxes = BN / box;
         const int kb = lane % boxes, col = lane / boxes * 64;
         const bool mine = col < DP;
@@ -664,7 +748,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         for (; i < n; i++) {
             const int st = i % ST;
             const int next = page_of(i + 1);
-            const bool ok = i < ST || mbar_wait_bounded(&empty[st], (i / ST - 1) & 1, gone, WAIT_LIMIT_NS);
+            const bool ok = i < ST || wait_soon(&empty[st], (i / ST - 1) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 break;
@@ -684,65 +768,82 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         if (!is_v && n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_MMA) {
         fewer();
-        if (lane == 0 && n > 0) {
+        // the whole warp walks the loop, so that addresses and descriptors are
+        // uniform; one elected thread issues
+        if (n > 0) {
             constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
             constexpr uint32_t QK = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
             constexpr uint32_t PV = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
+            const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm), v_desc = sw128_desc_mn(v_sm, BN * 128);
             auto wait = [&](uint64_t *bar, int phase) {
-                if (mbar_wait_bounded(bar, phase & 1, gone, WAIT_LIMIT_NS)) {
+                if (__all_sync(0xffffffffu, wait_soon(bar, phase & 1, gone))) {
                     tc_fence_after();
                     return true;
                 }
-                give_up();
+                if (lane == 0) give_up();
                 return false;
             };
+            auto commit = [&](uint64_t *bar) {
+                if (elect_one()) tc_commit(bar);
+            };
             auto s_col = [&](int q, int b) { return tmem + C::S_COL + (q * NS + b) * BN; };
+            // a descriptor's address counts 16 bytes, and no tile passes its 18 bits
             auto scores = [&](int q, int i) {
-                const uint8_t *kt = k_sm + i % ST * C::KV_BYTES, *qt = q_sm + q * C::Q_BYTES;
-                const uint32_t d = s_col(q, NS > 1 ? i % NS : 0);
+                const uint64_t kt = k_desc + i % KST * (C::KV_BYTES >> 4), qt = q_desc + q * (C::Q_BYTES >> 4);
+                const int b = NS > 1 ? i % NS : 0;
+                const uint32_t d = s_col(q, b);
+                if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < DP / 16; ks++)
-                    tc_mma_bf16(d, sw128_desc(qt + ks / 4 * (128 * 128) + ks % 4 * 32),
-                                sw128_desc(kt + ks / 4 * (BN * 128) + ks % 4 * 32), QK, ks > 0);
-                tc_commit(&s_full[q * NS + (NS > 1 ? i % NS : 0)]);
+                    for (int ks = 0; ks < DP / 16; ks++)
+                        tc_mma_bf16(d, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
+                                    kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
+                    tc_commit(&s_full[q * NS + b]);
+                }
             };
             auto values = [&](int q, int i) {
-                const uint8_t *vt = v_sm + i % ST * C::KV_BYTES;
+                const int b = q * NS + (NS > 1 ? i % NS : 0);
+                const uint64_t vt = v_desc + i % VST * (C::KV_BYTES >> 4);
                 const uint32_t a = s_col(q, NS > 1 ? i % NS : 0);
 #pragma unroll
-                for (int ks = 0; ks < BN / 16; ks++)
-                    tc_mma_f16_ts(tmem + C::O_COL + q * DP, a + ks * 8, sw128_desc_mn(vt + ks * 16 * 128, BN * 128),
-                                  PV, i > 0 || ks > 0);
+                for (int h = 0; h < H; h++) {
+                    if (!wait(&p_full[b * H + h], i / NS)) return false;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 4 * h; ks < 4 * h + 4; ks++)
+                            tc_mma_f16_ts(tmem + C::O_COL + q * DP, a + ks * 8, vt + (ks * 16 * 128 >> 4), PV,
+                                          i > 0 || ks > 0);
+                    }
+                }
+                return true;
             };
             bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
             if (ok) {
                 for (int q = 0; q < nq; q++) scores(q, 0);
-                tc_commit(&k_empty[0]);
+                commit(&k_empty[0]);
             }
             for (int i = 0; ok && i < n; i++) {
                 const bool more = i + 1 < n;
                 if (NS > 1 && more) {  // the other buffer: its weights went into the product before
-                    if (!(ok = wait(&k_full[(i + 1) % ST], (i + 1) / ST))) break;
+                    if (!(ok = wait(&k_full[(i + 1) % KST], (i + 1) / KST))) break;
                     scores(0, i + 1);
-                    tc_commit(&k_empty[(i + 1) % ST]);
+                    commit(&k_empty[(i + 1) % KST]);
                 }
-                if (!(ok = wait(&v_full[i % ST], i / ST))) break;
+                if (!(ok = wait(&v_full[i % VST], i / VST))) break;
                 for (int q = 0; ok && q < nq; q++) {
-                    if (!(ok = wait(&p_full[q * NS + (NS > 1 ? i % NS : 0)], i / NS))) break;
-                    values(q, i);
-                    if (q == nq - 1) tc_commit(&v_empty[i % ST]);
+                    if (!(ok = values(q, i))) break;
+                    if (q == nq - 1) commit(&v_empty[i % VST]);
                     if (NS > 1 || i == n - 1) {
-                        if (q == nq - 1) tc_commit(&pv_done);
+                        if (q == nq - 1) commit(&pv_done);
                     }
                     if (NS == 1 && more) {
-                        if (q == 0 && !(ok = wait(&k_full[(i + 1) % ST], (i + 1) / ST))) break;
+                        if (q == 0 && !(ok = wait(&k_full[(i + 1) % KST], (i + 1) / KST))) break;
                         scores(q, i + 1);
-                        if (q == nq - 1) tc_commit(&k_empty[(i + 1) % ST]);
+                        if (q == nq - 1) commit(&k_empty[(i + 1) % KST]);
                     }
                 }
             }
             if (!ok) {  // what was issued still ends before TMEM goes
-                tc_commit(&drained);
+                commit(&drained);
                 mbar_wait_bounded(&drained, 0, nullptr, WAIT_LIMIT_NS);
             }
         }
@@ -763,7 +864,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         bool ok = q < nq;
         for (int i = 0; i < n && q < nq; i++) {
             const int b = NS > 1 ? i % NS : 0;
-            ok = mbar_wait_bounded(&s_full[q * NS + b], (i / NS) & 1, gone, WAIT_LIMIT_NS);
+            ok = wait_soon(&s_full[q * NS + b], (i / NS) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 ok = false;
@@ -777,7 +878,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
             const int64_t key0 = from + (int64_t) i * BN;
-            if (key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to)) {
+            const bool masked = key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to);
+            if (masked) {
                 const int a = (int) (max((int64_t) lo, key0) - key0), z = (int) (min((int64_t) hi, to) - key0);
 #pragma unroll
                 for (int c = 0; c < BN / 32; c++)
@@ -789,13 +891,13 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
                 if (!__all_sync(0xffffffffu,
-                                mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1, gone, WAIT_LIMIT_NS))) {
+                                wait_soon(&v_full[i % VST], (i / VST) & 1, gone))) {
                     if (lane == 0) give_up();
                     ok = false;
                     break;
                 }
                 bool found = false;
-                uint8_t *vt = v_sm + i % ST * C::KV_BYTES;
+                uint8_t *vt = v_sm + i % VST * C::KV_BYTES;
                 for (int e = row; e < C::KV_BYTES / 16; e += 128) {
                     const int64_t key = key0 + e / 8 % BN;
                     if (key >= sp.clo && key < min((int64_t) sp.chi, to)) continue;
@@ -815,19 +917,25 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 if (found) not_finite = 1;
                 fence_proxy_async_shared();
             }
-            float mx = -INFINITY;
+            float top[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
             for (int c = 0; c < BN / 32; c++)
 #pragma unroll
-                for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(x[c][e]));
-            mx = fmaxf(m, mx * A.scale_log2);
+                for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        top[k] = max3_nan(top[k], __uint_as_float(x[c][e + k]), __uint_as_float(x[c][e + 4 + k]));
+            float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * A.scale_log2;
+            // a NaN or an infinite score: the row's weights are NaN, as the formula's
+            const bool odd = !(mx < INFINITY);
+            mx = odd ? m : fmaxf(m, mx);
             if (i == 0) {
                 m = mx;
             } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
                 // o relative to the new maxima; every product before is done
                 // (one score buffer: this tile's scores were issued after it)
                 if (NS > 1) {
-                    ok = mbar_wait_bounded(&pv_done, (i - 1) & 1, gone, WAIT_LIMIT_NS);
+                    ok = wait_soon(&pv_done, (i - 1) & 1, gone);
                     if (!__all_sync(0xffffffffu, ok)) {
                         if (lane == 0) give_up();
                         ok = false;
@@ -848,35 +956,29 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 l *= f;
                 m = mx;
             }
-            const float base = m == -INFINITY ? 0.0f : -m;
-            float sum[4] = {};
+            const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
+            uint64_t s0 = 0, s1 = 0;
 #pragma unroll
-            for (int h = 0; h < BN / 64; h++) {
+            for (int h = 0; h < H; h++) {
                 uint32_t p[32];
-#pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    float u = __uint_as_float(x[2 * h + e / 16][2 * e % 32]);
-                    float w = __uint_as_float(x[2 * h + e / 16][2 * e % 32 + 1]);
-                    fma2(u, w, A.scale_log2, base);
-                    u = exp2_fast(u);
-                    w = exp2_fast(w);
-                    sum[e & 1] += u;
-                    sum[2 + (e & 1)] += w;
-                    p[e] = kv_bits2<F16>(u, w);
-                }
+                if (masked) weights<false, F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, s0, s1);
+                else weights<true, F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, s0, s1);
                 tmem_st_32x32b_x32(s_at + h * 32, p);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[(q * NS + b) * H + h]);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[q * NS + b]);
+            float sa, sb, sc, sd;
+            unpack2(s0, sa, sb);
+            unpack2(s1, sc, sd);
+            l += (sa + sb) + (sc + sd);
         }
         // the last product
         if (ok && n > 0) {
             // by phases: the one before it may not have ended either
-            if (NS > 1 && n > 1) mbar_wait_bounded(&pv_done, (n - 2) & 1, gone, WAIT_LIMIT_NS);
-            ok = mbar_wait_bounded(&pv_done, NS > 1 ? (n - 1) & 1 : 0, gone, WAIT_LIMIT_NS);
+            if (NS > 1 && n > 1) wait_soon(&pv_done, (n - 2) & 1, gone);
+            ok = wait_soon(&pv_done, NS > 1 ? (n - 1) & 1 : 0, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 ok = false;

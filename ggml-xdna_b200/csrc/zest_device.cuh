@@ -222,6 +222,18 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return (uint32_t) __cvta_generic_to_shared(p);
 }
 
+// One lane of a converged warp, in a way that tells the compiler that what it
+// guards runs in one thread with warp-uniform operands.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ uint64_t global_ns() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
