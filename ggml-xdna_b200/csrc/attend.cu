@@ -546,56 +546,11 @@ struct many_rows {
 // weights relative to the old one: they stay within 2^8, and o is not touched.
 constexpr float LAZY = 8.0f;
 
-// Two f32 operations an instruction.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-
-__device__ __forceinline__ void unpack2(uint64_t p, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-// 2^u and 2^w without the exponential unit: x = n + f, n the nearest integer
-// (adding 1.5 * 2^23 leaves it in the low mantissa bits), 2^f by a polynomial
-// of degree 4 on [-1/2, 1/2] whose relative error, fitted to be even
-// (iteratively reweighted least squares), is 2^-18.5; n added to the
-// exponent. Below 2^-126 the result is 2^-126; u, w < 127, no NaN.
-__device__ __forceinline__ void exp2_poly(float &u, float &w) {
-    const float R = 12582912.0f;  // 1.5 * 2^23
-    const uint64_t x = pack2(fmaxf(u, -126.0f), fmaxf(w, -126.0f));
-    const uint64_t t = add2(x, pack2(R, R)), n = add2(t, pack2(-R, -R));
-    const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), x);
-    uint64_t p = pack2(9.5701022e-3f, 9.5701022e-3f);
-    p = fma2(p, f, pack2(5.5917859e-2f, 5.5917859e-2f));
-    p = fma2(p, f, pack2(2.4024744e-1f, 2.4024744e-1f));
-    p = fma2(p, f, pack2(6.9312179e-1f, 6.9312179e-1f));
-    p = fma2(p, f, pack2(9.9999928e-1f, 9.9999928e-1f));
-    float tu, tw;
-    unpack2(t, tu, tw);
-    unpack2(p, u, w);
-    u = __uint_as_float(__float_as_uint(u) + (__float_as_uint(tu) << 23));
-    w = __uint_as_float(__float_as_uint(w) + (__float_as_uint(tw) << 23));
 }
 
 // Waits as mbar_wait_bounded does, reading the clock only now and then: the
@@ -614,25 +569,18 @@ __device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volati
 }
 
 // The weights of 64 keys: x in (bits of scores), 2^(x scale + base) rounded to
-// the cache's type and packed out, their f32 sums into s0 and s1. MIXED: one
-// pair of four by polynomial, so that the exponential unit (16 a clock and SM,
-// as long as the tile's products take) is not what the tile waits for.
-template <bool MIXED, bool F16>
-__device__ __forceinline__ void weights(const uint32_t *x, float scale, float base, uint32_t (&p)[32], uint64_t &s0,
-                                        uint64_t &s1) {
-    const uint64_t m = pack2(scale, scale), c = pack2(base, base);
+// the cache's type and packed out, their f32 sums into s. Plain f32 operations:
+// 278 clocks for 64 keys of two warps of a scheduler, where paired f32x2 ones
+// around the exponentials took 624, and a quarter of the exponentials by a
+// polynomial 309.
+template <bool F16>
+__device__ __forceinline__ void weights(const uint32_t *x, float scale, float base, uint32_t (&p)[32], float (&s)[4]) {
 #pragma unroll
     for (int e = 0; e < 32; e++) {
-        float u, w;
-        unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m, c), u, w);
-        if (MIXED && e % 4 == 3) {
-            exp2_poly(u, w);
-        } else {
-            u = exp2_fast(u);
-            w = exp2_fast(w);
-        }
-        if (e & 1) s1 = add2(s1, pack2(u, w));
-        else s0 = add2(s0, pack2(u, w));
+        const float u = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e]), scale, base));
+        const float w = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e + 1]), scale, base));
+        s[e & 1] += u;
+        s[2 + (e & 1)] += w;
         p[e] = kv_bits2<F16>(u, w);
     }
 }
@@ -878,8 +826,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
             const int64_t key0 = from + (int64_t) i * BN;
-            const bool masked = key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to);
-            if (masked) {
+            if (key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to)) {
                 const int a = (int) (max((int64_t) lo, key0) - key0), z = (int) (min((int64_t) hi, to) - key0);
 #pragma unroll
                 for (int c = 0; c < BN / 32; c++)
@@ -957,22 +904,18 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 m = mx;
             }
             const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
-            uint64_t s0 = 0, s1 = 0;
+            float sum[4] = {};
 #pragma unroll
             for (int h = 0; h < H; h++) {
                 uint32_t p[32];
-                if (masked) weights<false, F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, s0, s1);
-                else weights<true, F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, s0, s1);
+                weights<F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, sum);
                 tmem_st_32x32b_x32(s_at + h * 32, p);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[(q * NS + b) * H + h]);
             }
-            float sa, sb, sc, sd;
-            unpack2(s0, sa, sb);
-            unpack2(s1, sc, sd);
-            l += (sa + sb) + (sc + sd);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         // the last product
         if (ok && n > 0) {
