@@ -522,23 +522,21 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 
 // --- many rows: tcgen05 -------------------------------------------------------------
 
-// Shapes by padded head size. Two tiles of 128 query rows share each tile of
-// keys and values (one tile where the head is 256 wide, whose scores then have
-// two buffers): while one tile's rows take their exponentials, the tensor
-// cores work for the other.
+// Shapes by padded head size. A block's query tiles of 128 rows share each tile
+// of 64 keys and values. Each has two score buffers in TMEM: the next tile's
+// scores are there before this tile's weights are done, so the softmax warps
+// never wait for a product and the tensor cores work beside them.
 template <int DP>
 struct many_rows {
-    static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
-    static constexpr int NS = DP == 256 ? 2 : 1;    // score buffers of each
-    static constexpr int BN = DP == 256 ? 64 : 128; // keys of a tile
-    static constexpr int HALVES = BN / 64;          // a tile's weights are handed over 64 keys at a time
-    static constexpr int KST = 3, VST = 2;          // stages of K, and of V
+    static constexpr int NQ = DP == 256 ? 1 : 2;  // query tiles of a block
+    static constexpr int BN = 64;                 // keys of a tile
     static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int SMEM = 1024 + NQ * Q_BYTES + (KST + VST) * KV_BYTES;
-    static constexpr int SOFTMAX = NQ * 128;        // threads
-    static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for the MMAs, K's copies and V's
-    // TMEM columns: O of each query tile, then its scores (P lies over them)
+    static constexpr int ST = DP == 256 ? 2 : 4;  // stages, of a tile of K and one of V
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + ST * 2 * KV_BYTES;
+    static constexpr int SOFTMAX = NQ * 128;      // threads: one a row
+    static constexpr int THREADS = SOFTMAX + 64;  // and a warp each for the MMAs and the copies
+    // TMEM columns: O of each query tile, then its two score buffers (P lies over them)
     static constexpr int O_COL = 0, S_COL = NQ * DP, COLS = 512;
 };
 
@@ -553,19 +551,20 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return r;
 }
 
-// Waits as mbar_wait_bounded does, reading the clock only now and then: the
-// waits here are short and in the way of the next tile.
-__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile int *gone) {
-    uint64_t t0 = 0;
+// The rest of a wait whose first look found nothing, for at most WAIT_LIMIT_NS
+// or until *gone. Out of line: the warps of a block share the instruction
+// caches, and a warp that issues MMAs between others' long straight code pays
+// for every line of its own.
+__device__ __noinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile int *gone) {
+    const uint64_t t0 = global_ns();
     for (uint32_t it = 1;; it++) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 0) {
-            if (gone && *gone) return false;
-            const uint64_t now = global_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > WAIT_LIMIT_NS) return false;
-        }
+        if ((it & 63u) == 0 && ((gone && *gone) || global_ns() - t0 > WAIT_LIMIT_NS)) return false;
     }
+}
+
+__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile int *gone) {
+    return mbar_try_wait(bar, parity) || wait_on(bar, parity, gone);
 }
 
 // The weights of 64 keys: x in (bits of scores), 2^(x scale + base) rounded to
@@ -596,12 +595,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, NS = C::NS, BN = C::BN, KST = C::KST, VST = C::VST, H = C::HALVES;
+    constexpr int NQ = C::NQ, BN = C::BN, ST = C::ST;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
-    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + KST * C::KV_BYTES;
-    __shared__ uint64_t q_full, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[NQ * NS],
-        p_full[NQ * NS * H], pv_done, drained;
+    uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // a stage: a tile of K, then one of V
+    __shared__ uint64_t q_full, full[ST], empty[ST], s_full[NQ][2], p_full[NQ][2], pv_done[NQ], drained;
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -619,25 +617,24 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     if (t0 >= t1) return;
     const int nq = NQ > 1 && t0 + per_tile < t1 ? 2 : 1;  // query tiles that have rows
     const key_span sp = span_of(A, s, t0, t1 - 1);
-    const int64_t from = (int64_t) sp.lo / KEYS * KEYS + split * A.chunk;
-    const int64_t to = min((int64_t) sp.hi, from + A.chunk);
-    const int n = to > from ? (int) ((to - from + BN - 1) / BN) : 0;
+    const int from = (int) min((int64_t) sp.lo / KEYS * KEYS + split * A.chunk, (int64_t) sp.hi);
+    const int to = (int) min((int64_t) sp.hi, from + A.chunk), n = max(0, (to - from + BN - 1) / BN);
     if (n == 0 && split > 0) return;
 
-    constexpr int W_MMA = C::SOFTMAX / 32, W_K = W_MMA + 1, W_V = W_MMA + 2;
+    constexpr int W_MMA = C::SOFTMAX / 32, W_COPY = W_MMA + 1;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        for (int i = 0; i < KST; i++) {
-            mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 1);
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < VST; i++) {
-            mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], 1);
+        for (int i = 0; i < NQ; i++) {
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&s_full[i][b], 1);
+                mbar_init(&p_full[i][b], 4);
+            }
+            mbar_init(&pv_done[i], 1);
         }
-        for (int i = 0; i < NQ * NS; i++) mbar_init(&s_full[i], 1);
-        for (int i = 0; i < NQ * NS * H; i++) mbar_init(&p_full[i], 4);
-        mbar_init(&pv_done, 1);
         mbar_init(&drained, 1);
         stop = 0;
         not_finite = 0;
@@ -657,24 +654,16 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         atomicOr(A.err, ERR_TIMEOUT);
     };
 
-    // A row of scores lives in registers: the softmax warps take the others'
-    // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
-    auto fewer = [] {
-        if (NQ > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    };
-    if (warp == W_K || warp == W_V) {
-        fewer();
-        // copies: Q once (K's warp), then a tile a step, a box of
-        // min(page, 64) keys by 64 columns a lane
-        const bool is_v = warp == W_V;
+    // Steps t = 0 .. n + 1: a stage brings K of tile t and V of tile t - 2, and
+    // the MMA warp then does P V of tile t - 2 and Q K^T of tile t for each
+    // query tile: two tiles of scores are ahead of the softmax warps.
+    if (warp == W_COPY) {
+        // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
+        // the lower half of the warp, V's by the upper
+        const int box = min(A.page_size, KEYS), boxes = BN / box, which = lane % 16;
+        const int is_v = lane / 16, kb = which % boxes, col = which / boxes * 64;
         const CUtensorMap *map = is_v ? &tv : &tk;
-        uint8_t *sm = is_v ? v_sm : k_sm;
-        uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
-        const int ST = is_v ? VST : KST;
-        const int box = min(A.page_size, KEYS), boxes = BN / box;
-        const int kb = lane % boxes, col = lane / boxes * 64;
-        const bool mine = col < DP;
-        if (!is_v && n > 0 && lane == 0) {
+        if (n > 0 && lane == 0) {
             mbar_arrive_expect_tx(&q_full, nq * (DP / 64) * per_tile * A.group * 128);
             for (int q = 0; q < nq; q++)
                 for (int c = 0; c < DP / 64; c++)
@@ -682,9 +671,13 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                                 s.q0 + t0 + q * per_tile);
         }
         __syncwarp();
-        auto page_of = [&](int i) {
-            const int64_t key = from + (int64_t) i * BN + kb * box;
-            if (!mine || i >= n || key >= to) return (int) A.pages;  // outside the tensor: zeros
+        auto mine = [&](int t) {
+            const int i = t - 2 * is_v;
+            return col < DP && i >= 0 && i < n;
+        };
+        auto page_of = [&](int t) {
+            const int key = from + (t - 2 * is_v) * BN + kb * box;
+            if (!mine(t) || key >= to) return (int) A.pages;  // outside the tensor: zeros
             const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
             if (p < 0 || p >= A.pages) {
                 atomicOr(A.err, ZEST_ERR_BAD_PAGE);
@@ -692,114 +685,82 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             }
             return p;
         };
-        int page = page_of(0), i = 0;
-        for (; i < n; i++) {
-            const int st = i % ST;
-            const int next = page_of(i + 1);
-            const bool ok = i < ST || wait_soon(&empty[st], (i / ST - 1) & 1, gone);
+        const int steps = n > 0 ? n + 2 : 0;
+        int page = page_of(0), t = 0;
+        for (; t < steps; t++) {
+            const int st = t % ST;
+            const int next = page_of(t + 1);
+            const bool ok = t < ST || wait_soon(&empty[st], (t / ST - 1) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 break;
             }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], ((t < n) + (t >= 2)) * C::KV_BYTES);
             __syncwarp();
-            if (mine) {
-                const int64_t key = from + (int64_t) i * BN + kb * box;
-                tma_load_4d(sm + st * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, &full[st], col,
-                            (int) (key % A.page_size), kv_head, page);
+            if (mine(t)) {
+                const int key = from + (t - 2 * is_v) * BN + kb * box;
+                tma_load_4d(ring + (2 * st + is_v) * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map,
+                            &full[st], col, key % A.page_size, kv_head, page);
             }
             page = next;
         }
         // the last copies land before the block ends, whatever the others do
-        for (int k = max(0, i - ST); k < i; k++)
+        for (int k = max(0, t - ST); k < t; k++)
             mbar_wait_bounded(&full[k % ST], (k / ST) & 1, nullptr, WAIT_LIMIT_NS);
-        if (!is_v && n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
+        if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_MMA) {
-        fewer();
-        // the whole warp walks the loop, so that addresses and descriptors are
-        // uniform; one elected thread issues
-        if (n > 0) {
+        // one elected thread; its loops stay rolled (wait_on says why). A
+        // descriptor's address counts 16 bytes in its low word, and no tile
+        // passes its 18 bits
+        if (n > 0 && elect_one()) {
             constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
             constexpr uint32_t QK = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
             constexpr uint32_t PV = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
-            const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm), v_desc = sw128_desc_mn(v_sm, BN * 128);
-            auto wait = [&](uint64_t *bar, int phase) {
-                if (__all_sync(0xffffffffu, wait_soon(bar, phase & 1, gone))) {
-                    tc_fence_after();
-                    return true;
+            const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(ring);
+            const uint64_t v_desc = sw128_desc_mn(ring + C::KV_BYTES, BN * 128);
+            auto wait = [&](uint64_t *bar, uint32_t phase) {
+                if (!wait_soon(bar, phase & 1, gone)) {
+                    give_up();
+                    return false;
                 }
-                if (lane == 0) give_up();
-                return false;
-            };
-            auto commit = [&](uint64_t *bar) {
-                if (elect_one()) tc_commit(bar);
-            };
-            auto s_col = [&](int q, int b) { return tmem + C::S_COL + (q * NS + b) * BN; };
-            // a descriptor's address counts 16 bytes, and no tile passes its 18 bits
-            auto scores = [&](int q, int i) {
-                const uint64_t kt = k_desc + i % KST * (C::KV_BYTES >> 4), qt = q_desc + q * (C::Q_BYTES >> 4);
-                const int b = NS > 1 ? i % NS : 0;
-                const uint32_t d = s_col(q, b);
-                if (elect_one()) {
-#pragma unroll
-                    for (int ks = 0; ks < DP / 16; ks++)
-                        tc_mma_bf16(d, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
-                                    kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
-                    tc_commit(&s_full[q * NS + b]);
-                }
-            };
-            auto values = [&](int q, int i) {
-                const int b = q * NS + (NS > 1 ? i % NS : 0);
-                const uint64_t vt = v_desc + i % VST * (C::KV_BYTES >> 4);
-                const uint32_t a = s_col(q, NS > 1 ? i % NS : 0);
-#pragma unroll
-                for (int h = 0; h < H; h++) {
-                    if (!wait(&p_full[b * H + h], i / NS)) return false;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int ks = 4 * h; ks < 4 * h + 4; ks++)
-                            tc_mma_f16_ts(tmem + C::O_COL + q * DP, a + ks * 8, vt + (ks * 16 * 128 >> 4), PV,
-                                          i > 0 || ks > 0);
-                    }
-                }
+                tc_fence_after();
                 return true;
             };
-            bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
-            if (ok) {
-                for (int q = 0; q < nq; q++) scores(q, 0);
-                commit(&k_empty[0]);
-            }
-            for (int i = 0; ok && i < n; i++) {
-                const bool more = i + 1 < n;
-                if (NS > 1 && more) {  // the other buffer: its weights went into the product before
-                    if (!(ok = wait(&k_full[(i + 1) % KST], (i + 1) / KST))) break;
-                    scores(0, i + 1);
-                    commit(&k_empty[(i + 1) % KST]);
-                }
-                if (!(ok = wait(&v_full[i % VST], i / VST))) break;
-                for (int q = 0; ok && q < nq; q++) {
-                    if (!(ok = values(q, i))) break;
-                    if (q == nq - 1) commit(&v_empty[i % VST]);
-                    if (NS > 1 || i == n - 1) {
-                        if (q == nq - 1) commit(&pv_done);
+            bool ok = wait(&q_full, 0);
+#pragma unroll 1
+            for (int t = 0; ok && t < n + 2; t++) {
+                const int st = t % ST;
+                if (!(ok = wait(&full[st], t / ST))) break;
+#pragma unroll 1
+                for (int q = 0; q < nq; q++) {
+                    const uint32_t s_at = tmem + C::S_COL + (q * 2 + (t & 1)) * BN;
+                    if (t >= 2) {
+                        const uint64_t vt = v_desc + st * (2 * C::KV_BYTES >> 4);
+                        if (!(ok = wait(&p_full[q][t & 1], t / 2 - 1))) break;
+#pragma unroll
+                        for (int ks = 0; ks < BN / 16; ks++)
+                            tc_mma_f16_ts(tmem + C::O_COL + q * DP, s_at + ks * 8, vt + (ks * 16 * 128 >> 4), PV,
+                                          t > 2 || ks > 0);
+                        tc_commit(&pv_done[q]);
                     }
-                    if (NS == 1 && more) {
-                        if (q == 0 && !(ok = wait(&k_full[(i + 1) % KST], (i + 1) / KST))) break;
-                        scores(q, i + 1);
-                        if (q == nq - 1) commit(&k_empty[(i + 1) % KST]);
+                    if (t < n) {  // into the buffer whose weights just went into the product
+                        const uint64_t kt = k_desc + st * (2 * C::KV_BYTES >> 4), qt = q_desc + q * (C::Q_BYTES >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < DP / 16; ks++)
+                            tc_mma_bf16(s_at, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
+                                        kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
+                        tc_commit(&s_full[q][t & 1]);
                     }
                 }
+                if (ok) tc_commit(&empty[st]);
             }
             if (!ok) {  // what was issued still ends before TMEM goes
-                commit(&drained);
+                tc_commit(&drained);
                 mbar_wait_bounded(&drained, 0, nullptr, WAIT_LIMIT_NS);
             }
         }
         __syncwarp();
-    } else if (warp > W_MMA) {
-        fewer();
-    } else {
-        if (NQ > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    } else if (warp / 4 < nq) {
         const int q = warp / 4, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t) (warp % 4 * 32) << 16;
         const uint32_t o_at = tmem + lanes + C::O_COL + q * DP;
@@ -809,45 +770,43 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const int lo = valid ? row_lo(A, s, t) : 0, hi = valid ? row_hi(A, s, t) : 0;
         const key_span mine = span_of(A, s, tq0, tq1 - 1);
         float m = -INFINITY, l = 0.0f;
-        bool ok = q < nq;
-        for (int i = 0; i < n && q < nq; i++) {
-            const int b = NS > 1 ? i % NS : 0;
-            ok = wait_soon(&s_full[q * NS + b], (i / NS) & 1, gone);
+        bool ok = true;
+        for (int i = 0; i < n; i++) {
+            ok = wait_soon(&s_full[q][i & 1], (i / 2) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t s_at = tmem + lanes + C::S_COL + (q * NS + b) * BN;
+            const uint32_t s_at = tmem + lanes + C::S_COL + (q * 2 + (i & 1)) * BN;
             uint32_t x[BN / 32][32];
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(s_at + c * 32, x[c]);
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
-            const int64_t key0 = from + (int64_t) i * BN;
-            if (key0 < mine.clo || key0 + BN > min((int64_t) mine.chi, to)) {
-                const int a = (int) (max((int64_t) lo, key0) - key0), z = (int) (min((int64_t) hi, to) - key0);
+            const int key0 = from + i * BN;
+            if (key0 < mine.clo || key0 + BN > min(mine.chi, to)) {
+                const int a = lo - key0, z = min(hi, to) - key0;
 #pragma unroll
                 for (int c = 0; c < BN / 32; c++)
 #pragma unroll
                     for (int e = 0; e < 32; e++)
                         if (c * 32 + e < a || c * 32 + e >= z) x[c][e] = 0xff800000u;
             }
-            if (key0 < sp.clo || key0 + BN > min((int64_t) sp.chi, to)) {
+            if (key0 < sp.clo || key0 + BN > min(sp.chi, to)) {
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
-                if (!__all_sync(0xffffffffu,
-                                wait_soon(&v_full[i % VST], (i / VST) & 1, gone))) {
+                if (!__all_sync(0xffffffffu, wait_soon(&full[(i + 2) % ST], ((i + 2) / ST) & 1, gone))) {
                     if (lane == 0) give_up();
                     ok = false;
                     break;
                 }
                 bool found = false;
-                uint8_t *vt = v_sm + i % VST * C::KV_BYTES;
+                uint8_t *vt = ring + ((i + 2) % ST * 2 + 1) * C::KV_BYTES;
                 for (int e = row; e < C::KV_BYTES / 16; e += 128) {
-                    const int64_t key = key0 + e / 8 % BN;
-                    if (key >= sp.clo && key < min((int64_t) sp.chi, to)) continue;
+                    const int key = key0 + e / 8 % BN;
+                    if (key >= sp.clo && key < min(sp.chi, to)) continue;
                     uint4 w = *reinterpret_cast<uint4 *>(vt + e * 16);
                     uint32_t h[4] = { w.x, w.y, w.z, w.w };
                     bool bad = false;
@@ -879,17 +838,14 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             if (i == 0) {
                 m = mx;
             } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
-                // o relative to the new maxima; every product before is done
-                // (one score buffer: this tile's scores were issued after it)
-                if (NS > 1) {
-                    ok = wait_soon(&pv_done, (i - 1) & 1, gone);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        if (lane == 0) give_up();
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
+                // o relative to the new maxima, once the product before is in it
+                ok = wait_soon(&pv_done[q], (i - 1) & 1, gone);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    if (lane == 0) give_up();
+                    ok = false;
+                    break;
                 }
+                tc_fence_after();
                 const float f = mx == m ? 1.0f : exp2_fast(m - mx);
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; c++) {
@@ -905,23 +861,20 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             }
             const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
             float sum[4] = {};
-#pragma unroll
-            for (int h = 0; h < H; h++) {
-                uint32_t p[32];
-                weights<F16>(&x[0][0] + 64 * h, A.scale_log2, base, p, sum);
-                tmem_st_32x32b_x32(s_at + h * 32, p);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[(q * NS + b) * H + h]);
-            }
+            uint32_t p[32];
+            weights<F16>(&x[0][0], A.scale_log2, base, p, sum);
+            tmem_st_32x32b_x32(s_at, p);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[q][i & 1]);
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         // the last product
         if (ok && n > 0) {
             // by phases: the one before it may not have ended either
-            if (NS > 1 && n > 1) wait_soon(&pv_done, (n - 2) & 1, gone);
-            ok = wait_soon(&pv_done, NS > 1 ? (n - 1) & 1 : 0, gone);
+            if (n > 1) wait_soon(&pv_done[q], (n - 2) & 1, gone);
+            ok = wait_soon(&pv_done[q], (n - 1) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 ok = false;
@@ -932,7 +885,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             const int head = kv_head * A.group + row % A.group;
             const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
             const float inv = A.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const int fa = (int) max((int64_t) lo, from), fz = (int) min((int64_t) hi, to);
+            const int fa = max(lo, from), fz = min(hi, to);
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
                 uint32_t o[32];
