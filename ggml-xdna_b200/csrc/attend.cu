@@ -523,26 +523,55 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 // --- many rows: tcgen05 -------------------------------------------------------------
 
 // Shapes by padded head size. A block's query tiles of 128 rows share each tile
-// of 64 keys and values. Each has two score buffers in TMEM: the next tile's
-// scores are there before this tile's weights are done, so the softmax warps
-// never wait for a product and the tensor cores work beside them.
+// of keys and values, and one score buffer in TMEM in turn: it is free again as
+// soon as a tile's rows are in registers, so the other tile's scores are made
+// while these take their exponentials, and the tensor cores and the
+// exponential units both work throughout. (A buffer of each tile's own, with P
+// over it as the first form had it, holds the next scores back until P has
+// been used: 229 us where this takes XXX for 2,048 tokens over 8,192.)
 template <int DP>
 struct many_rows {
-    static constexpr int NQ = DP == 256 ? 1 : 2;  // query tiles of a block
-    static constexpr int BN = 64;                 // keys of a tile
+    static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
+    static constexpr int BN = DP == 256 ? 64 : 128; // keys of a tile
+    static constexpr int PART = 64;                 // keys whose weights are handed over at once
+    static constexpr int PARTS = BN / PART;
     static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int ST = DP == 256 ? 2 : 4;  // stages, of a tile of K and one of V
+    static constexpr int ST = DP == 64 ? 4 : 2;     // stages, of a tile of K and one of V
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + ST * 2 * KV_BYTES;
-    static constexpr int SOFTMAX = NQ * 128;      // threads: one a row
-    static constexpr int THREADS = SOFTMAX + 64;  // and a warp each for the MMAs and the copies
-    // TMEM columns: O of each query tile, then its two score buffers (P lies over them)
-    static constexpr int O_COL = 0, S_COL = NQ * DP, COLS = 512;
+    static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
+    static constexpr int THREADS = SOFTMAX + 64;    // and a warp each for the MMAs and the copies
+    // TMEM columns: O of each query tile, the scores, P of each query tile
+    static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
+    static_assert(P_COL + NQ * BN / 2 <= COLS, "TMEM holds O, S and P");
 };
 
 // A rise of the running maximum below this (in powers of two) leaves the
 // weights relative to the old one: they stay within 2^8, and o is not touched.
 constexpr float LAZY = 8.0f;
+
+// Two f32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -567,19 +596,19 @@ __device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volati
     return mbar_try_wait(bar, parity) || wait_on(bar, parity, gone);
 }
 
-// The weights of 64 keys: x in (bits of scores), 2^(x scale + base) rounded to
-// the cache's type and packed out, their f32 sums into s. Plain f32 operations:
-// 278 clocks for 64 keys of two warps of a scheduler, where paired f32x2 ones
-// around the exponentials took 624, and a quarter of the exponentials by a
-// polynomial 309.
+// The weights of 32 keys: x in as bits of scores, out as bits of 2^(x scale +
+// base), which p gets rounded to the cache's type.
 template <bool F16>
-__device__ __forceinline__ void weights(const uint32_t *x, float scale, float base, uint32_t (&p)[32], float (&s)[4]) {
+__device__ __forceinline__ void weights(uint32_t (&x)[32], float scale, float base, uint32_t *p) {
+    const uint64_t m = pack2(scale, scale), c = pack2(base, base);
 #pragma unroll
-    for (int e = 0; e < 32; e++) {
-        const float u = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e]), scale, base));
-        const float w = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * e + 1]), scale, base));
-        s[e & 1] += u;
-        s[2 + (e & 1)] += w;
+    for (int e = 0; e < 16; e++) {
+        float u, w;
+        unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m, c), u, w);
+        u = exp2_fast(u);
+        w = exp2_fast(w);
+        x[2 * e] = __float_as_uint(u);
+        x[2 * e + 1] = __float_as_uint(w);
         p[e] = kv_bits2<F16>(u, w);
     }
 }
@@ -595,11 +624,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, BN = C::BN, ST = C::ST;
+    constexpr int NQ = C::NQ, BN = C::BN, ST = C::ST, PARTS = C::PARTS;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
     uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // a stage: a tile of K, then one of V
-    __shared__ uint64_t q_full, full[ST], empty[ST], s_full[NQ][2], p_full[NQ][2], pv_done[NQ], drained;
+    __shared__ uint64_t q_full, full[ST], empty[ST], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ], drained;
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -629,12 +658,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < NQ; i++) {
-            for (int b = 0; b < 2; b++) {
-                mbar_init(&s_full[i][b], 1);
-                mbar_init(&p_full[i][b], 4);
-            }
+            mbar_init(&s_full[i], 1);
+            for (int h = 0; h < PARTS; h++) mbar_init(&p_full[i][h], 4);
             mbar_init(&pv_done[i], 1);
         }
+        mbar_init(&s_free, 4);
         mbar_init(&drained, 1);
         stop = 0;
         not_finite = 0;
@@ -654,9 +682,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         atomicOr(A.err, ERR_TIMEOUT);
     };
 
-    // Steps t = 0 .. n + 1: a stage brings K of tile t and V of tile t - 2, and
-    // the MMA warp then does P V of tile t - 2 and Q K^T of tile t for each
-    // query tile: two tiles of scores are ahead of the softmax warps.
+    // Steps t = 0 .. n: a stage brings K of tile t and V of tile t - 1, and the MMA
+    // warp does, for each query tile, Q K^T of tile t and P V of tile t - 1.
     if (warp == W_COPY) {
         // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
         // the lower half of the warp, V's by the upper
@@ -672,11 +699,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         }
         __syncwarp();
         auto mine = [&](int t) {
-            const int i = t - 2 * is_v;
+            const int i = t - is_v;
             return col < DP && i >= 0 && i < n;
         };
         auto page_of = [&](int t) {
-            const int key = from + (t - 2 * is_v) * BN + kb * box;
+            const int key = from + (t - is_v) * BN + kb * box;
             if (!mine(t) || key >= to) return (int) A.pages;  // outside the tensor: zeros
             const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
             if (p < 0 || p >= A.pages) {
@@ -685,7 +712,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             }
             return p;
         };
-        const int steps = n > 0 ? n + 2 : 0;
+        const int steps = n > 0 ? n + 1 : 0;
         int page = page_of(0), t = 0;
         for (; t < steps; t++) {
             const int st = t % ST;
@@ -695,10 +722,10 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 if (lane == 0) give_up();
                 break;
             }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], ((t < n) + (t >= 2)) * C::KV_BYTES);
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], ((t < n) + (t > 0)) * C::KV_BYTES);
             __syncwarp();
             if (mine(t)) {
-                const int key = from + (t - 2 * is_v) * BN + kb * box;
+                const int key = from + (t - is_v) * BN + kb * box;
                 tma_load_4d(ring + (2 * st + is_v) * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map,
                             &full[st], col, key % A.page_size, kv_head, page);
             }
@@ -709,53 +736,62 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_wait_bounded(&full[k % ST], (k / ST) & 1, nullptr, WAIT_LIMIT_NS);
         if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_MMA) {
-        // one elected thread; its loops stay rolled (wait_on says why). A
-        // descriptor's address counts 16 bytes in its low word, and no tile
-        // passes its 18 bits
-        if (n > 0 && elect_one()) {
+        // the whole warp walks the loop, so that addresses and descriptors are
+        // uniform (an MMA issues in a few clocks, not in 80); one elected thread
+        // issues. A descriptor's address counts 16 bytes in its low word, and no
+        // tile passes its 18 bits
+        if (n > 0) {
             constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
             constexpr uint32_t QK = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
             constexpr uint32_t PV = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
             const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(ring);
             const uint64_t v_desc = sw128_desc_mn(ring + C::KV_BYTES, BN * 128);
             auto wait = [&](uint64_t *bar, uint32_t phase) {
-                if (!wait_soon(bar, phase & 1, gone)) {
-                    give_up();
+                if (!__all_sync(0xffffffffu, wait_soon(bar, phase & 1, gone))) {
+                    if (lane == 0) give_up();
                     return false;
                 }
                 tc_fence_after();
                 return true;
             };
             bool ok = wait(&q_full, 0);
-#pragma unroll 1
-            for (int t = 0; ok && t < n + 2; t++) {
+            uint32_t used = 0;  // score tiles so far: the next waits until the last is in registers
+            for (int t = 0; ok && t <= n; t++) {
                 const int st = t % ST;
                 if (!(ok = wait(&full[st], t / ST))) break;
-#pragma unroll 1
-                for (int q = 0; q < nq; q++) {
-                    const uint32_t s_at = tmem + C::S_COL + (q * 2 + (t & 1)) * BN;
-                    if (t >= 2) {
-                        const uint64_t vt = v_desc + st * (2 * C::KV_BYTES >> 4);
-                        if (!(ok = wait(&p_full[q][t & 1], t / 2 - 1))) break;
+                const uint64_t kt = k_desc + st * (2 * C::KV_BYTES >> 4), vt = v_desc + st * (2 * C::KV_BYTES >> 4);
+                for (int q = 0; ok && q < nq; q++) {
+                    if (t < n) {
+                        if (used > 0 && !(ok = wait(&s_free, used - 1))) break;
+                        used++;
+                        const uint64_t qt = q_desc + q * (C::Q_BYTES >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < BN / 16; ks++)
-                            tc_mma_f16_ts(tmem + C::O_COL + q * DP, s_at + ks * 8, vt + (ks * 16 * 128 >> 4), PV,
-                                          t > 2 || ks > 0);
-                        tc_commit(&pv_done[q]);
+                            for (int ks = 0; ks < DP / 16; ks++)
+                                tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
+                                            kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
+                            tc_commit(&s_full[q]);
+                        }
                     }
-                    if (t < n) {  // into the buffer whose weights just went into the product
-                        const uint64_t kt = k_desc + st * (2 * C::KV_BYTES >> 4), qt = q_desc + q * (C::Q_BYTES >> 4);
+                    if (t > 0) {
+                        const uint32_t p_at = tmem + C::P_COL + q * (BN / 2);
 #pragma unroll
-                        for (int ks = 0; ks < DP / 16; ks++)
-                            tc_mma_bf16(s_at, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
-                                        kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
-                        tc_commit(&s_full[q][t & 1]);
+                        for (int h = 0; h < PARTS; h++) {
+                            if (!(ok = wait(&p_full[q][h], t - 1))) break;
+                            if (elect_one()) {
+#pragma unroll
+                                for (int ks = h * (C::PART / 16); ks < (h + 1) * (C::PART / 16); ks++)
+                                    tc_mma_f16_ts(tmem + C::O_COL + q * DP, p_at + ks * 8, vt + (ks * 16 * 128 >> 4),
+                                                  PV, t > 1 || ks > 0);
+                                if (h == PARTS - 1) tc_commit(&pv_done[q]);
+                            }
+                        }
                     }
                 }
-                if (ok) tc_commit(&empty[st]);
+                if (ok && elect_one()) tc_commit(&empty[st]);
             }
             if (!ok) {  // what was issued still ends before TMEM goes
-                tc_commit(&drained);
+                if (elect_one()) tc_commit(&drained);
                 mbar_wait_bounded(&drained, 0, nullptr, WAIT_LIMIT_NS);
             }
         }
@@ -772,19 +808,21 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int i = 0; i < n; i++) {
-            ok = wait_soon(&s_full[q][i & 1], (i / 2) & 1, gone);
+            ok = wait_soon(&s_full[q], i & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t s_at = tmem + lanes + C::S_COL + (q * 2 + (i & 1)) * BN;
             uint32_t x[BN / 32][32];
 #pragma unroll
-            for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(s_at + c * 32, x[c]);
+            for (int c = 0; c < BN / 32; c++) tmem_ld_32x32b_x32(tmem + lanes + C::S_COL + c * 32, x[c]);
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free);
             const int key0 = from + i * BN;
             if (key0 < mine.clo || key0 + BN > min(mine.chi, to)) {
                 const int a = lo - key0, z = min(hi, to) - key0;
@@ -797,13 +835,13 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             if (key0 < sp.clo || key0 + BN > min(sp.chi, to)) {
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
-                if (!__all_sync(0xffffffffu, wait_soon(&full[(i + 2) % ST], ((i + 2) / ST) & 1, gone))) {
+                if (!__all_sync(0xffffffffu, wait_soon(&full[(i + 1) % ST], ((i + 1) / ST) & 1, gone))) {
                     if (lane == 0) give_up();
                     ok = false;
                     break;
                 }
                 bool found = false;
-                uint8_t *vt = ring + ((i + 2) % ST * 2 + 1) * C::KV_BYTES;
+                uint8_t *vt = ring + ((i + 1) % ST * 2 + 1) * C::KV_BYTES;
                 for (int e = row; e < C::KV_BYTES / 16; e += 128) {
                     const int key = key0 + e / 8 % BN;
                     if (key >= sp.clo && key < min(sp.chi, to)) continue;
@@ -835,10 +873,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             // a NaN or an infinite score: the row's weights are NaN, as the formula's
             const bool odd = !(mx < INFINITY);
             mx = odd ? m : fmaxf(m, mx);
-            if (i == 0) {
-                m = mx;
-            } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
-                // o relative to the new maxima, once the product before is in it
+            if (i > 0) {  // the product before is done: its P may go, and o may be touched
                 ok = wait_soon(&pv_done[q], (i - 1) & 1, gone);
                 if (!__all_sync(0xffffffffu, ok)) {
                     if (lane == 0) give_up();
@@ -846,6 +881,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     break;
                 }
                 tc_fence_after();
+            }
+            if (i == 0) {
+                m = mx;
+            } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
+                // o relative to the new maxima
                 const float f = mx == m ? 1.0f : exp2_fast(m - mx);
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; c++) {
@@ -860,20 +900,30 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 m = mx;
             }
             const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
-            float sum[4] = {};
-            uint32_t p[32];
-            weights<F16>(&x[0][0], A.scale_log2, base, p, sum);
-            tmem_st_32x32b_x32(s_at, p);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[q][i & 1]);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int h = 0; h < PARTS; h++) {
+                uint32_t p[32];
+                weights<F16>(x[2 * h], A.scale_log2, base, p);
+                weights<F16>(x[2 * h + 1], A.scale_log2, base, p + 16);
+                tmem_st_32x32b_x32(tmem + lanes + C::P_COL + q * (BN / 2) + h * 32, p);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[q][h]);
+            }
+            // the sums while the tensor cores work
+            uint64_t sum[4] = {};
+#pragma unroll
+            for (int c = 0; c < BN / 32; c++)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+                    sum[e / 2 % 4] = add2(sum[e / 2 % 4], pack2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])));
+            float sa, sb;
+            unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sa, sb);
+            l += sa + sb;
         }
         // the last product
         if (ok && n > 0) {
-            // by phases: the one before it may not have ended either
-            if (n > 1) wait_soon(&pv_done[q], (n - 2) & 1, gone);
             ok = wait_soon(&pv_done[q], (n - 1) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
