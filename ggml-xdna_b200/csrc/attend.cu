@@ -537,10 +537,10 @@ struct many_rows {
     static constexpr int PARTS = BN / PART;
     static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int ST = DP == 64 ? 4 : 2;     // stages, of a tile of K and one of V
-    static constexpr int SMEM = 1024 + NQ * Q_BYTES + ST * 2 * KV_BYTES;
+    static constexpr int SLOTS = DP == 64 ? 8 : 5;  // tiles of K or V in flight or in use
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
-    static constexpr int THREADS = SOFTMAX + 64;    // and a warp each for the MMAs and the copies
+    static constexpr int THREADS = SOFTMAX + 96;    // and a warp each for Q K^T, P V and the copies
     // TMEM columns: O of each query tile, the scores, P of each query tile
     static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
     static_assert(P_COL + NQ * BN / 2 <= COLS, "TMEM holds O, S and P");
@@ -580,35 +580,70 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return r;
 }
 
-// The rest of a wait whose first look found nothing, for at most WAIT_LIMIT_NS
-// or until *gone. Out of line: the warps of a block share the instruction
-// caches, and a warp that issues MMAs between others' long straight code pays
-// for every line of its own.
-__device__ __noinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile int *gone) {
+// A warp's wait: one look, and the rest, for at most WAIT_LIMIT_NS or until
+// *gone, out of line. The same answer in every lane; a wait that runs out sets
+// *gone and the error bit.
+__device__ __noinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile int *gone, unsigned *err) {
     const uint64_t t0 = global_ns();
-    for (uint32_t it = 1;; it++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 0 && ((gone && *gone) || global_ns() - t0 > WAIT_LIMIT_NS)) return false;
+    bool ok = false;
+    for (uint32_t it = 1; !ok; it++) {
+        ok = mbar_try_wait(bar, parity);
+        if (!ok && (it & 63u) == 0 && (*gone || global_ns() - t0 > WAIT_LIMIT_NS)) break;
     }
+    if (__all_sync(0xffffffffu, ok)) return true;
+    *gone = 1;
+    atomicOr(err, ERR_TIMEOUT);
+    return false;
 }
 
-__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile int *gone) {
-    return mbar_try_wait(bar, parity) || wait_on(bar, parity, gone);
+__device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile int *gone, unsigned *err) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_on(bar, parity, gone, err);
 }
 
-// The weights of 32 keys: x in as bits of scores, out as bits of 2^(x scale +
-// base), which p gets rounded to the cache's type.
+// 2^u and 2^w without the exponential unit: x = n + f, n the nearest integer
+// (adding 1.5 * 2^23 leaves it in the low mantissa bits), 2^f by a polynomial
+// of degree 4 on [-1/2, 1/2] whose relative error, fitted to be even
+// (iteratively reweighted least squares), is 2^-18.5; n added to the exponent.
+// Zero below 2^-126; u, w < 127 and not NaN.
+__device__ __forceinline__ void exp2_poly(float &u, float &w) {
+    const float R = 12582912.0f;  // 1.5 * 2^23
+    const uint64_t x = pack2(fmaxf(u, -126.0f), fmaxf(w, -126.0f));
+    const uint64_t t = add2(x, pack2(R, R)), n = add2(t, pack2(-R, -R));
+    const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), x);
+    uint64_t p = pack2(9.5701022e-3f, 9.5701022e-3f);
+    p = fma2(p, f, pack2(5.5917859e-2f, 5.5917859e-2f));
+    p = fma2(p, f, pack2(2.4024744e-1f, 2.4024744e-1f));
+    p = fma2(p, f, pack2(6.9312179e-1f, 6.9312179e-1f));
+    p = fma2(p, f, pack2(9.9999928e-1f, 9.9999928e-1f));
+    float tu, tw, pu, pw;
+    unpack2(t, tu, tw);
+    unpack2(p, pu, pw);
+    u = u < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(pu) + (__float_as_uint(tu) << 23));
+    w = w < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(pw) + (__float_as_uint(tw) << 23));
+}
+
+// The weights of 64 keys: x in as bits of scores, 2^(x scale + base) rounded to
+// the cache's type into p, their f32 sums into s0 and s1. One pair of eight by
+// polynomial: the exponential unit (16 a clock and SM) is what the rows wait
+// for. Clocks for 128 keys of a warp alone and of two warps a scheduler, with
+// the maximum before: 1,676 and 2,334 with none, 1,536 and 2,146 with one of
+// eight, 1,451 and 2,258 with one of four.
 template <bool F16>
-__device__ __forceinline__ void weights(uint32_t (&x)[32], float scale, float base, uint32_t *p) {
+__device__ __forceinline__ void weights(const uint32_t *x, float scale, float base, uint32_t (&p)[32], uint64_t &s0,
+                                        uint64_t &s1) {
     const uint64_t m = pack2(scale, scale), c = pack2(base, base);
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
+    for (int e = 0; e < 32; e++) {
         float u, w;
         unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m, c), u, w);
-        u = exp2_fast(u);
-        w = exp2_fast(w);
-        x[2 * e] = __float_as_uint(u);
-        x[2 * e + 1] = __float_as_uint(w);
+        if (e % 8 == 7) {
+            exp2_poly(u, w);
+        } else {
+            u = exp2_fast(u);
+            w = exp2_fast(w);
+        }
+        if (e & 1) s1 = add2(s1, pack2(u, w));
+        else s0 = add2(s0, pack2(u, w));
         p[e] = kv_bits2<F16>(u, w);
     }
 }
@@ -624,11 +659,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, BN = C::BN, ST = C::ST, PARTS = C::PARTS;
+    constexpr int NQ = C::NQ, BN = C::BN, SLOTS = C::SLOTS, PARTS = C::PARTS;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
-    uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // a stage: a tile of K, then one of V
-    __shared__ uint64_t q_full, full[ST], empty[ST], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ], drained;
+    uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // of tiles of K and V
+    __shared__ uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ], drained[2];
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -650,10 +685,10 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     const int to = (int) min((int64_t) sp.hi, from + A.chunk), n = max(0, (to - from + BN - 1) / BN);
     if (n == 0 && split > 0) return;
 
-    constexpr int W_MMA = C::SOFTMAX / 32, W_COPY = W_MMA + 1;
+    constexpr int W_QK = C::SOFTMAX / 32, W_PV = W_QK + 1, W_COPY = W_QK + 2;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        for (int i = 0; i < ST; i++) {
+        for (int i = 0; i < SLOTS; i++) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
@@ -663,12 +698,13 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_init(&pv_done[i], 1);
         }
         mbar_init(&s_free, 4);
-        mbar_init(&drained, 1);
+        mbar_init(&drained[0], 1);
+        mbar_init(&drained[1], 1);
         stop = 0;
         not_finite = 0;
         fence_barrier_init();
     }
-    if (warp == W_MMA) {
+    if (warp == W_QK) {
         tmem_alloc(&tmem_sh, C::COLS);
         tmem_relinquish();
     }
@@ -677,13 +713,10 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
     volatile int *const gone = &stop;
-    auto give_up = [&] {
-        stop = 1;
-        atomicOr(A.err, ERR_TIMEOUT);
-    };
 
-    // Steps t = 0 .. n: a stage brings K of tile t and V of tile t - 1, and the MMA
-    // warp does, for each query tile, Q K^T of tile t and P V of tile t - 1.
+    // The tiles' order in the ring: K(0) K(1) V(0) K(2) V(1) ... K(n - 1) V(n - 2) V(n - 1).
+    auto slot_of_k = [](int i) { return (uint32_t) max(0, 2 * i - 1); };
+    auto slot_of_v = [](int i, int n) { return (uint32_t) (i + 1 < n ? 2 * i + 2 : 2 * i + 1); };
     if (warp == W_COPY) {
         // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
         // the lower half of the warp, V's by the upper
@@ -698,13 +731,10 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                                 s.q0 + t0 + q * per_tile);
         }
         __syncwarp();
-        auto mine = [&](int t) {
-            const int i = t - is_v;
-            return col < DP && i >= 0 && i < n;
-        };
-        auto page_of = [&](int t) {
-            const int key = from + (t - is_v) * BN + kb * box;
-            if (!mine(t) || key >= to) return (int) A.pages;  // outside the tensor: zeros
+        const bool has = col < DP;
+        auto page_of = [&](int i) {  // of this lane's box of tile i (K or V)
+            const int key = from + i * BN + kb * box;
+            if (!has || i < 0 || i >= n || key >= to) return (int) A.pages;  // outside the tensor: zeros
             const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
             if (p < 0 || p >= A.pages) {
                 atomicOr(A.err, ZEST_ERR_BAD_PAGE);
@@ -712,88 +742,96 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             }
             return p;
         };
-        const int steps = n > 0 ? n + 1 : 0;
-        int page = page_of(0), t = 0;
-        for (; t < steps; t++) {
-            const int st = t % ST;
-            const int next = page_of(t + 1);
-            const bool ok = t < ST || wait_soon(&empty[st], (t / ST - 1) & 1, gone);
-            if (!__all_sync(0xffffffffu, ok)) {
-                if (lane == 0) give_up();
-                break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], ((t < n) + (t > 0)) * C::KV_BYTES);
-            __syncwarp();
-            if (mine(t)) {
-                const int key = from + (t - is_v) * BN + kb * box;
-                tma_load_4d(ring + (2 * st + is_v) * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map,
-                            &full[st], col, key % A.page_size, kv_head, page);
+        int slot = 0, turn = 0, brought = 0, page = page_of(-is_v);
+        bool ok = true;
+        for (int t = 0; ok && t <= n && n > 0; t++) {
+            const int next = page_of(t + 1 - is_v);
+            for (int v = 0; v < 2; v++) {
+                if (v ? t == 0 : t == n) continue;
+                if (turn > 0 && !(ok = wait_soon(&empty[slot], (turn - 1) & 1, gone, A.err))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::KV_BYTES);
+                __syncwarp();
+                if (has && v == is_v) {
+                    const int key = from + (t - v) * BN + kb * box;
+                    tma_load_4d(ring + slot * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, &full[slot],
+                                col, key % A.page_size, kv_head, page);
+                }
+                brought++;
+                if (++slot == SLOTS) slot = 0, turn++;
             }
             page = next;
         }
         // the last copies land before the block ends, whatever the others do
-        for (int k = max(0, t - ST); k < t; k++)
-            mbar_wait_bounded(&full[k % ST], (k / ST) & 1, nullptr, WAIT_LIMIT_NS);
+        for (int k = max(0, brought - SLOTS); k < brought; k++)
+            mbar_wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, nullptr, WAIT_LIMIT_NS);
         if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
-    } else if (warp == W_MMA) {
-        // the whole warp walks the loop, so that addresses and descriptors are
-        // uniform (an MMA issues in a few clocks, not in 80); one elected thread
-        // issues. A descriptor's address counts 16 bytes in its low word, and no
-        // tile passes its 18 bits
-        if (n > 0) {
-            constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
-            constexpr uint32_t QK = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
-            constexpr uint32_t PV = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
+    } else if (warp == W_QK || warp == W_PV) {
+        // The scores' MMAs and the products' by a warp each: a wait or a commit
+        // takes 100 to 250 clocks before the next MMA issues, and the tensor
+        // cores, which hold but a few MMAs ahead, work for the other warp
+        // meanwhile. The whole warp walks the loop, so that addresses and
+        // descriptors are uniform (an MMA issues in a few clocks, not in 80);
+        // one elected thread issues. A descriptor's address counts 16 bytes in
+        // its low word, and no tile passes its 18 bits.
+        constexpr uint32_t TYPE = F16 ? 0 : (1u << 7) | (1u << 10);
+        auto wait = [&](uint64_t *bar, uint32_t phase) {
+            const bool ok = wait_soon(bar, phase & 1, gone, A.err);
+            tc_fence_after();
+            return ok;
+        };
+        bool ok = true;
+        if (warp == W_QK && n > 0) {
+            constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
             const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(ring);
-            const uint64_t v_desc = sw128_desc_mn(ring + C::KV_BYTES, BN * 128);
-            auto wait = [&](uint64_t *bar, uint32_t phase) {
-                if (!__all_sync(0xffffffffu, wait_soon(bar, phase & 1, gone))) {
-                    if (lane == 0) give_up();
-                    return false;
-                }
-                tc_fence_after();
-                return true;
-            };
-            bool ok = wait(&q_full, 0);
             uint32_t used = 0;  // score tiles so far: the next waits until the last is in registers
-            for (int t = 0; ok && t <= n; t++) {
-                const int st = t % ST;
-                if (!(ok = wait(&full[st], t / ST))) break;
-                const uint64_t kt = k_desc + st * (2 * C::KV_BYTES >> 4), vt = v_desc + st * (2 * C::KV_BYTES >> 4);
+            ok = wait(&q_full, 0);
+            for (int i = 0; ok && i < n; i++) {
+                const uint32_t u = slot_of_k(i), at = u % SLOTS;
+                const uint64_t kt = k_desc + at * (C::KV_BYTES >> 4);
+                if (!(ok = wait(&full[at], u / SLOTS))) break;
+                for (int q = 0; q < nq; q++) {
+                    if (used > 0 && !(ok = wait(&s_free, used - 1))) break;
+                    used++;
+                    const uint64_t qt = q_desc + q * (C::Q_BYTES >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < DP / 16; ks++)
+                            tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
+                                        kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), ID, ks > 0);
+                        tc_commit(&s_full[q]);
+                        if (q == nq - 1) tc_commit(&empty[at]);
+                    }
+                }
+            }
+        } else if (n > 0) {
+            constexpr uint32_t ID = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
+            const uint64_t v_desc = sw128_desc_mn(ring, BN * 128);
+            for (int i = 0; ok && i < n; i++) {
+                const uint32_t u = slot_of_v(i, n), at = u % SLOTS;
+                const uint64_t vt = v_desc + at * (C::KV_BYTES >> 4);
+                if (!(ok = wait(&full[at], u / SLOTS))) break;
                 for (int q = 0; ok && q < nq; q++) {
-                    if (t < n) {
-                        if (used > 0 && !(ok = wait(&s_free, used - 1))) break;
-                        used++;
-                        const uint64_t qt = q_desc + q * (C::Q_BYTES >> 4);
+                    const uint32_t p_at = tmem + C::P_COL + q * (BN / 2);
+#pragma unroll
+                    for (int h = 0; h < PARTS; h++) {
+                        if (!(ok = wait(&p_full[q][h], i))) break;
                         if (elect_one()) {
 #pragma unroll
-                            for (int ks = 0; ks < DP / 16; ks++)
-                                tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
-                                            kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), QK, ks > 0);
-                            tc_commit(&s_full[q]);
-                        }
-                    }
-                    if (t > 0) {
-                        const uint32_t p_at = tmem + C::P_COL + q * (BN / 2);
-#pragma unroll
-                        for (int h = 0; h < PARTS; h++) {
-                            if (!(ok = wait(&p_full[q][h], t - 1))) break;
-                            if (elect_one()) {
-#pragma unroll
-                                for (int ks = h * (C::PART / 16); ks < (h + 1) * (C::PART / 16); ks++)
-                                    tc_mma_f16_ts(tmem + C::O_COL + q * DP, p_at + ks * 8, vt + (ks * 16 * 128 >> 4),
-                                                  PV, t > 1 || ks > 0);
-                                if (h == PARTS - 1) tc_commit(&pv_done[q]);
+                            for (int ks = h * (C::PART / 16); ks < (h + 1) * (C::PART / 16); ks++)
+                                tc_mma_f16_ts(tmem + C::O_COL + q * DP, p_at + ks * 8, vt + (ks * 16 * 128 >> 4), ID,
+                                              i > 0 || ks > 0);
+                            if (h == PARTS - 1) {
+                                tc_commit(&pv_done[q]);
+                                if (q == nq - 1) tc_commit(&empty[at]);
                             }
                         }
                     }
                 }
-                if (ok && elect_one()) tc_commit(&empty[st]);
             }
-            if (!ok) {  // what was issued still ends before TMEM goes
-                if (elect_one()) tc_commit(&drained);
-                mbar_wait_bounded(&drained, 0, nullptr, WAIT_LIMIT_NS);
-            }
+        }
+        if (!ok) {  // what was issued still ends before TMEM goes
+            if (elect_one()) tc_commit(&drained[warp - W_QK]);
+            mbar_wait_bounded(&drained[warp - W_QK], 0, nullptr, WAIT_LIMIT_NS);
         }
         __syncwarp();
     } else if (warp / 4 < nq) {
@@ -804,16 +842,12 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const int t = tq0 + row / A.group;
         const bool valid = row < per_tile * A.group && t < t1;
         const int lo = valid ? row_lo(A, s, t) : 0, hi = valid ? row_hi(A, s, t) : 0;
-        const key_span mine = span_of(A, s, tq0, tq1 - 1);
+        // tiles [i0, i1) are seen whole by every row of the block
+        const int i0 = max(0, sp.clo - from + BN - 1) / BN, i1 = max(0, min(sp.chi, to) - from) / BN;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int i = 0; i < n; i++) {
-            ok = wait_soon(&s_full[q], i & 1, gone);
-            if (!__all_sync(0xffffffffu, ok)) {
-                if (lane == 0) give_up();
-                ok = false;
-                break;
-            }
+            if (!(ok = wait_soon(&s_full[q], i & 1, gone, A.err))) break;
             tc_fence_after();
             uint32_t x[BN / 32][32];
 #pragma unroll
@@ -823,25 +857,19 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free);
-            const int key0 = from + i * BN;
-            if (key0 < mine.clo || key0 + BN > min(mine.chi, to)) {
-                const int a = lo - key0, z = min(hi, to) - key0;
+            if (i < i0 || i >= i1) {
+                const int key0 = from + i * BN, a = lo - key0, z = min(hi, to) - key0;
 #pragma unroll
                 for (int c = 0; c < BN / 32; c++)
 #pragma unroll
                     for (int e = 0; e < 32; e++)
                         if (c * 32 + e < a || c * 32 + e >= z) x[c][e] = 0xff800000u;
-            }
-            if (key0 < sp.clo || key0 + BN > min(sp.chi, to)) {
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
-                if (!__all_sync(0xffffffffu, wait_soon(&full[(i + 1) % ST], ((i + 1) / ST) & 1, gone))) {
-                    if (lane == 0) give_up();
-                    ok = false;
-                    break;
-                }
+                const uint32_t at = slot_of_v(i, n);
+                if (!(ok = wait_soon(&full[at % SLOTS], (at / SLOTS) & 1, gone, A.err))) break;
                 bool found = false;
-                uint8_t *vt = ring + ((i + 1) % ST * 2 + 1) * C::KV_BYTES;
+                uint8_t *vt = ring + at % SLOTS * C::KV_BYTES;
                 for (int e = row; e < C::KV_BYTES / 16; e += 128) {
                     const int key = key0 + e / 8 % BN;
                     if (key >= sp.clo && key < min(sp.chi, to)) continue;
@@ -873,62 +901,50 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             // a NaN or an infinite score: the row's weights are NaN, as the formula's
             const bool odd = !(mx < INFINITY);
             mx = odd ? m : fmaxf(m, mx);
-            if (i > 0) {  // the product before is done: its P may go, and o may be touched
-                ok = wait_soon(&pv_done[q], (i - 1) & 1, gone);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    if (lane == 0) give_up();
-                    ok = false;
-                    break;
+            if (i == 0) {
+                m = mx;
+            } else {
+                // the product before is done: its P may go, and o may be touched
+                const bool done = mbar_try_wait(&pv_done[q], (i - 1) & 1);
+                if (__any_sync(0xffffffffu, !done || mx > m + LAZY)) {
+                    if (!(ok = wait_soon(&pv_done[q], (i - 1) & 1, gone, A.err))) break;
+                    tc_fence_after();
+                    if (__any_sync(0xffffffffu, mx > m + LAZY)) {  // o relative to the new maxima
+                        const float f = mx == m ? 1.0f : exp2_fast(m - mx);
+#pragma unroll 1
+                        for (int c = 0; c < DP / 32; c++) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(o_at + c * 32, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st_32x32b_x32(o_at + c * 32, o);
+                        }
+                        l *= f;
+                        m = mx;
+                    }
                 }
                 tc_fence_after();
             }
-            if (i == 0) {
-                m = mx;
-            } else if (__any_sync(0xffffffffu, mx > m + LAZY)) {
-                // o relative to the new maxima
-                const float f = mx == m ? 1.0f : exp2_fast(m - mx);
-#pragma unroll 1
-                for (int c = 0; c < DP / 32; c++) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(o_at + c * 32, o);
-                    tmem_ld_wait(o);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tmem_st_32x32b_x32(o_at + c * 32, o);
-                }
-                l *= f;
-                m = mx;
-            }
             const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
+            uint64_t s0 = 0, s1 = 0;
 #pragma unroll
             for (int h = 0; h < PARTS; h++) {
                 uint32_t p[32];
-                weights<F16>(x[2 * h], A.scale_log2, base, p);
-                weights<F16>(x[2 * h + 1], A.scale_log2, base, p + 16);
+                weights<F16>(x[2 * h], A.scale_log2, base, p, s0, s1);
                 tmem_st_32x32b_x32(tmem + lanes + C::P_COL + q * (BN / 2) + h * 32, p);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[q][h]);
             }
-            // the sums while the tensor cores work
-            uint64_t sum[4] = {};
-#pragma unroll
-            for (int c = 0; c < BN / 32; c++)
-#pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                    sum[e / 2 % 4] = add2(sum[e / 2 % 4], pack2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])));
             float sa, sb;
-            unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sa, sb);
+            unpack2(add2(s0, s1), sa, sb);
             l += sa + sb;
         }
         // the last product
         if (ok && n > 0) {
-            ok = wait_soon(&pv_done[q], (n - 1) & 1, gone);
-            if (!__all_sync(0xffffffffu, ok)) {
-                if (lane == 0) give_up();
-                ok = false;
-            }
+            ok = wait_soon(&pv_done[q], (n - 1) & 1, gone, A.err);
             tc_fence_after();
         }
         if (ok) {
@@ -973,7 +989,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == W_MMA) {
+    if (warp == W_QK) {
         tc_fence_after();
         tmem_dealloc(tmem, C::COLS);
     }
