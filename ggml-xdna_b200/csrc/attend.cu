@@ -540,7 +540,7 @@ struct many_rows {
     static constexpr int SLOTS = DP == 64 ? 8 : 5;  // tiles of K or V in flight or in use
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
-    static constexpr int THREADS = SOFTMAX + 96;    // and a warp each for Q K^T, P V and the copies
+    static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V and the copies, one idle
     // TMEM columns: O of each query tile, the scores, P of each query tile
     static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
     static_assert(P_COL + NQ * BN / 2 <= COLS, "TMEM holds O, S and P");
@@ -583,7 +583,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // A warp's wait: one look, and the rest, for at most WAIT_LIMIT_NS or until
 // *gone, out of line. The same answer in every lane; a wait that runs out sets
 // *gone and the error bit.
-__device__ __noinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile int *gone, unsigned *err) {
+__device__ __forceinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile int *gone, unsigned *err) {
     const uint64_t t0 = global_ns();
     bool ok = false;
     for (uint32_t it = 1; !ok; it++) {
@@ -714,10 +714,16 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     const uint32_t tmem = tmem_sh;
     volatile int *const gone = &stop;
 
+    // A row of scores lives in registers: the softmax warps take the others'
+    // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
+    auto fewer = [] {
+        if (NQ > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    };
     // The tiles' order in the ring: K(0) K(1) V(0) K(2) V(1) ... K(n - 1) V(n - 2) V(n - 1).
     auto slot_of_k = [](int i) { return (uint32_t) max(0, 2 * i - 1); };
     auto slot_of_v = [](int i, int n) { return (uint32_t) (i + 1 < n ? 2 * i + 2 : 2 * i + 1); };
     if (warp == W_COPY) {
+        fewer();
         // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
         // the lower half of the warp, V's by the upper
         const int box = min(A.page_size, KEYS), boxes = BN / box, which = lane % 16;
@@ -766,6 +772,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, nullptr, WAIT_LIMIT_NS);
         if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_QK || warp == W_PV) {
+        fewer();
         // The scores' MMAs and the products' by a warp each: a wait or a commit
         // takes 100 to 250 clocks before the next MMA issues, and the tensor
         // cores, which hold but a few MMAs ahead, work for the other warp
@@ -834,7 +841,10 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_wait_bounded(&drained[warp - W_QK], 0, nullptr, WAIT_LIMIT_NS);
         }
         __syncwarp();
-    } else if (warp / 4 < nq) {
+    } else if (warp > W_COPY) {
+        fewer();
+    } else {
+        if (NQ > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp / 4, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t) (warp % 4 * 32) << 16;
         const uint32_t o_at = tmem + lanes + C::O_COL + q * DP;
@@ -845,8 +855,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         // tiles [i0, i1) are seen whole by every row of the block
         const int i0 = max(0, sp.clo - from + BN - 1) / BN, i1 = max(0, min(sp.chi, to) - from) / BN;
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int i = 0; i < n; i++) {
+        bool ok = q < nq;
+        for (int i = 0; ok && i < n; i++) {
             if (!(ok = wait_soon(&s_full[q], i & 1, gone, A.err))) break;
             tc_fence_after();
             uint32_t x[BN / 32][32];
@@ -857,6 +867,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free);
+            // is the product before done? Then its P may go, and o may be touched
+            const bool done = i == 0 || mbar_try_wait(&pv_done[q], (i - 1) & 1);
             if (i < i0 || i >= i1) {
                 const int key0 = from + i * BN, a = lo - key0, z = min(hi, to) - key0;
 #pragma unroll
@@ -898,18 +910,16 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     for (int k = 0; k < 4; k++)
                         top[k] = max3_nan(top[k], __uint_as_float(x[c][e + k]), __uint_as_float(x[c][e + 4 + k]));
             float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * A.scale_log2;
-            // a NaN or an infinite score: the row's weights are NaN, as the formula's
-            const bool odd = !(mx < INFINITY);
-            mx = odd ? m : fmaxf(m, mx);
-            if (i == 0) {
-                m = mx;
-            } else {
-                // the product before is done: its P may go, and o may be touched
-                const bool done = mbar_try_wait(&pv_done[q], (i - 1) & 1);
-                if (__any_sync(0xffffffffu, !done || mx > m + LAZY)) {
-                    if (!(ok = wait_soon(&pv_done[q], (i - 1) & 1, gone, A.err))) break;
-                    tc_fence_after();
-                    if (__any_sync(0xffffffffu, mx > m + LAZY)) {  // o relative to the new maxima
+            float base = m == -INFINITY ? 0.0f : -m;
+            const bool rose = !(mx <= m + LAZY);  // or NaN
+            if (__any_sync(0xffffffffu, rose || !done)) {
+                if (!(ok = i == 0 || wait_soon(&pv_done[q], (i - 1) & 1, gone, A.err))) break;
+                tc_fence_after();
+                if (__any_sync(0xffffffffu, rose)) {
+                    // a NaN or an infinite score: the row's weights are NaN, as the formula's
+                    const bool odd = !(mx < INFINITY);
+                    mx = odd ? m : fmaxf(m, mx);
+                    if (i > 0) {  // o relative to the new maxima
                         const float f = mx == m ? 1.0f : exp2_fast(m - mx);
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; c++) {
@@ -921,12 +931,12 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                             tmem_st_32x32b_x32(o_at + c * 32, o);
                         }
                         l *= f;
-                        m = mx;
                     }
+                    m = mx;
+                    base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
                 }
-                tc_fence_after();
             }
-            const float base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
+            tc_fence_after();
             uint64_t s0 = 0, s1 = 0;
 #pragma unroll
             for (int h = 0; h < PARTS; h++) {
