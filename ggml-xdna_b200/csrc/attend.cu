@@ -68,42 +68,54 @@ __device__ __forceinline__ key_span span_of(const attend_args &A, const kv_seq &
     return { row_lo(A, s, t_lo), row_hi(A, s, t_hi), row_lo(A, s, t_hi), row_hi(A, s, t_lo) };
 }
 
-// Eight results of one row, from column c on: as asked for in the cache's
-// type, in f32, and as the next matmul's operand.
+// Eight results of one row: rounded to the cache's type, and as the next
+// matmul's operand.
+template <bool F16>
+__device__ __forceinline__ uint4 round8(const float (&o)[8]) {
+    return make_uint4(kv_bits2<F16>(o[0], o[1]), kv_bits2<F16>(o[2], o[3]), kv_bits2<F16>(o[4], o[5]),
+                      kv_bits2<F16>(o[6], o[7]));
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&o)[8]) {
+    uint8_t enc[9];
+    uint32_t bf[4];
+    encode_block(o, enc, bf);
+    return make_uint4(bf[0], bf[1], bf[2], bf[3]);
+}
+
+__device__ __forceinline__ void store8_f32(const attend_args &A, int64_t t, int head, int c, const float (&o)[8]) {
+    float4 *y = reinterpret_cast<float4 *>(A.y + t * A.ldy + (int64_t) head * A.d + c);
+    y[0] = make_float4(o[0], o[1], o[2], o[3]);
+    y[1] = make_float4(o[4], o[5], o[6], o[7]);
+}
+
+// As asked for: in the cache's type, in f32, and as the next matmul's operand.
 template <bool F16>
 __device__ __forceinline__ void store8(const attend_args &A, int64_t t, int head, int c, const float (&o)[8]) {
     const int64_t col = (int64_t) head * A.d + c;
-    if (A.out) {
-        uint4 w;
-        w.x = kv_bits2<F16>(o[0], o[1]);
-        w.y = kv_bits2<F16>(o[2], o[3]);
-        w.z = kv_bits2<F16>(o[4], o[5]);
-        w.w = kv_bits2<F16>(o[6], o[7]);
-        *reinterpret_cast<uint4 *>(A.out + t * A.ldo + col) = w;
-    }
-    if (A.y) {
-        float4 *y = reinterpret_cast<float4 *>(A.y + t * A.ldy + col);
-        y[0] = make_float4(o[0], o[1], o[2], o[3]);
-        y[1] = make_float4(o[4], o[5], o[6], o[7]);
-    }
-    if (A.a_next) {
-        uint8_t enc[9];
-        uint32_t bf[4];
-        encode_block(o, enc, bf);
-        *reinterpret_cast<uint4 *>(A.a_next + t * A.lda + col) = make_uint4(bf[0], bf[1], bf[2], bf[3]);
-    }
+    if (A.out) *reinterpret_cast<uint4 *>(A.out + t * A.ldo + col) = round8<F16>(o);
+    if (A.y) store8_f32(A, t, head, c, o);
+    if (A.a_next) *reinterpret_cast<uint4 *>(A.a_next + t * A.lda + col) = pack8(o);
 }
 
 // A NaN or infinite value that some rows of a tile see and others do not is
 // taken as zero in the tile's product (0 times it would reach every row) and
-// added here to the rows that see it: keys [lo, hi) of the row's own range.
+// added here to a row that sees keys [lo, hi), from those of them outside
+// [clo, chi), which every row sees.
 template <bool F16>
-__device__ void add_not_finite(const attend_args &A, int s, int kv_head, int c, int lo, int hi, float (&o)[8]) {
+__device__ __forceinline__ void add_not_finite(const attend_args &A, int s, int kv_head, int c, int lo, int hi, int clo,
+                                               int chi, float (&o)[8]) {
+#pragma unroll 1
     for (int j = lo; j < hi; j++) {
+        if (j >= clo && j < chi) {
+            j = chi - 1;
+            continue;
+        }
         const int64_t page = A.b.table[s * A.b.table_stride + j / A.page_size];
         if (page < 0 || page >= A.pages) continue;
         const uint16_t *v =
             A.v + page * A.page_stride + j % A.page_size * A.token_stride + kv_head * A.head_stride + c;
+#pragma unroll
         for (int i = 0; i < 8; i++) {
             const float x = kv_value<F16>(v[i]);
             if (!(fabsf(x) <= 3.4028234e38f)) o[i] += x;
@@ -447,8 +459,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(os[(k * ROWS + row) * LD + c + e], w[k], x[e]);
         if (not_finite && live && c < A.d) {
             const int a = (int) max((int64_t) row_lo(A, s, t), from), z = (int) min((int64_t) row_hi(A, s, t), to);
-            add_not_finite<F16>(A, seq, kv_head, c, a, min(z, sp.clo), x);
-            add_not_finite<F16>(A, seq, kv_head, c, max(a, max(sp.chi, sp.clo)), z, x);
+            add_not_finite<F16>(A, seq, kv_head, c, a, z, sp.clo, max(sp.clo, sp.chi), x);
         }
         if (A.join) {  // over the first warp's part, which this thread alone reads
             float4 *dst = reinterpret_cast<float4 *>(os + row * LD + c);
@@ -541,9 +552,12 @@ struct many_rows {
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
     static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V and the copies, one idle
+    // Buffers of P: two where one query tile has the block to itself, since the
+    // next scores' MMAs (1,000 clocks at 256 columns) go ahead of P's otherwise
+    static constexpr int NP = NQ > 1 ? 1 : 2;
     // TMEM columns: O of each query tile, the scores, P of each query tile
     static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
-    static_assert(P_COL + NQ * BN / 2 <= COLS, "TMEM holds O, S and P");
+    static_assert(P_COL + NQ * NP * BN / 2 <= COLS, "TMEM holds O, S and P");
 };
 
 // A rise of the running maximum below this (in powers of two) leaves the
@@ -659,11 +673,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, BN = C::BN, SLOTS = C::SLOTS, PARTS = C::PARTS;
+    constexpr int NQ = C::NQ, NP = C::NP, BN = C::BN, SLOTS = C::SLOTS, PARTS = C::PARTS;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
     uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // of tiles of K and V
-    __shared__ uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ], drained[2];
+    __shared__ uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ][NP], drained[2];
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -695,7 +709,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         for (int i = 0; i < NQ; i++) {
             mbar_init(&s_full[i], 1);
             for (int h = 0; h < PARTS; h++) mbar_init(&p_full[i][h], 4);
-            mbar_init(&pv_done[i], 1);
+            for (int b = 0; b < NP; b++) mbar_init(&pv_done[i][b], 1);
         }
         mbar_init(&s_free, 4);
         mbar_init(&drained[0], 1);
@@ -818,7 +832,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 const uint64_t vt = v_desc + at * (C::KV_BYTES >> 4);
                 if (!(ok = wait(&full[at], u / SLOTS))) break;
                 for (int q = 0; ok && q < nq; q++) {
-                    const uint32_t p_at = tmem + C::P_COL + q * (BN / 2);
+                    const uint32_t p_at = tmem + C::P_COL + (q * NP + i % NP) * (BN / 2);
 #pragma unroll
                     for (int h = 0; h < PARTS; h++) {
                         if (!(ok = wait(&p_full[q][h], i))) break;
@@ -828,7 +842,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                                 tc_mma_f16_ts(tmem + C::O_COL + q * DP, p_at + ks * 8, vt + (ks * 16 * 128 >> 4), ID,
                                               i > 0 || ks > 0);
                             if (h == PARTS - 1) {
-                                tc_commit(&pv_done[q]);
+                                tc_commit(&pv_done[q][i % NP]);
                                 if (q == nq - 1) tc_commit(&empty[at]);
                             }
                         }
@@ -867,8 +881,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free);
-            // is the product before done? Then its P may go, and o may be touched
-            const bool done = i == 0 || mbar_try_wait(&pv_done[q], (i - 1) & 1);
+            // the last product of P's buffer is done: P may go
+            if (i >= NP) {
+                if (!(ok = wait_soon(&pv_done[q][i % NP], (i / NP - 1) & 1, gone, A.err))) break;
+                tc_fence_after();
+            }
             if (i < i0 || i >= i1) {
                 const int key0 = from + i * BN, a = lo - key0, z = min(hi, to) - key0;
 #pragma unroll
@@ -912,37 +929,36 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * A.scale_log2;
             float base = m == -INFINITY ? 0.0f : -m;
             const bool rose = !(mx <= m + LAZY);  // or NaN
-            if (__any_sync(0xffffffffu, rose || !done)) {
-                if (!(ok = i == 0 || wait_soon(&pv_done[q], (i - 1) & 1, gone, A.err))) break;
-                tc_fence_after();
-                if (__any_sync(0xffffffffu, rose)) {
-                    // a NaN or an infinite score: the row's weights are NaN, as the formula's
-                    const bool odd = !(mx < INFINITY);
-                    mx = odd ? m : fmaxf(m, mx);
-                    if (i > 0) {  // o relative to the new maxima
-                        const float f = mx == m ? 1.0f : exp2_fast(m - mx);
-#pragma unroll 1
-                        for (int c = 0; c < DP / 32; c++) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(o_at + c * 32, o);
-                            tmem_ld_wait(o);
-#pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st_32x32b_x32(o_at + c * 32, o);
-                        }
-                        l *= f;
-                    }
-                    m = mx;
-                    base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
+            if (__any_sync(0xffffffffu, rose)) {
+                if (i > 0 && NP > 1) {  // and the last product into o
+                    if (!(ok = wait_soon(&pv_done[q][(i - 1) % NP], ((i - 1) / NP) & 1, gone, A.err))) break;
+                    tc_fence_after();
                 }
+                // a NaN or an infinite score: the row's weights are NaN, as the formula's
+                const bool odd = !(mx < INFINITY);
+                mx = odd ? m : fmaxf(m, mx);
+                if (i > 0) {  // o relative to the new maxima
+                    const float f = mx == m ? 1.0f : exp2_fast(m - mx);
+#pragma unroll 1
+                    for (int c = 0; c < DP / 32; c++) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(o_at + c * 32, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st_32x32b_x32(o_at + c * 32, o);
+                    }
+                    l *= f;
+                }
+                m = mx;
+                base = odd ? NAN : m == -INFINITY ? 0.0f : -m;
             }
-            tc_fence_after();
             uint64_t s0 = 0, s1 = 0;
 #pragma unroll
             for (int h = 0; h < PARTS; h++) {
                 uint32_t p[32];
                 weights<F16>(x[2 * h], A.scale_log2, base, p, s0, s1);
-                tmem_st_32x32b_x32(tmem + lanes + C::P_COL + q * (BN / 2) + h * 32, p);
+                tmem_st_32x32b_x32(tmem + lanes + C::P_COL + (q * NP + i % NP) * (BN / 2) + h * 32, p);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -954,43 +970,86 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         }
         // the last product
         if (ok && n > 0) {
-            ok = wait_soon(&pv_done[q], (n - 1) & 1, gone, A.err);
+            ok = wait_soon(&pv_done[q][(n - 1) % NP], ((n - 1) / NP) & 1, gone, A.err);
             tc_fence_after();
         }
         if (ok) {
             const int head = kv_head * A.group + row % A.group;
             const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
-            const float inv = A.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const int fa = max(lo, from), fz = min(hi, to);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (not_finite) {
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld_32x32b_x32(o_at + c, o);
-                    tmem_ld_wait(o);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0;
-                }
-                if (!valid) continue;
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (c + e >= A.d) break;
+                for (int c = 0; c < DP; c += 8) {
                     float r[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) r[k] = __uint_as_float(o[e + k]);
-                    if (not_finite) {
-                        add_not_finite<F16>(A, seq, kv_head, c + e, fa, min(fz, sp.clo), r);
-                        add_not_finite<F16>(A, seq, kv_head, c + e, max(fa, max(sp.chi, sp.clo)), fz, r);
-                    }
-                    if (A.splits > 1) {
-                        float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c + e);
-                        dst[0] = make_float4(r[0], r[1], r[2], r[3]);
-                        dst[1] = make_float4(r[4], r[5], r[6], r[7]);
+                    tmem_ld_32x32b_x8(o_at + c, r);
+                    if (valid && c < A.d)
+                        add_not_finite<F16>(A, seq, kv_head, c, max(lo, from), min(hi, to), sp.clo, max(sp.clo, sp.chi), r);
+                    tmem_st_32x32b_x8(o_at + c, r);
+                }
+            }
+            // Rolled, since every block comes through here once and pays for
+            // each line of code. 16-bit results go through the query tile's
+            // shared memory (its scores are all made), a row of DP a thread, 16
+            // bytes at unit ^ (row % 8), and out of it in whole rows.
+            uint8_t *const rows16 = q_sm + q * C::Q_BYTES + warp % 4 * 32 * (DP * 2);
+            const bool whole = A.splits == 1;
+#pragma unroll 1
+            for (int pass = 0; pass < (whole && A.a_next ? 2 : 1); pass++) {  // A.out and the rest; A.a_next
+                __syncwarp();
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tmem_ld_32x32b_x32(o_at + c, o);
+                        tmem_ld_wait(o);
                     } else {
 #pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0;
+                    }
+                    if (!valid) continue;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float r[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) r[k] = __uint_as_float(o[e + k]);
+                        if (!whole) {  // (the workspace's rows have room for DP values)
+                            float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c + e);
+                            dst[0] = make_float4(r[0], r[1], r[2], r[3]);
+                            dst[1] = make_float4(r[4], r[5], r[6], r[7]);
+                            continue;
+                        }
+#pragma unroll
                         for (int k = 0; k < 8; k++) r[k] *= inv;
-                        store8<F16>(A, tok, head, c + e, r);
+                        uint4 *at =
+                            reinterpret_cast<uint4 *>(rows16 + lane * (DP * 2) + (((c + e) / 8 ^ (lane & 7)) << 4));
+                        if (pass == 1) *at = pack8(r);
+                        else {
+                            if (A.out) *at = round8<F16>(r);
+                            if (A.y && c + e < A.d) store8_f32(A, tok, head, c + e, r);
+                        }
+                    }
+                }
+                uint16_t *const base = pass == 0 ? A.out : A.a_next;
+                if (!whole || !base) continue;
+                __syncwarp();
+                const int64_t ld = pass == 0 ? A.ldo : A.lda;
+                constexpr int UNITS = DP / 8, AT_ONCE = 32 / UNITS, N = 4;
+                const int u = lane % UNITS, rows = min(32, (tq1 - tq0) * A.group - warp % 4 * 32);
+                uint16_t *const col = base + kv_head * A.group * A.d + u * 8;
+                int g = (warp % 4 * 32 + lane / UNITS) % A.group, tk = (warp % 4 * 32 + lane / UNITS) / A.group;
+#pragma unroll 1
+                for (int r0 = lane / UNITS; r0 < rows; r0 += N * AT_ONCE) {
+                    uint4 v[N];
+#pragma unroll
+                    for (int k = 0; k < N; k++) {
+                        const int r = (r0 + k * AT_ONCE) & 31;
+                        v[k] = *reinterpret_cast<const uint4 *>(rows16 + r * (DP * 2) + ((u ^ (r & 7)) << 4));
+                    }
+#pragma unroll
+                    for (int k = 0; k < N; k++) {
+                        if (r0 + k * AT_ONCE < rows && u * 8 < A.d)
+                            *reinterpret_cast<uint4 *>(col + (s.q0 + (int64_t) (tq0 + tk)) * ld + g * A.d) = v[k];
+                        for (g += AT_ONCE; g >= A.group; g -= A.group) tk++;
                     }
                 }
             }
