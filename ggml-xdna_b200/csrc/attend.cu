@@ -165,6 +165,14 @@ __device__ __forceinline__ bool bad_half(uint32_t h) {
     return (h & m) == m;
 }
 
+// Whether one of eight halves is NaN or infinite: one more in an exponent of
+// all ones carries into the sign's place.
+template <bool F16>
+__device__ __forceinline__ bool any_bad(const uint4 &w) {
+    const uint32_t m = F16 ? 0x7c007c00u : 0x7f807f80u, one = F16 ? 0x04000400u : 0x00800080u;
+    return (((w.x & m) + one) | ((w.y & m) + one) | ((w.z & m) + one) | ((w.w & m) + one)) & 0x80008000u;
+}
+
 // A stage's bytes, and as many stages as keep about 64 KB in flight on an SM.
 template <int DP>
 struct few_rows {
@@ -887,33 +895,40 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 tc_fence_after();
             }
             if (i < i0 || i >= i1) {
-                const int key0 = from + i * BN, a = lo - key0, z = min(hi, to) - key0;
+                const int key0 = from + i * BN, z = min(hi, to) - key0;
+                if (A.window) {
+                    const int a = lo - key0;
+#pragma unroll
+                    for (int c = 0; c < BN / 32; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (c * 32 + e < a) x[c][e] = 0xff800000u;
+                }
 #pragma unroll
                 for (int c = 0; c < BN / 32; c++)
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (c * 32 + e < a || c * 32 + e >= z) x[c][e] = 0xff800000u;
+                        if (c * 32 + e >= z) x[c][e] = 0xff800000u;
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
                 const uint32_t at = slot_of_v(i, n);
                 if (!(ok = wait_soon(&full[at % SLOTS], (at / SLOTS) & 1, gone, A.err))) break;
-                bool found = false;
                 uint8_t *vt = ring + at % SLOTS * C::KV_BYTES;
+                const int c0 = sp.clo - key0, c1 = min(sp.chi, to) - key0;
+                bool found = false;
+#pragma unroll 4
                 for (int e = row; e < C::KV_BYTES / 16; e += 128) {
-                    const int key = key0 + e / 8 % BN;
-                    if (key >= sp.clo && key < min(sp.chi, to)) continue;
+                    const int key = e / 8 % BN;
                     uint4 w = *reinterpret_cast<uint4 *>(vt + e * 16);
+                    if ((key >= c0 && key < c1) || !any_bad<F16>(w)) continue;
                     uint32_t h[4] = { w.x, w.y, w.z, w.w };
-                    bool bad = false;
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        if (bad_half<F16>(h[k])) h[k] &= 0xffff0000u, bad = true;
-                        if (bad_half<F16>(h[k] >> 16)) h[k] &= 0x0000ffffu, bad = true;
+                        if (bad_half<F16>(h[k])) h[k] &= 0xffff0000u;
+                        if (bad_half<F16>(h[k] >> 16)) h[k] &= 0x0000ffffu;
                     }
-                    if (bad) {
-                        *reinterpret_cast<uint4 *>(vt + e * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-                        found |= key < to;
-                    }
+                    *reinterpret_cast<uint4 *>(vt + e * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                    found |= key0 + key < to;
                 }
                 if (found) not_finite = 1;
                 fence_proxy_async_shared();
