@@ -9,11 +9,11 @@
 // base 2 (the scale times log2 e folded into one multiply-add):
 //   m' = max(m, s_j),  o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j,  l' alike.
 //
-// A long row of keys is cut into chunks that different blocks take. Few rows
-// in at most 8 chunks: the blocks are one cluster and join their o, m and l
-// through each other's shared memory. More chunks, or many rows: each leaves
-// its unnormalised o, m and l in the workspace, joined in order by
-// kv_combine_kernel. With one chunk the result is written at once.
+// A long row of keys is cut into chunks that different blocks take. Few rows:
+// the blocks of up to 8 chunks are a cluster and join their o, m and l through
+// each other's shared memory. What more than one cluster, or (many rows) more
+// than one block made of a row goes to the workspace, unnormalised, with its m
+// and l, and kv_combine_kernel joins it in order.
 #include "zest_kv.cuh"
 
 #include <algorithm>
@@ -43,9 +43,10 @@ struct attend_args {
     int64_t ldy;
     uint16_t *a_next;
     int64_t lda;
-    int64_t chunk;      // keys a block takes, a multiple of 64; splits chunks at most
-    int splits;
-    int join;           // the chunks' blocks are a cluster (few rows): each sequence in equal chunks
+    int64_t chunk;      // many rows: keys a block takes, a multiple of 128
+    int splits;         // parts of a row that go to the workspace (1: none does, the result is whole)
+    int join;           // few rows: blocks of a cluster; each sequence's keys in splits * join equal chunks
+    int wide;           // few rows: a box has a head's columns whole
     float2 *ml;         // [splits][T * heads]: m and l
     float *part;        // [splits][T * heads][DP]: o
     unsigned *err;
@@ -185,9 +186,12 @@ struct few_rows {
 constexpr int FEW_THREADS = 160;  // four warps of products, one that copies
 
 // A block: up to 16 rows of one kv head of one sequence over one chunk of
-// keys. Warp 4 brings 64 keys a stage by TMA, page by page (K and V as
-// 64-column blocks, 128-byte swizzle); warps 0-3 take 16 keys of a stage
-// each, with a running m, l and o of their own, joined at the end.
+// keys. Warp 4 brings 64 keys a stage by TMA in boxes of min(page, 64) keys
+// (64-column blocks of 128-byte rows, swizzled; all of a head's blocks in one
+// box where it is whole blocks: a box costs the TMA unit about 45 clocks
+// besides 2 a row, and 32 sequences in pages of 16 took 142 us with a box a
+// block); warps 0-3 take 16 keys of a stage each, with a running m, l and o of
+// their own, joined at the end.
 template <int DP, bool F16>
 __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid_constant__ CUtensorMap tk,
                                                                     const __grid_constant__ CUtensorMap tv,
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     __shared__ int stop, not_finite;
     __shared__ float m_sh[4][ROWS], l_sh[4][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int seq = blockIdx.z, split = blockIdx.x;
+    const int seq = blockIdx.z, split = blockIdx.x / A.join, rank = blockIdx.x % A.join;
     const int row_tiles = gridDim.y / (A.heads / A.group);
     const int kv_head = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
 
@@ -212,13 +216,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     if (r0 >= rows) return;
     const key_span sp = span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + ROWS, rows) - 1) / A.group));
     // this block's keys: from the first of the span's 64-key block on, by chunks
-    const int64_t first = (int64_t) sp.lo / KEYS * KEYS;
-    const int64_t chunk =
-        A.join ? ((max((int64_t) sp.hi - first, (int64_t) 1) + KEYS - 1) / KEYS + A.splits - 1) / A.splits * KEYS
-               : A.chunk;
-    const int64_t from = first + split * chunk, to = min((int64_t) sp.hi, from + chunk);
+    const int64_t first = (int64_t) sp.lo / KEYS * KEYS, blocks = (max((int64_t) sp.hi - first, (int64_t) 0) + KEYS - 1) / KEYS;
+    const int64_t chunk = (blocks + gridDim.x - 1) / gridDim.x * KEYS;
+    const int64_t from = min(first + blockIdx.x * chunk, (int64_t) sp.hi), to = min((int64_t) sp.hi, from + chunk);
     const int steps = to > from ? (int) ((to - from + KEYS - 1) / KEYS) : 0;
-    if (steps == 0 && split > 0 && !A.join) return;  // kv_combine_kernel counts the chunks as this does
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; i++) {
@@ -232,12 +233,14 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     __syncthreads();
 
     if (warp == 4) {
-        // boxes of min(page, 64) keys by 64 columns; a lane brings one of them
-        const int box = min(A.page_size, KEYS), boxes = KEYS / box, blocks = DP / 64;
-        const int which = lane / boxes, kb = lane % boxes;  // K's column blocks, then V's
+        // a lane brings one box: of K, then of V
+        const int box = min(A.page_size, KEYS), boxes = KEYS / box, blocks = A.wide ? 1 : DP / 64;
+        const int which = lane / boxes, kb = lane % boxes;
         const bool mine = which < 2 * blocks;
-        const int col = which % blocks * 64;
+        const int col = which % blocks;
         const bool is_v = which >= blocks;
+        const CUtensorMap *map = is_v ? &tv : &tk;
+        const int at = (is_v ? C::HALF : 0) + kb * box * (DP * 2) + col * (box * 128);
         auto page_of = [&](int i) {
             const int64_t key = from + (int64_t) i * KEYS + kb * box;
             if (!mine || i >= steps || key >= to) return (int) A.pages;  // outside the tensor: zeros
@@ -264,9 +267,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             if (lane == 0) mbar_arrive_expect_tx(&full[st], C::STAGE);
             __syncwarp();
             if (mine) {
-                const int64_t key = from + (int64_t) i * KEYS + kb * box;
-                uint8_t *dst = ring + st * C::STAGE + (is_v ? C::HALF : 0) + col / 64 * (KEYS * 128) + kb * box * 128;
-                tma_load_4d(dst, is_v ? &tv : &tk, &full[st], col, (int) (key % A.page_size), kv_head, page);
+                const int token = (int) ((from + (int64_t) i * KEYS + kb * box) % A.page_size);
+                uint8_t *dst = ring + st * C::STAGE + at;
+                if (A.wide) tma_load_5d(dst, map, &full[st], 0, token, 0, kv_head, page);
+                else tma_load_4d(dst, map, &full[st], col * 64, token, kv_head, page);
             }
             page = next;
         }
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         for (int k = max(0, i - C::STAGES); k < i; k++)
             mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
         __syncthreads();
-        if (A.join) {
+        if (A.join > 1) {
             cluster_sync();
             cluster_sync();
         }
@@ -310,6 +314,12 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     for (int j = 0; j < DP / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = { -INFINITY, -INFINITY }, l[2] = { 0.0f, 0.0f };
     bool bad = false, timeout = false;
+    // where this lane's row of K's and of V's fragments lies in a stage, and how
+    // far on the next column block is
+    const int box = min(A.page_size, KEYS), block = box * 128;
+    const int k_key = warp * 16 + (lane >> 4) * 8 + (lane & 7), v_key = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+    const int k_at = k_key / box * (box * DP * 2) + k_key % box * 128;
+    const int v_at = C::HALF + v_key / box * (box * DP * 2) + v_key % box * 128;
 
     for (int i = 0; i < steps; i++) {
         const int st = i % C::STAGES;
@@ -324,18 +334,18 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             timeout = true;
             break;
         }
-        const uint32_t kb = smem_u32(ring + st * C::STAGE), vb = kb + C::HALF;
+        const uint32_t stage = smem_u32(ring + st * C::STAGE);
         const int k0 = warp * 16;  // this warp's keys of the stage
         const int64_t key0 = from + (int64_t) i * KEYS + k0;
         float sc[2][4] = {};
         {
-            const int key = k0 + (lane >> 4) * 8 + (lane & 7), odd = (lane >> 3) & 1;
-            const uint32_t row = kb + key * 128;
+            const int odd = (lane >> 3) & 1;
+            const uint32_t row = stage + k_at;
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ks++) {
                 uint32_t b[4];
                 const int unit = (ks * 2 + odd) & 7;
-                ldmatrix_x4(b, row + (ks / 4) * (KEYS * 128) + ((unit ^ (key & 7)) << 4));
+                ldmatrix_x4(b, row + (ks / 4) * block + ((unit ^ (lane & 7)) << 4));
                 mma16816<F16>(sc[0], qf[ks], b[0], b[1]);
                 mma16816<F16>(sc[1], qf[ks], b[2], b[3]);
             }
@@ -391,13 +401,13 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             }
         }
         {
-            const int key = k0 + ((lane >> 3) & 1) * 8 + (lane & 7), right = lane >> 4;
-            const uint32_t row = vb + key * 128;
+            const int right = lane >> 4;
+            const uint32_t row = stage + v_at;
 #pragma unroll
             for (int j = 0; j < DP / 8; j += 2) {
                 uint32_t b[4];
                 const int unit = (j + right) & 7;
-                ldmatrix_x4_t(b, row + (j / 8) * (KEYS * 128) + ((unit ^ (key & 7)) << 4));
+                ldmatrix_x4_t(b, row + (j / 8) * block + ((unit ^ (lane & 7)) << 4));
                 if (masked) {
                     // a key that not every row sees: its NaN and infinities apart (add_not_finite)
 #pragma unroll
@@ -469,7 +479,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             const int a = (int) max((int64_t) row_lo(A, s, t), from), z = (int) min((int64_t) row_hi(A, s, t), to);
             add_not_finite<F16>(A, seq, kv_head, c, a, z, sp.clo, max(sp.clo, sp.chi), x);
         }
-        if (A.join) {  // over the first warp's part, which this thread alone reads
+        if (A.join > 1) {  // over the first warp's part, which this thread alone reads
             float4 *dst = reinterpret_cast<float4 *>(os + row * LD + c);
             dst[0] = make_float4(x[0], x[1], x[2], x[3]);
             dst[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -485,7 +495,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             }
         }
     }
-    if (!A.join) {
+    if (A.join == 1) {
         if (live && A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
         return;
     }
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     if ((threadIdx.x & 7) == 0) ml_sh[row] = make_float2(stop ? NAN : mx, sum);
     cluster_sync();
     const int live_rows = (int) min((int64_t) ROWS, rows - r0);
-    for (int u = split * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.splits * 128) {
+    for (int u = rank * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.join * 128) {
         const int jr = u / (DP / 8), c = u % (DP / 8) * 8;
         if (c >= A.d) continue;
         float2 part[8];
@@ -502,7 +512,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         bool whole = true;
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (k < A.splits) {
+            if (k < A.join) {
                 asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
                              : "=f"(part[k].x), "=f"(part[k].y)
                              : "r"(map_to_rank(&ml_sh[jr], k))
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             }
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (k < A.splits) {
+            if (k < A.join) {
                 const float f = part[k].x == -INFINITY ? 0.0f : exp2_fast(part[k].x - top);
                 total += f * part[k].y;
                 float4 a, b;
@@ -529,12 +539,21 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(v[e], f, x[e]);
             }
+        const int64_t jrow = r0 + jr, jtok = s.q0 + jrow / A.group;
+        const int jhead = kv_head * A.group + (int) (jrow % A.group);
+        if (!whole) continue;
+        if (A.splits > 1) {
+            const int64_t jslot = split * (A.b.T * A.heads) + jtok * A.heads + jhead;
+            float4 *dst = reinterpret_cast<float4 *>(A.part + jslot * DP + c);
+            dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+            dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            if (c == 0) A.ml[jslot] = make_float2(top, total);
+            continue;
+        }
         const float scale = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= scale;
-        const int64_t jrow = r0 + jr;
-        if (whole)
-            store8<F16>(A, s.q0 + jrow / A.group, kv_head * A.group + (int) (jrow % A.group), c, x);
+        store8<F16>(A, jtok, jhead, c, x);
     }
     cluster_sync();  // nobody's shared memory goes while another reads it
 }
@@ -1079,31 +1098,33 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     }
 }
 
-// The chunks' parts of each row joined in order: the weights 2^(m_i - m) once
-// per row and thread, then eight columns a thread.
-template <int DP, bool F16>
+// The parts of each row joined in order, eight columns a thread. Few rows: the
+// block's groups of threads take every GROUPS-th part of one row and meet in
+// shared memory, so that 37 parts cost five loads one after another.
+template <int DP, bool F16, bool FEW>
 __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__ attend_args A, int tile_rows) {
-    constexpr int PER_ROW = DP / 8, ROWS_B = 128 / PER_ROW;
-    const int seq = blockIdx.z, kv_head = blockIdx.y;
+    constexpr int PER_ROW = DP / 8, GROUPS = 128 / PER_ROW;
+    const int seq = blockIdx.z, kv_head = blockIdx.y, group = threadIdx.x / PER_ROW;
     const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
     if (!s.ok) return;
     const int64_t rows = (int64_t) s.n * A.group;
-    const int64_t r = (int64_t) blockIdx.x * ROWS_B + threadIdx.x / PER_ROW;
+    const int64_t r = FEW ? blockIdx.x : (int64_t) blockIdx.x * GROUPS + group;
     const int c = threadIdx.x % PER_ROW * 8;
-    if (r >= rows || c >= A.d) return;
-    // the chunks of the row's tile, counted as its blocks counted them
-    const int64_t r0 = r / tile_rows * tile_rows;
-    const key_span sp =
-        span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + tile_rows, rows) - 1) / A.group));
-    const int64_t span = sp.hi - (int64_t) sp.lo / KEYS * KEYS;
-    const int n = span > 0 ? (int) ((span + A.chunk - 1) / A.chunk) : 1;
+    if (FEW ? r >= rows : r >= rows || c >= A.d) return;
+    int n = A.splits;
+    if (!FEW) {  // the chunks of the row's tile, counted as its blocks counted them
+        const int64_t r0 = r / tile_rows * tile_rows;
+        const key_span sp = span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + tile_rows, rows) - 1) / A.group));
+        const int64_t span = sp.hi - (int64_t) sp.lo / KEYS * KEYS;
+        n = span > 0 ? (int) ((span + A.chunk - 1) / A.chunk) : 1;
+    }
     const int t = (int) (r / A.group), head = kv_head * A.group + (int) (r % A.group);
     const int64_t tok = s.q0 + (int64_t) t, stride = A.b.T * A.heads, slot = tok * A.heads + head;
-    float mx = -INFINITY;
-    for (int i = 0; i < n; i++) mx = fmaxf(mx, A.ml[i * stride + slot].x);
-    float sum = 0.0f, x[8] = {};
+    float mx = -INFINITY, sum = 0.0f, x[8] = {};
+    const int first = FEW ? group : 0, step = FEW ? GROUPS : 1;
+    for (int i = first; i < n; i += step) mx = fmaxf(mx, A.ml[i * stride + slot].x);
 #pragma unroll 4
-    for (int i = 0; i < n; i++) {
+    for (int i = first; i < n; i += step) {
         const float2 ml = A.ml[i * stride + slot];
         const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mx);
         const float4 *p = reinterpret_cast<const float4 *>(A.part + (i * stride + slot) * DP + c);
@@ -1112,6 +1133,26 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
         const float v[8] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(v[e], w, x[e]);
+    }
+    if (FEW) {
+        __shared__ float sh[GROUPS][DP + 4];
+        __shared__ float2 ml_sh[GROUPS];
+        if (c == 0) ml_sh[group] = make_float2(mx, sum);
+#pragma unroll
+        for (int e = 0; e < 8; e++) sh[group][c + e] = x[e];
+        __syncthreads();
+        if (group > 0 || c >= A.d) return;
+        float top = -INFINITY;
+        for (int g = 0; g < GROUPS; g++) top = fmaxf(top, ml_sh[g].x);
+        sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        for (int g = 0; g < GROUPS; g++) {
+            const float w = ml_sh[g].x == -INFINITY ? 0.0f : exp2_fast(ml_sh[g].x - top);
+            sum += w * ml_sh[g].y;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(sh[g][c + e], w, x[e]);
+        }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -1133,19 +1174,30 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // One layer's pool as (value, token of a page, kv head, page), in boxes of 64
-// values by min(page, 64) tokens. Columns past d and pages past the pool read
-// zeros.
-bool pool_tmap(CUtensorMap *m, const zest_kv_cache *kv, const void *base) {
+// values by min(page, 64) tokens; wide: as (value of a block of 64, token,
+// block, kv head, page), in boxes of whole heads (whole blocks of 64 only: a
+// partial one would reach into the next head). Columns past d and pages past
+// the pool read zeros.
+bool pool_tmap(CUtensorMap *m, const zest_kv_cache *kv, const void *base, bool wide) {
     auto fn = encode_fn();
     if (!fn) return false;
     // a dimension of one entry is never stepped over: any valid stride does
     const int64_t hs = kv->kv_heads > 1 ? kv->head_stride : 8 * 32, ps = kv->pages > 1 ? kv->page_stride : 8 * 32;
-    cuuint64_t dims[4] = { (cuuint64_t) kv->d, (cuuint64_t) kv->page_size, (cuuint64_t) kv->kv_heads,
-                           (cuuint64_t) kv->pages };
-    cuuint64_t strides[3] = { (cuuint64_t) kv->token_stride * 2, (cuuint64_t) hs * 2, (cuuint64_t) ps * 2 };
-    cuuint32_t box[4] = { 64, (cuuint32_t) std::min(kv->page_size, KEYS), 1, 1 };
-    cuuint32_t estr[4] = { 1, 1, 1, 1 };
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, box, estr,
+    const cuuint64_t tokens = (cuuint64_t) kv->page_size, heads = (cuuint64_t) kv->kv_heads, pages = (cuuint64_t) kv->pages;
+    const cuuint32_t box_keys = (cuuint32_t) std::min(kv->page_size, KEYS), blocks = (cuuint32_t) kv->d / 64;
+    cuuint64_t dims[5] = { (cuuint64_t) kv->d, tokens, heads, pages, 1 };
+    cuuint64_t strides[4] = { (cuuint64_t) kv->token_stride * 2, (cuuint64_t) hs * 2, (cuuint64_t) ps * 2, 16 };
+    cuuint32_t box[5] = { 64, box_keys, 1, 1, 1 };
+    if (wide) {
+        const cuuint64_t wide_dims[5] = { 64, tokens, blocks, heads, pages };
+        const cuuint64_t wide_strides[4] = { (cuuint64_t) kv->token_stride * 2, 128, (cuuint64_t) hs * 2,
+                                             (cuuint64_t) ps * 2 };
+        std::copy(wide_dims, wide_dims + 5, dims);
+        std::copy(wide_strides, wide_strides + 4, strides);
+        box[2] = blocks;
+    }
+    cuuint32_t estr[5] = { 1, 1, 1, 1, 1 };
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, wide ? 5 : 4, const_cast<void *>(base), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1154,8 +1206,8 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a call runs: its row tiles, and the chunks its keys are cut into.
 struct attend_plan {
-    int dp, tile_rows, splits;
-    bool many, join;
+    int dp, tile_rows, splits, join;
+    bool many, wide;
     int64_t row_tiles, chunk, ws_ml, ws_part;
 };
 
@@ -1164,13 +1216,16 @@ struct attend_plan {
 // to the tensor-core tiles.
 // The keys are cut so that the blocks fill the GPU: one batch of resident
 // blocks where every sequence is as long as the next (one sequence), about
-// four where lengths differ, for balance; never below 128 keys a chunk (512
-// for many rows).
+// four where lengths differ, for balance; never below 128 keys a block (512
+// for many rows). Up to 8 blocks join as one cluster; more go through the
+// workspace (as clusters of 4 too, one token over 131,072 keys took 127 us
+// where it takes 100: clusters leave SMs of their GPC unused).
 attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
     attend_plan p;
     p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
     const int64_t group = at->heads / kv->kv_heads;
     p.many = b->max_q * group > ROWS;
+    p.wide = !p.many && kv->d % 64 == 0 && kv->d == p.dp;
     p.tile_rows = p.many ? (int) ((p.dp == 256 ? 1 : 2) * (128 / group) * group) : ROWS;
     p.row_tiles = std::max<int64_t>(1, up(b->max_q * group, p.tile_rows));
     const int64_t units = std::max<int64_t>(1, b->n_seqs * (int64_t) kv->kv_heads * p.row_tiles);
@@ -1179,12 +1234,20 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
     if (at->causal && at->window)  // which may start inside a block of keys
         span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
     const int64_t want = 148 * per_sm * (b->n_seqs > 1 ? 4 : 1);
-    const int64_t splits = std::max<int64_t>(1, want / units);
-    p.chunk = std::max<int64_t>(p.many ? 512 : 128, up(up(span, splits), 2 * KEYS) * 2 * KEYS);
-    p.splits = (int) std::max<int64_t>(1, up(span, p.chunk));
-    p.join = !p.many && p.splits > 1 && p.splits <= 8;
+    const int64_t most = std::max<int64_t>(1, want / units), least = p.many ? 512 : 128;
+    int64_t splits = std::max<int64_t>(1, std::min(most, up(span, least)));
+    p.chunk = 0;
+    p.join = 1;
+    if (p.many) {
+        p.chunk = std::max<int64_t>(1, up(up(span, splits), 2 * KEYS)) * 2 * KEYS;
+        splits = std::max<int64_t>(1, up(span, p.chunk));
+    } else if (splits <= 8) {
+        p.join = (int) splits;
+        splits = 1;
+    }
+    p.splits = (int) splits;
     p.ws_ml = p.ws_part = 0;
-    if (p.splits > 1 && !p.join) {
+    if (p.splits > 1) {
         p.ws_ml = up((int64_t) p.splits * b->T * at->heads * 8, 256) * 256;
         p.ws_part = (int64_t) p.splits * b->T * at->heads * p.dp * 4;
     }
@@ -1242,23 +1305,26 @@ int launch_attend(const zest_kv_cache *kv, const CUtensorMap &tk, const CUtensor
         using C = few_rows<DP>;
         if (!allow_smem(kv_attend_few_kernel<DP, F16>, C::SMEM, few_ready)) return check_launch(call);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(p.splits, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
+        cfg.gridDim = dim3(p.splits * p.join, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
         cfg.blockDim = dim3(FEW_THREADS);
         cfg.dynamicSmemBytes = C::SMEM;
         cfg.stream = st;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = p.join ? p.splits : 1;
+        attr.val.clusterDim.x = p.join;
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         cudaLaunchKernelEx(&cfg, kv_attend_few_kernel<DP, F16>, tk, tv, a);
     }
     if (check_launch(call)) return -1;
-    if (p.splits == 1 || p.join) return 0;
-    const int rows_b = 128 / (DP / 8);
-    const dim3 cg((unsigned) up(a.b.max_q * a.group, rows_b), kv->kv_heads, a.b.n_seqs);
-    kv_combine_kernel<DP, F16><<<cg, 128, 0, st>>>(a, p.tile_rows);
+    if (p.splits == 1) return 0;
+    const int64_t rows = a.b.max_q * a.group;
+    if (p.many)
+        kv_combine_kernel<DP, F16, false><<<dim3((unsigned) up(rows, 128 / (DP / 8)), kv->kv_heads, a.b.n_seqs), 128, 0, st>>>(
+            a, p.tile_rows);
+    else
+        kv_combine_kernel<DP, F16, true><<<dim3((unsigned) rows, kv->kv_heads, a.b.n_seqs), 128, 0, st>>>(a, p.tile_rows);
     return check_launch(call);
 }
 
@@ -1300,7 +1366,8 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     if (batch->T == 0 || batch->n_seqs == 0 || batch->max_q == 0) return 0;
     const int64_t off = kv->layers > 1 ? layer * kv->layer_stride : 0;
     CUtensorMap tk, tv;
-    if (!pool_tmap(&tk, kv, (const uint16_t *) kv->k + off) || !pool_tmap(&tv, kv, (const uint16_t *) kv->v + off))
+    if (!pool_tmap(&tk, kv, (const uint16_t *) kv->k + off, p.wide) ||
+        !pool_tmap(&tv, kv, (const uint16_t *) kv->v + off, p.wide))
         return kv_refuse(call, "the pools' strides make no tensor map");
     attend_args a;
     a.b = *batch;
@@ -1327,6 +1394,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.chunk = p.chunk;
     a.splits = p.splits;
     a.join = p.join;
+    a.wide = p.wide;
     a.ml = (float2 *) workspace;
     a.part = (float *) ((uint8_t *) workspace + p.ws_ml);
     a.err = err;

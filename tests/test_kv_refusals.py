@@ -100,6 +100,7 @@ def test_attend_workspace():
     size = lambda **kw: Z.lib().zest_kv_attend_workspace(ref(cache()), ref(batch(**kw)), ref(attn()))
     assert size(n=0, T=0, max_q=0, max_kv=0) == 0
     assert size(n=1, T=1, max_q=1, max_kv=200) == 0
+    assert size(n=1, T=1000, max_q=1000, max_kv=0) == 0
     # an m and an l and a head's values in f32 for each chunk of each row
     got = size(n=1, T=1, max_q=1, max_kv=131072)
     assert got > 0 and got <= 148 * 4 * 32 * (128 * 4 + 8) + 256
