@@ -1214,12 +1214,13 @@ struct attend_plan {
 // Up to 16 rows of a kv head go to the few-rows kernel: the cache's bytes
 // bound it, and its smaller blocks keep more of them in flight. More rows go
 // to the tensor-core tiles.
-// The keys are cut so that the blocks fill the GPU: one batch of resident
-// blocks where every sequence is as long as the next (one sequence), about
-// four where lengths differ, for balance; never below 128 keys a block (512
-// for many rows). Up to 8 blocks join as one cluster; more go through the
-// workspace (as clusters of 4 too, one token over 131,072 keys took 127 us
-// where it takes 100: clusters leave SMs of their GPC unused).
+// The keys are cut so that the blocks fill the GPU once; where sequences may
+// differ in length, up to four times for balance, in chunks of 1,024 keys or
+// more (32 tokens over up to 8,192: 132 us filling it twice, 119 four times, 128
+// eight times). Never below 128 keys a block (512 for many rows). Up to 8 blocks
+// that have an SM each join as one cluster, without a second launch; more go
+// through the workspace (as clusters of 4 the 32 tokens took 128 us, and one
+// token over 131,072 keys 127 for 91: clusters wait for a GPC's SMs together).
 attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
     attend_plan p;
     p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
@@ -1233,15 +1234,16 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
     int64_t span = b->max_kv;
     if (at->causal && at->window)  // which may start inside a block of keys
         span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
-    const int64_t want = 148 * per_sm * (b->n_seqs > 1 ? 4 : 1);
-    const int64_t most = std::max<int64_t>(1, want / units), least = p.many ? 512 : 128;
-    int64_t splits = std::max<int64_t>(1, std::min(most, up(span, least)));
+    const int64_t once = std::max<int64_t>(1, 148 * per_sm / units), least = p.many ? 512 : 128;
+    int64_t splits = once;
+    if (b->n_seqs > 1) splits = std::max(once, std::min(148 * per_sm * 4 / units, up(span, 1024)));
+    splits = std::max<int64_t>(1, std::min(splits, up(span, least)));
     p.chunk = 0;
     p.join = 1;
     if (p.many) {
         p.chunk = std::max<int64_t>(1, up(up(span, splits), 2 * KEYS)) * 2 * KEYS;
         splits = std::max<int64_t>(1, up(span, p.chunk));
-    } else if (splits <= 8) {
+    } else if (splits <= 8 && splits * units <= 148) {
         p.join = (int) splits;
         splits = 1;
     }
