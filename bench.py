@@ -825,9 +825,10 @@ class Prefill:
     """A Qwen3-shaped model's prompt prefill in chunks. The chunks the gate
     claims (>= min_batch tokens) run every claimed op through the C ABI:
     RMS_NORM and its MUL, the q/k/v group, the per-head q/k norms, ROPE
-    (NeoX), o, the residual ADDs, the fused gate/up SwiGLU and down.
-    Attention, the embedding lookup, the LM head (last token) and chunks
-    below the floor run as torch ops, as the sibling backend would."""
+    (NeoX), o, the residual ADDs, the fused gate/up SwiGLU and down; and
+    beside them the paged cache's write and its attention. The embedding
+    lookup, the LM head (last token) and chunks below the floor run as torch
+    ops, as the sibling backend would."""
 
     def __init__(self, c: dict, seed: int = 0, threads: int = 1):
         import torch
@@ -876,12 +877,17 @@ class Prefill:
         self.q16 = torch.empty((Tm, hq * hd), dtype=torch.bfloat16, device="cuda")
         self.fused = True
         self.a_h = {K: torch.empty((mp, K), dtype=torch.int16, device="cuda") for K in (H, hq * hd, F)}
-        self.page = 64
-        Pp = Z.pad_to(P, self.page)  # the cache in 64-token pages for the paged attention kernel
+        # the cache in 64-token pages, one after another: a single sequence's table
+        page = 64
+        Pp = Z.pad_to(P, page)
         self.kc = torch.zeros((nL, Pp, hk, hd), dtype=torch.bfloat16, device="cuda")
         self.vc = torch.zeros((nL, Pp, hk, hd), dtype=torch.bfloat16, device="cuda")
-        self.att16 = torch.empty((Tm, hq, hd), dtype=torch.bfloat16, device="cuda")
-        self.attn_impl = self._pick_attention()
+        pages = (nL, Pp // page, page, hk, hd)
+        self.kv = Z.KvCache(self.kc.view(pages), self.vc.view(pages))
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+        blocks = torch.arange(Pp // page, dtype=torch.int32, device="cuda")[None]
+        self.batches = {p0: Z.KvBatch(i32([0, T]), i32([p0 + T]), blocks, T=T, max_q=T, max_kv=p0 + T)
+                        for p0, T in self.chunks}
         self.table = f32(Tm, hd)
         self.pos = torch.arange(P, dtype=torch.int32, device="cuda")
         self.par = (ctypes.c_float * 6)(c["rope_base"], 1.0, 0.0, 1.0, 32.0, 1.0)
@@ -922,57 +928,14 @@ class Prefill:
                                       self._sp()))
         self._ok(self.L.zest_mul_row(self._p(dst), self._p(wt), rows, d, self._p(dst), self._sp()))
 
-    def _pick_attention(self) -> str:
-        """Attention outside the path: flashinfer's trtllm-gen paged context
-        kernel for chunks that attend over earlier ones (2-3x torch SDPA
-        there on B200), torch SDPA for a chunk on its own. Checked once
-        against SDPA; SDPA everywhere if the library is missing or differs."""
-        torch = self.torch
-        try:
-            from flashinfer.prefill import trtllm_batch_context_with_kv_cache
-            nL, H, hq, hk, hd, F = self.dims
-            Pp = self.kc.shape[1]
-            self._trt = trtllm_batch_context_with_kv_cache
-            self._ws = torch.zeros(128 << 20, dtype=torch.uint8, device="cuda")
-            self._blocks = torch.arange(Pp // self.page, dtype=torch.int32, device="cuda")[None]
-            self._meta = {}
-            for p0, T in self.chunks:
-                S = p0 + T
-                self._meta[p0] = (torch.tensor([S], dtype=torch.int32, device="cuda"),
-                                  torch.tensor([0, T], dtype=torch.int32, device="cuda"),
-                                  torch.tensor([0, S], dtype=torch.int32, device="cuda"))
-            # check on the second chunk's shape with random keys
-            p0, T = self.chunks[1] if len(self.chunks) > 1 else self.chunks[0]
-            g = torch.Generator("cuda").manual_seed(7)
-            self.kc[0, :p0 + T] = torch.randn(p0 + T, hk, hd, device="cuda", generator=g).to(torch.bfloat16)
-            self.vc[0, :p0 + T] = torch.randn(p0 + T, hk, hd, device="cuda", generator=g).to(torch.bfloat16)
-            q = torch.randn(T, hq, hd, device="cuda", generator=g).to(torch.bfloat16)
-            got = self._attend_paged(0, p0, T, q).float()
-            want = self._attend(q, self.kc[0, :p0 + T], self.vc[0, :p0 + T]).float()
-            torch.cuda.synchronize()
-            if ((got - want).abs().max() / want.abs().max()).item() > 2e-2:
-                return "torch SDPA (trtllm-gen disagreed)"
-            return "flashinfer trtllm-gen paged context attention; torch SDPA for the first chunk"
-        except Exception as e:  # the library is optional: SDPA is the stock path
-            self._trt = None
-            return f"torch SDPA ({type(e).__name__} from flashinfer)"
+    def _append(self, li, p0, T, q, k, v, **norm_rope):
+        """A chunk's keys and values into layer li's pages, its queries to q16."""
+        self.Z.kv_append(self.kv, li, self.batches[p0], k[:T], v[:T], q=q[:T], q_out=self.q16[:T], err=self.err,
+                         **norm_rope)
 
-    def _attend_paged(self, li, p0, T, q):
-        """A chunk's queries q [T, hq, hd] over layer li's cache up to the chunk's end."""
-        nL, H, hq, hk, hd, F = self.dims
-        Pp, ps = self.kc.shape[1], self.page
-        seq, cq, ckv = self._meta[p0]
-        out = self.att16[:T]
-        self._trt(q, (self.kc[li].view(Pp // ps, ps, hk, hd), self.vc[li].view(Pp // ps, ps, hk, hd)), self._ws,
-                  self._blocks, seq, T, p0 + T, 1.0 / math.sqrt(hd), 1.0, 1, cq, ckv, out=out, kv_layout="NHD",
-                  causal=True)
-        return out
-
-    def _attention(self, li, p0, T, q):
-        """Layer li's attention for a chunk (queries q [T, hq, hd] bf16)."""
-        if self._trt is not None and p0 > 0:
-            return self._attend_paged(li, p0, T, q)
-        return self._attend(q, self.kc[li, :p0 + T], self.vc[li, :p0 + T])
+    def _attention(self, li, p0, T, **out):
+        """Layer li's attention for a chunk (queries in q16) over the cache up to the chunk's end."""
+        self.Z.kv_attend(self.kv, li, self.batches[p0], self.q16[:T], err=self.err, **out)
 
     def _attend(self, q, k, v):
         """Causal attention of a chunk's queries over the cache up to the
@@ -1040,12 +1003,12 @@ class Prefill:
             ev[1].record()
 
     def claimed_chunk(self, p0, T, evs=None, att_ev=None):
-        """Every op of a claimed chunk through the C ABI (attention aside);
-        the chunk's hidden state ends in self.x[:T]. With self.fused the
-        block executor's ops ride in the kernels beside them (the norm in
-        the pack, q/k norm with rope, the residual ADDs in the GEMM epilogue,
-        SwiGLU writing the down projection's operand): 8 launches of ours a
-        layer instead of 20."""
+        """Every op of a claimed chunk through the C ABI; the chunk's hidden
+        state ends in self.x[:T]. With self.fused the block executor's ops
+        ride in the kernels beside them (the norm in the pack, q/k norm and
+        rope in the cache's write, the residual ADDs in the GEMM epilogue,
+        SwiGLU and the attention writing the next projection's operand): 8
+        launches of ours a layer instead of 22."""
         if self.fused:
             return self._claimed_chunk_fused(p0, T, evs, att_ev)
         torch, Z, L, p, sp = self.torch, self.Z, self.L, self._p, self._sp()
@@ -1063,12 +1026,10 @@ class Prefill:
             self._norm(k, T * hk, hd, d["k_norm"], self.kn)
             self._ok(L.zest_rope(p(self.qn), T, hq, hd, hd, Z.ROPE_NEOX, p(self.table), p(self.qr), sp))
             self._ok(L.zest_rope(p(self.kn), T, hk, hd, hd, Z.ROPE_NEOX, p(self.table), p(self.kr), sp))
-            self.kc[li, p0:p0 + T] = self.kr[:T].view(T, hk, hd)
-            self.vc[li, p0:p0 + T] = v[:T].view(T, hk, hd)
+            self._append(li, p0, T, self.qr, self.kr, v)
             if att_ev is not None:
                 att_ev[li][0].record()
-            self.att[:T] = self._attend(self.qr[:T].view(T, hq, hd).to(torch.bfloat16), self.kc[li, :p0 + T],
-                                        self.vc[li, :p0 + T]).reshape(T, hq * hd)
+            self._attention(li, p0, T, y=self.att[:T])
             if att_ev is not None:
                 att_ev[li][1].record()
             self._pack(self.att, T, hq * hd)
@@ -1082,7 +1043,7 @@ class Prefill:
             self._ok(L.zest_add(p(x), p(self.d_out), 0, T, H, p(x), sp))
         return x[:T]
 
-    LAUNCHES_PER_LAYER = 20  # our kernels per layer of a claimed chunk, unfused
+    LAUNCHES_PER_LAYER = 22  # our kernels per layer of a claimed chunk, unfused
     LAUNCHES_PER_LAYER_FUSED = 8
 
     def _claimed_chunk_fused(self, p0, T, evs, att_ev):
@@ -1097,18 +1058,13 @@ class Prefill:
             self._ok(L.zest_pack_rms_norm(p(x), T, H, H, eps, p(d["attn_norm"]), None, 0, mp, p(self.a_h[H]), H, sp))
             self._segs(H, T, [(d["q"], hq * hd, B, self.q, None, None), (d["k"], hk * hd, B, self.k, None, None),
                               (d["v"], hk * hd, B, self.v, None, None)], ev[0])
-            kc = self.kc[li, p0:p0 + T]
-            self._ok(L.zest_norm_rope(p(self.q), T, hq, hd, eps, p(d["q_norm"]), hd, Z.ROPE_NEOX, p(self.table),
-                                      None, p(self.q16), sp))
-            self._ok(L.zest_norm_rope(p(self.k), T, hk, hd, eps, p(d["k_norm"]), hd, Z.ROPE_NEOX, p(self.table),
-                                      None, p(kc), sp))
-            self.vc[li, p0:p0 + T] = self.v[:T].view(T, hk, hd)
+            self._append(li, p0, T, self.q, self.k, self.v, k_norm=d["k_norm"], q_norm=d["q_norm"], eps=self.c["eps"],
+                         rope=self.table)
             if att_ev is not None:
                 att_ev[li][0].record()
-            self.att[:T] = self._attention(li, p0, T, self.q16[:T].view(T, hq, hd)).reshape(T, hq * hd)
+            self._attention(li, p0, T, a_next=self.a_h[hq * hd][:T])  # the o matmul's operand
             if att_ev is not None:
                 att_ev[li][1].record()
-            self._pack(self.att, T, hq * hd)
             self._segs(hq * hd, T, [(d["o"], H, B, x, x, None)], ev[1])
             self._ok(L.zest_pack_rms_norm(p(x), T, H, H, eps, p(d["ffn_norm"]), None, 0, mp, p(self.a_h[H]), H, sp))
             self._segs(H, T, [(d["gate_up"], d["gate_up"].shape[0], Z.MODE_SWIGLU, None, None, self.a_h[F])], ev[2])
@@ -1288,10 +1244,10 @@ def run_model(args, w: dict) -> None:
                        "weights": f"Q4_K; Q6_K for attn_v and ffn_down on {n_six} of {nL} layers (first and last "
                                   "eighth, every third between). One seeded set of raw bytes per type, converted "
                                   "into every layer's own device copy",
-                       "attention": m.attn_impl + " (outside the path)",
+                       "attention": "zest_kv_attend over 64-token pages; torch SDPA in the unclaimed tail",
                        "graphs": "each claimed chunk, and the tail with the LM head, replayed from CUDA graphs",
-                       "fused": "norm in the pack, q/k norm with rope, residual ADDs and SwiGLU's packed output in "
-                                "the GEMM epilogues" if m.fused else "every op its own kernel",
+                       "fused": "norm in the pack, q/k norm and rope in the cache's write, residual ADDs and SwiGLU's "
+                                "packed output in the GEMM epilogues, the attention's result packed" if m.fused else "every op its own kernel",
                        "unclaimed": f"the {m.chunks[-1][1]}-token tail (< {c['min_batch']} tokens) in torch ops",
                        "parallelism": f"tokens{world} (each GPU its own prompt, no collective)" if world > 1
                        else "1 GPU",

@@ -158,7 +158,7 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
 // loads run beside. Bound by the f32 rows' bytes in and the 16-bit ones out
 // for a chunk, by those loads' latency for a few tokens.
 template <int NC, bool F16>
-__global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const __grid_constant__ append_args A) {
+__global__ void __launch_bounds__(AP_WARPS * 32, NC == 1 ? 4 : 2) kv_append_kernel(const __grid_constant__ append_args A) {
     constexpr int N = AP_ROWS<NC>;
     __shared__ float4 buf[AP_WARPS][NC * 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = A.d;
