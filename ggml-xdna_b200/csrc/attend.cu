@@ -27,6 +27,7 @@ namespace {
 constexpr uint64_t WAIT_LIMIT_NS = 1000000000ull;  // 1 s
 constexpr int ROWS = 16;                           // query rows of a tile of the few-rows kernel
 constexpr int KEYS = 64;                           // keys of a stage
+constexpr float LOG2E = 1.44269504088896340736f;
 
 struct attend_args {
     zest_kv_batch b;
@@ -243,7 +244,8 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         const int at = (is_v ? C::HALF : 0) + kb * box * (DP * 2) + col * (box * 128);
         auto page_of = [&](int i) {
             const int64_t key = from + (int64_t) i * KEYS + kb * box;
-            if (!mine || i >= steps || key >= to) return (int) A.pages;  // outside the tensor: zeros
+            // a page that no row sees is outside the tensor: zeros (its entry may be none)
+            if (!mine || i >= steps || key >= to || (key / A.page_size + 1) * A.page_size <= sp.lo) return (int) A.pages;
             const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
             if (p < 0 || p >= A.pages) {
                 atomicOr(A.err, ZEST_ERR_BAD_PAGE);
@@ -781,7 +783,9 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const bool has = col < DP;
         auto page_of = [&](int i) {  // of this lane's box of tile i (K or V)
             const int key = from + i * BN + kb * box;
-            if (!has || i < 0 || i >= n || key >= to) return (int) A.pages;  // outside the tensor: zeros
+            // a page that no row sees is outside the tensor: zeros (its entry may be none)
+            if (!has || i < 0 || i >= n || key >= to || (key / A.page_size + 1) * A.page_size <= sp.lo)
+                return (int) A.pages;
             const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
             if (p < 0 || p >= A.pages) {
                 atomicOr(A.err, ZEST_ERR_BAD_PAGE);
@@ -1204,6 +1208,14 @@ bool pool_tmap(CUtensorMap *m, const zest_kv_cache *kv, const void *base, bool w
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The batch with bounds no looser than its arrays allow: they shape the launch.
+zest_kv_batch tightened(const zest_kv_cache *kv, const zest_kv_batch *b) {
+    zest_kv_batch t = *b;
+    t.max_q = std::min(t.max_q, t.T);
+    t.max_kv = std::min(t.max_kv, t.table_stride * kv->page_size);
+    return t;
+}
+
 // How a call runs: its row tiles, and the chunks its keys are cut into.
 struct attend_plan {
     int dp, tile_rows, splits, join;
@@ -1233,7 +1245,7 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
     const int64_t per_sm = p.many ? 1 : p.dp == 64 ? 3 : p.dp == 128 ? 2 : 1;
     int64_t span = b->max_kv;
     if (at->causal && at->window)  // which may start inside a block of keys
-        span = std::min(span, at->window + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
+        span = std::min(span, std::min(at->window, span) + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
     const int64_t once = std::max<int64_t>(1, 148 * per_sm / units), least = p.many ? 512 : 128;
     int64_t splits = once;
     if (b->n_seqs > 1) splits = std::max(once, std::min(148 * per_sm * 4 / units, up(span, 1024)));
@@ -1260,9 +1272,11 @@ const char *attend_fault(const zest_kv_cache *kv, const zest_kv_batch *b, const 
     if (!at) return "nothing to attend with";
     if (at->heads < 1 || at->heads % kv->kv_heads || at->heads / kv->kv_heads > 128)
         return "heads are a multiple of the kv heads, at most 128 times";
-    if (!(at->scale > 0.0f) || std::isinf(at->scale)) return "scale is not positive";
+    if (!(at->scale > 0.0f) || std::isinf(at->scale * LOG2E)) return "scale is not positive and finite";
     if (at->window < 0 || (at->window > 0 && !at->causal)) return "a window is positive and causal";
-    if (plan_attend(kv, b, at).splits * (int64_t) kv->kv_heads > 65535) return "too many heads for the keys";
+    const attend_plan p = plan_attend(kv, b, at);
+    if (p.splits * (int64_t) kv->kv_heads > 65535 || b->max_q * (at->heads / kv->kv_heads) > 0x7fffffff)
+        return "too many rows, or too many heads for the keys";
     return nullptr;
 }
 
@@ -1342,8 +1356,9 @@ int64_t zest_kv_attend_workspace(const zest_kv_cache *kv, const zest_kv_batch *b
     const char *call = "zest_kv_attend_workspace";
     if (const char *why = kv_cache_fault(kv, 0)) return kv_refuse(call, why);
     if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
-    if (const char *why = attend_fault(kv, batch, at)) return kv_refuse(call, why);
-    const attend_plan p = plan_attend(kv, batch, at);
+    const zest_kv_batch b = tightened(kv, batch);
+    if (const char *why = attend_fault(kv, &b, at)) return kv_refuse(call, why);
+    const attend_plan p = plan_attend(kv, &b, at);
     return p.ws_ml + p.ws_part;
 }
 
@@ -1352,7 +1367,8 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     const char *call = "zest_kv_attend";
     if (const char *why = kv_cache_fault(kv, layer)) return kv_refuse(call, why);
     if (const char *why = kv_batch_fault(batch)) return kv_refuse(call, why);
-    if (const char *why = attend_fault(kv, batch, at)) return kv_refuse(call, why);
+    const zest_kv_batch b = tightened(kv, batch);
+    if (const char *why = attend_fault(kv, &b, at)) return kv_refuse(call, why);
     if (!err) return kv_refuse(call, "no device error word");
     const int64_t wide = (int64_t) at->heads * kv->d;
     auto rows = [&](const void *p, int64_t ld, int64_t unit) { return ld >= wide && ld % unit == 0 && !((uintptr_t) p & 15); };
@@ -1361,18 +1377,18 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     if ((at->out && !rows(at->out, at->ldo, 8)) || (at->y && !rows(at->y, at->ldy, 4)) ||
         (at->a_next && !rows(at->a_next, at->lda, 8)))
         return kv_refuse(call, "output rows cover the heads and are 16-byte aligned");
-    const attend_plan p = plan_attend(kv, batch, at);
+    const attend_plan p = plan_attend(kv, &b, at);
     const int64_t need = p.ws_ml + p.ws_part;
     if (need > 0 && (!workspace || ((uintptr_t) workspace & 15) || (int64_t) workspace_bytes < need))
         return kv_refuse(call, "the workspace is smaller than zest_kv_attend_workspace says, or not 16-byte aligned");
-    if (batch->T == 0 || batch->n_seqs == 0 || batch->max_q == 0) return 0;
+    if (b.T == 0 || b.n_seqs == 0 || b.max_q == 0) return 0;
     const int64_t off = kv->layers > 1 ? layer * kv->layer_stride : 0;
     CUtensorMap tk, tv;
     if (!pool_tmap(&tk, kv, (const uint16_t *) kv->k + off, p.wide) ||
         !pool_tmap(&tv, kv, (const uint16_t *) kv->v + off, p.wide))
         return kv_refuse(call, "the pools' strides make no tensor map");
     attend_args a;
-    a.b = *batch;
+    a.b = b;
     a.q = (const uint16_t *) at->q;
     a.ldq = at->ldq;
     a.pages = kv->pages;
@@ -1386,7 +1402,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.page_size = kv->page_size;
     a.causal = at->causal != 0;
     a.window = at->window;
-    a.scale_log2 = at->scale * 1.44269504088896340736f;
+    a.scale_log2 = at->scale * LOG2E;
     a.out = (uint16_t *) at->out;
     a.ldo = at->ldo;
     a.y = at->y;

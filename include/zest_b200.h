@@ -354,9 +354,11 @@ int zest_kv_append(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
  * that the row sees in kv head h / (heads / kv_heads): j < kv_len; if causal,
  * j <= pos, the row's own position kv_len - (new tokens) + (its index among
  * them); if window > 0 (causal only), j > pos - window. A row that sees
- * nothing is zero. What a row does not see does not reach it, NaN or infinite
- * values among it. Not causal: the attention to states of another length.
- * Sums in f32; p is rounded to the cache's type before it meets v. */
+ * nothing (or only scores of minus infinity) is zero. What a row does not see
+ * does not reach it, NaN or infinite values among it; pages that no row sees
+ * (behind a window) are not read, whatever their table entry. Not causal: the
+ * attention to states of another length. Sums in f32; p is rounded to the
+ * cache's type before it meets v. Outputs do not overlap q. */
 typedef struct {
     const void *q;              /* [T][ldq], heads heads of d, the cache's type; 16-byte aligned rows */
     int64_t ldq;                /* a multiple of 8 */
@@ -376,7 +378,9 @@ typedef struct {
 /* The attention of a step's rows over one layer of the cache (append the
  * step's tokens first). workspace: zest_kv_attend_workspace bytes of device
  * memory, 16-byte aligned, its contents free before and after; calls that may
- * overlap take one each. */
+ * overlap take one each. The most new tokens of a sequence (max_q) choose the
+ * kernel: a step of prompts' chunks and single tokens over long caches is two
+ * calls, each with the rows of its kind. */
 int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *batch, const zest_kv_attn *at,
                    void *workspace, size_t workspace_bytes, unsigned *err, void *stream);
 /* Bytes of workspace such a call needs (0: none); -1 for a call that

@@ -13,6 +13,8 @@ sum p |v| / sum p. f16 weights below 2^-14 are held to 2^-25 absolutely,
 relative to a largest weight of 2^-8 to 1."""
 import math
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -178,6 +180,54 @@ def test_values_a_row_does_not_see_do_not_reach_it(d, lens, window, bad):
     rest = torch.ones(n, 8, dtype=torch.bool, device="cuda")
     rest[n - 1, 4:] = False
     assert torch.isfinite(got[rest]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 96, 256])
+@pytest.mark.parametrize("n,window", [(1, 50), (3, 77), (40, 30), (150, 100)])
+def test_pages_behind_the_window_may_be_gone(n, window, d):
+    """Pages that no row of the step sees any more: their entries none, or out of the pool."""
+    c = Case([(n, 700), (n, 333)], 8, 2, d, 16, BF, seed=21)
+    want = c.want(True, window)
+    for s, (new, kv) in enumerate(c.lens):
+        gone = max(0, kv - new - window + 1) // 16
+        c.table[s, :gone] = torch.tensor([-1, 1 << 30], dtype=torch.int32, device="cuda").repeat(gone)[:gone]
+    c.want = lambda *a: want
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, window=window), True, window)
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, window=window, workspace=torch.empty(1 << 24, dtype=torch.uint8,
+                                                                                    device="cuda")), True, window)
+
+
+def test_bounds_as_wide_as_they_go():
+    """max_q and max_kv of 2^31 - 1 - 4096 cost nothing: no sequence has more than the step's rows or its table row."""
+    for lens in ([(1, 900), (2, 40)], [(50, 300)]):
+        c = Case(lens, 8, 2, 128, 16, BF, seed=22)
+        wide = 0x7fffffff - 4096
+        b = Z.KvBatch(c.q_start, c.kv_len, c.table, T=c.T, max_q=wide, max_kv=wide)
+        c.check(Z.kv_attend(c.cache, 0, b, c.q))
+        c.check(Z.kv_attend(c.cache, 0, b, c.q, window=(1 << 62)))
+
+
+def test_a_first_call_that_is_captured():
+    """A process whose first calls are captured: nothing is set up that a capture forbids."""
+    code = """
+import sys, torch
+sys.path[:0] = ["ggml-xdna_b200", "tests"]
+import zest_b200 as Z
+from test_gpu_kv_attend import BF, Case
+for lens in ([(1, 200)], [(1, 4000)], [(100, 300)]):
+    c = Case(lens, 8, 2, 128, 16, BF, seed=1)
+    out, err = torch.zeros_like(c.q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        Z.kv_attend(c.cache, 0, c.batch, c.q, out=out, err=err, workspace=ws)
+    g.replay()
+    torch.cuda.synchronize()
+    assert int(err) == 0
+    c.check(out)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Z.PKG_DIR.parent, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_masked_lowest_and_infinite_scores():

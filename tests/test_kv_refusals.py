@@ -81,7 +81,7 @@ def test_caches_and_batches(call):
 def test_attend():
     for kw, words in [(dict(heads=12), "multiple of the kv heads"), (dict(heads=0), "multiple of the kv heads"),
                       (dict(heads=8 * 129, ldq=1 << 20, ldo=1 << 20), "128 times"), (dict(scale=0.0), "scale"),
-                      (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                      (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=3e38), "scale"),
                       (dict(window=-1), "window"), (dict(window=5, causal=0), "window"), (dict(q=0), "q rows"),
                       (dict(q=ODD), "q rows"), (dict(ldq=4095), "q rows"), (dict(ldq=4100), "q rows"),
                       (dict(out=0), "no output"), (dict(ldo=4000), "output rows"), (dict(out=ODD), "output rows"),
@@ -102,7 +102,7 @@ def test_attend_workspace():
     assert size(n=1, T=1, max_q=1, max_kv=200) == 0
     assert size(n=1, T=1000, max_q=1000, max_kv=0) == 0
     # an m and an l and a head's values in f32 for each chunk of each row
-    got = size(n=1, T=1, max_q=1, max_kv=131072)
+    got = size(n=1, T=1, max_q=1, max_kv=131072, stride=2048)
     assert got > 0 and got <= 148 * 4 * 32 * (128 * 4 + 8) + 256
     refused(Z.lib().zest_kv_attend_workspace(ref(cache()), ref(batch()), ref(attn(scale=-1.0))), "scale")
     refused(Z.lib().zest_kv_attend_workspace(None, ref(batch()), ref(attn())), "no cache")
