@@ -46,7 +46,7 @@ struct attend_args {
     int64_t lda;
     int64_t chunk;      // many rows: keys a block takes, a multiple of 128
     int splits;         // parts of a row that go to the workspace (1: none does, the result is whole)
-    int join;           // few rows: blocks of a cluster; each sequence's keys in splits * join equal chunks
+    int join;           // few rows: blocks of a cluster, each with an equal part of the keys (then splits is 1)
     int wide;           // few rows: a box has a head's columns whole
     float2 *ml;         // [splits][T * heads]: m and l
     float *part;        // [splits][T * heads][DP]: o
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     __shared__ int stop, not_finite;
     __shared__ float m_sh[4][ROWS], l_sh[4][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int seq = blockIdx.z, split = blockIdx.x / A.join, rank = blockIdx.x % A.join;
+    const int seq = blockIdx.z, split = blockIdx.x;  // the part of the keys (in a cluster, the block's rank)
     const int row_tiles = gridDim.y / (A.heads / A.group);
     const int kv_head = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
 
@@ -281,7 +281,9 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
         __syncthreads();
         if (A.join > 1) {
+            __syncwarp();
             cluster_sync();
+            __syncwarp();
             cluster_sync();
         }
         return;
@@ -504,9 +506,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     // the cluster's chunks joined in order, the rows' columns dealt to its blocks
     __shared__ float2 ml_sh[ROWS];
     if ((threadIdx.x & 7) == 0) ml_sh[row] = make_float2(stop ? NAN : mx, sum);
+    __syncwarp();
     cluster_sync();
     const int live_rows = (int) min((int64_t) ROWS, rows - r0);
-    for (int u = rank * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.join * 128) {
+    for (int u = split * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.join * 128) {
         const int jr = u / (DP / 8), c = u % (DP / 8) * 8;
         if (c >= A.d) continue;
         float2 part[8];
@@ -544,19 +547,12 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         const int64_t jrow = r0 + jr, jtok = s.q0 + jrow / A.group;
         const int jhead = kv_head * A.group + (int) (jrow % A.group);
         if (!whole) continue;
-        if (A.splits > 1) {
-            const int64_t jslot = split * (A.b.T * A.heads) + jtok * A.heads + jhead;
-            float4 *dst = reinterpret_cast<float4 *>(A.part + jslot * DP + c);
-            dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-            dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-            if (c == 0) A.ml[jslot] = make_float2(top, total);
-            continue;
-        }
         const float scale = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= scale;
         store8<F16>(A, jtok, jhead, c, x);
     }
+    __syncwarp();
     cluster_sync();  // nobody's shared memory goes while another reads it
 }
 
@@ -568,7 +564,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 // while these take their exponentials, and the tensor cores and the
 // exponential units both work throughout. (A buffer of each tile's own, with P
 // over it as the first form had it, holds the next scores back until P has
-// been used: 229 us where this takes XXX for 2,048 tokens over 8,192.)
+// been used: 229 us where this takes 199 for 2,048 tokens over 8,192.)
 template <int DP>
 struct many_rows {
     static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
@@ -577,8 +573,8 @@ struct many_rows {
     static constexpr int PARTS = BN / PART;
     static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int SLOTS = DP == 64 ? 8 : 5;  // tiles of K or V in flight or in use
-    static constexpr int SMEM = 1024 + NQ * Q_BYTES + SLOTS * KV_BYTES;
+    static constexpr int KS = DP == 64 ? 4 : 3, VS = DP == 64 ? 4 : 2;  // tiles of K and of V in flight or in use
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + (KS + VS) * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
     static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V and the copies, one idle
     // Buffers of P: two where one query tile has the block to itself, since the
@@ -587,6 +583,8 @@ struct many_rows {
     // TMEM columns: O of each query tile, the scores, P of each query tile
     static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
     static_assert(P_COL + NQ * NP * BN / 2 <= COLS, "TMEM holds O, S and P");
+    // a softmax warp looks at V(i) having seen the product of tile i - NP done
+    static_assert(VS >= NP, "V(i - VS) has been used when a softmax warp waits for V(i)");
 };
 
 // A rise of the running maximum below this (in powers of two) leaves the
@@ -702,11 +700,14 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     kv_attend_many_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                           const __grid_constant__ CUtensorMap tv, const __grid_constant__ attend_args A) {
     using C = many_rows<DP>;
-    constexpr int NQ = C::NQ, NP = C::NP, BN = C::BN, SLOTS = C::SLOTS, PARTS = C::PARTS;
+    constexpr int NQ = C::NQ, NP = C::NP, BN = C::BN, KS = C::KS, VS = C::VS, PARTS = C::PARTS;
     extern __shared__ uint8_t dyn[];
     uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
-    uint8_t *ring = q_sm + NQ * C::Q_BYTES;  // of tiles of K and V
-    __shared__ uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[NQ], s_free, p_full[NQ][PARTS], pv_done[NQ][NP], drained[2];
+    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + KS * C::KV_BYTES;
+    // Every barrier's phases are waited for one after another by whoever waits
+    // for it: a parity tells a phase from the one before it, not from the next.
+    __shared__ uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[NQ], s_free, p_full[NQ][NP][PARTS],
+        pv_done[NQ][NP], drained[2];
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -731,14 +732,20 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     constexpr int W_QK = C::SOFTMAX / 32, W_PV = W_QK + 1, W_COPY = W_QK + 2;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        for (int i = 0; i < SLOTS; i++) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+        for (int i = 0; i < KS; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < VS; i++) {
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < NQ; i++) {
             mbar_init(&s_full[i], 1);
-            for (int h = 0; h < PARTS; h++) mbar_init(&p_full[i][h], 4);
-            for (int b = 0; b < NP; b++) mbar_init(&pv_done[i][b], 1);
+            for (int b = 0; b < NP; b++) {
+                for (int h = 0; h < PARTS; h++) mbar_init(&p_full[i][b][h], 4);
+                mbar_init(&pv_done[i][b], 1);
+            }
         }
         mbar_init(&s_free, 4);
         mbar_init(&drained[0], 1);
@@ -759,14 +766,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 
     // A row of scores lives in registers: the softmax warps take the others'
     // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
-    auto fewer = [] {
-        if (NQ > 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    };
-    // The tiles' order in the ring: K(0) K(1) V(0) K(2) V(1) ... K(n - 1) V(n - 2) V(n - 1).
-    auto slot_of_k = [](int i) { return (uint32_t) max(0, 2 * i - 1); };
-    auto slot_of_v = [](int i, int n) { return (uint32_t) (i + 1 < n ? 2 * i + 2 : 2 * i + 1); };
+    if (NQ > 1 && warp >= W_QK) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == W_COPY) {
-        fewer();
         // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
         // the lower half of the warp, V's by the upper
         const int box = min(A.page_size, KEYS), boxes = BN / box, which = lane % 16;
@@ -793,31 +794,34 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             }
             return p;
         };
-        int slot = 0, turn = 0, brought = 0, page = page_of(-is_v);
+        int page = page_of(-is_v), k_tiles = 0, v_tiles = 0;
         bool ok = true;
-        for (int t = 0; ok && t <= n && n > 0; t++) {
+        for (int t = 0; ok && t <= n && n > 0; t++) {  // K(t), then V(t - 1)
             const int next = page_of(t + 1 - is_v);
             for (int v = 0; v < 2; v++) {
                 if (v ? t == 0 : t == n) continue;
-                if (turn > 0 && !(ok = wait_soon(&empty[slot], (turn - 1) & 1, gone, A.err))) break;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::KV_BYTES);
+                const int i = t - v, at = v ? i % VS : i % KS, turn = v ? i / VS : i / KS;
+                uint64_t *const full = v ? &v_full[at] : &k_full[at], *const empty = v ? &v_empty[at] : &k_empty[at];
+                if (turn > 0 && !(ok = wait_soon(empty, (turn - 1) & 1, gone, A.err))) break;
+                if (lane == 0) mbar_arrive_expect_tx(full, C::KV_BYTES);
                 __syncwarp();
                 if (has && v == is_v) {
-                    const int key = from + (t - v) * BN + kb * box;
-                    tma_load_4d(ring + slot * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, &full[slot],
+                    const int key = from + i * BN + kb * box;
+                    tma_load_4d((v ? v_sm : k_sm) + at * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, full,
                                 col, key % A.page_size, kv_head, page);
                 }
-                brought++;
-                if (++slot == SLOTS) slot = 0, turn++;
+                if (v) v_tiles = i + 1;
+                else k_tiles = i + 1;
             }
             page = next;
         }
         // the last copies land before the block ends, whatever the others do
-        for (int k = max(0, brought - SLOTS); k < brought; k++)
-            mbar_wait_bounded(&full[k % SLOTS], (k / SLOTS) & 1, nullptr, WAIT_LIMIT_NS);
+        for (int i = max(0, k_tiles - KS); i < k_tiles; i++)
+            mbar_wait_bounded(&k_full[i % KS], (i / KS) & 1, nullptr, WAIT_LIMIT_NS);
+        for (int i = max(0, v_tiles - VS); i < v_tiles; i++)
+            mbar_wait_bounded(&v_full[i % VS], (i / VS) & 1, nullptr, WAIT_LIMIT_NS);
         if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_QK || warp == W_PV) {
-        fewer();
         // The scores' MMAs and the products' by a warp each: a wait or a commit
         // takes 100 to 250 clocks before the next MMA issues, and the tensor
         // cores, which hold but a few MMAs ahead, work for the other warp
@@ -834,13 +838,13 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         bool ok = true;
         if (warp == W_QK && n > 0) {
             constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
-            const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(ring);
+            const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm);
             uint32_t used = 0;  // score tiles so far: the next waits until the last is in registers
             ok = wait(&q_full, 0);
             for (int i = 0; ok && i < n; i++) {
-                const uint32_t u = slot_of_k(i), at = u % SLOTS;
+                const int at = i % KS;
                 const uint64_t kt = k_desc + at * (C::KV_BYTES >> 4);
-                if (!(ok = wait(&full[at], u / SLOTS))) break;
+                if (!(ok = wait(&k_full[at], i / KS))) break;
                 for (int q = 0; q < nq; q++) {
                     if (used > 0 && !(ok = wait(&s_free, used - 1))) break;
                     used++;
@@ -851,22 +855,22 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                             tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
                                         kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), ID, ks > 0);
                         tc_commit(&s_full[q]);
-                        if (q == nq - 1) tc_commit(&empty[at]);
+                        if (q == nq - 1 && i + KS < n) tc_commit(&k_empty[at]);  // (else nobody waits for it)
                     }
                 }
             }
         } else if (n > 0) {
             constexpr uint32_t ID = (1u << 4) | TYPE | (1u << 16) | ((uint32_t) (DP >> 3) << 17) | (8u << 24);
-            const uint64_t v_desc = sw128_desc_mn(ring, BN * 128);
+            const uint64_t v_desc = sw128_desc_mn(v_sm, BN * 128);
             for (int i = 0; ok && i < n; i++) {
-                const uint32_t u = slot_of_v(i, n), at = u % SLOTS;
+                const int at = i % VS;
                 const uint64_t vt = v_desc + at * (C::KV_BYTES >> 4);
-                if (!(ok = wait(&full[at], u / SLOTS))) break;
+                if (!(ok = wait(&v_full[at], i / VS))) break;
                 for (int q = 0; ok && q < nq; q++) {
                     const uint32_t p_at = tmem + C::P_COL + (q * NP + i % NP) * (BN / 2);
 #pragma unroll
                     for (int h = 0; h < PARTS; h++) {
-                        if (!(ok = wait(&p_full[q][h], i))) break;
+                        if (!(ok = wait(&p_full[q][i % NP][h], i / NP))) break;
                         if (elect_one()) {
 #pragma unroll
                             for (int ks = h * (C::PART / 16); ks < (h + 1) * (C::PART / 16); ks++)
@@ -874,7 +878,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                                               i > 0 || ks > 0);
                             if (h == PARTS - 1) {
                                 tc_commit(&pv_done[q][i % NP]);
-                                if (q == nq - 1) tc_commit(&empty[at]);
+                                if (q == nq - 1 && i + VS < n) tc_commit(&v_empty[at]);
                             }
                         }
                     }
@@ -886,9 +890,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             mbar_wait_bounded(&drained[warp - W_QK], 0, nullptr, WAIT_LIMIT_NS);
         }
         __syncwarp();
-    } else if (warp > W_COPY) {
-        fewer();
-    } else {
+    } else if (warp < W_QK) {
         if (NQ > 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int q = warp / 4, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t) (warp % 4 * 32) << 16;
@@ -934,9 +936,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                         if (c * 32 + e >= z) x[c][e] = 0xff800000u;
                 // keys that not every row of the block sees: their NaN and
                 // infinities out of the tile of values (add_not_finite)
-                const uint32_t at = slot_of_v(i, n);
-                if (!(ok = wait_soon(&full[at % SLOTS], (at / SLOTS) & 1, gone, A.err))) break;
-                uint8_t *vt = ring + at % SLOTS * C::KV_BYTES;
+                if (!(ok = wait_soon(&v_full[i % VS], (i / VS) & 1, gone, A.err))) break;
+                uint8_t *vt = v_sm + i % VS * C::KV_BYTES;
                 const int c0 = sp.clo - key0, c1 = min(sp.chi, to) - key0;
                 bool found = false;
 #pragma unroll 4
@@ -1000,7 +1001,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[q][h]);
+                if (lane == 0) mbar_arrive(&p_full[q][i % NP][h]);
             }
             float sa, sb;
             unpack2(add2(s0, s1), sa, sb);
@@ -1019,9 +1020,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 #pragma unroll 1
                 for (int c = 0; c < DP; c += 8) {
                     float r[8];
+                    __syncwarp();
                     tmem_ld_32x32b_x8(o_at + c, r);
                     if (valid && c < A.d)
                         add_not_finite<F16>(A, seq, kv_head, c, max(lo, from), min(hi, to), sp.clo, max(sp.clo, sp.chi), r);
+                    __syncwarp();
                     tmem_st_32x32b_x8(o_at + c, r);
                 }
             }
@@ -1037,6 +1040,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 #pragma unroll 1
                 for (int c = 0; c < DP; c += 32) {
                     uint32_t o[32];
+                    __syncwarp();  // rows that hold nothing skip the stores, not the loads
                     if (n > 0) {
                         tmem_ld_32x32b_x32(o_at + c, o);
                         tmem_ld_wait(o);

@@ -131,6 +131,17 @@ def test_equals_the_definition(dt, d, heads, kv_heads, page, lens, causal, windo
     c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, causal=causal, window=window), causal, window)
 
 
+@pytest.mark.parametrize("dt,d,heads,kv_heads,page,lens,causal,window", [
+    (BF, 256, 6, 1, 128, [(39, 3068), (39, 3068)], True, 0), (HF, 256, 24, 4, 64, [(500, 3000)], True, 0),
+    (BF, 256, 8, 8, 16, [(190, 4000), (19, 2000)], False, 0), (BF, 200, 32, 8, 32, [(300, 2500)], True, 400),
+    (HF, 128, 16, 4, 16, [(600, 4000), (33, 1000)], True, 0), (BF, 64, 16, 4, 16, [(600, 4000), (33, 1000)], True, 0)])
+def test_many_tiles_one_after_another(dt, d, heads, kv_heads, page, lens, causal, window):
+    """Long enough for every buffer to be used many times over, several times."""
+    c = Case(lens, heads, kv_heads, d, page, dt, seed=d)
+    for _ in range(4):
+        c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, causal=causal, window=window), causal, window)
+
+
 @pytest.mark.parametrize("lens", [[(1, 3000)], [(1, 5000), (1, 100), (1, 2500)], [(40, 3000)], [(200, 6000)]])
 @pytest.mark.parametrize("heads_first", [False, True])
 def test_long_keys_are_cut_and_joined(lens, heads_first):
