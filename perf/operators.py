@@ -238,7 +238,7 @@ def _run_own(s):
             return Z.kv_attend(cache, 0, batch, s["q"], causal=c["causal"], window=c["window"], out=s["out"],
                                err=s["err"])
         Z.kv_append(cache, 0, batch, s["kn"], s["vn"], q=s["q"], q_out=s["q_out"], k_norm=s["k_norm"],
-                    q_norm=s["q_norm"], eps=EPS, rope=s["rope"], mode=Z.ROPE_NEOX if c["neox"] else Z.ROPE_NORMAL,
+                    q_norm=s["q_norm"], eps=EPS if c["norm"] else -1.0, rope=s["rope"], mode=Z.ROPE_NEOX if c["neox"] else Z.ROPE_NORMAL,
                     err=s["err"])
         return s["q_out"], s["k"], s["v"]
     tables = Z.KvTables(s["refs"], s["table"], s["len"])
