@@ -571,18 +571,22 @@ struct many_rows {
     static constexpr int BN = DP == 256 ? 64 : 128; // keys of a tile
     static constexpr int PART = 64;                 // keys whose weights are handed over at once
     static constexpr int PARTS = BN / PART;
-    static constexpr int Q_BYTES = 128 * DP * 2;
+    // One query tile leaves TMEM room for Q: its 64 KB of shared memory hold two
+    // tiles more of keys and values, and the scores' MMAs, 64 keys wide, read half
+    // as many bytes
+    static constexpr bool Q_TMEM = NQ == 1;
+    static constexpr int Q_BYTES = Q_TMEM ? 0 : 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
-    static constexpr int KS = DP == 64 ? 4 : 3, VS = DP == 64 ? 4 : 2;  // tiles of K and of V in flight or in use
+    static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 64 ? 4 : DP == 128 ? 2 : 3;  // tiles of K and of V in flight or in use
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + (KS + VS) * KV_BYTES;
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
-    static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V and the copies, one idle
+    static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V, K's copies and V's
     // Buffers of P: two where one query tile has the block to itself, since the
     // next scores' MMAs (1,000 clocks at 256 columns) go ahead of P's otherwise
     static constexpr int NP = NQ > 1 ? 1 : 2;
-    // TMEM columns: O of each query tile, the scores, P of each query tile
-    static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, COLS = 512;
-    static_assert(P_COL + NQ * NP * BN / 2 <= COLS, "TMEM holds O, S and P");
+    // TMEM columns: O of each query tile, the scores, P of each query tile, Q
+    static constexpr int O_COL = 0, S_COL = NQ * DP, P_COL = S_COL + BN, Q_COL = P_COL + NQ * NP * BN / 2, COLS = 512;
+    static_assert(Q_COL + (Q_TMEM ? DP / 2 : 0) <= COLS, "TMEM holds O, S, P and Q");
     // a softmax warp looks at V(i) having seen the product of tile i - NP done
     static_assert(VS >= NP, "V(i - VS) has been used when a softmax warp waits for V(i)");
 };
@@ -731,7 +735,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 
     constexpr int W_QK = C::SOFTMAX / 32, W_PV = W_QK + 1, W_COPY = W_QK + 2;
     if (threadIdx.x == 0) {
-        mbar_init(&q_full, 1);
+        mbar_init(&q_full, C::Q_TMEM ? 4 : 1);
         for (int i = 0; i < KS; i++) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
@@ -767,13 +771,18 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     // A row of scores lives in registers: the softmax warps take the others'
     // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
     if (NQ > 1 && warp >= W_QK) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == W_COPY) {
-        // Q once, then a box of min(page, 64) keys by 64 columns a lane: K's by
-        // the lower half of the warp, V's by the upper
-        const int box = min(A.page_size, KEYS), boxes = BN / box, which = lane % 16;
-        const int is_v = lane / 16, kb = which % boxes, col = which / boxes * 64;
+    if (warp >= W_COPY) {
+        // Q and K by one warp, V by the other: a box of min(page, 64) keys by 64
+        // columns a lane. Lanes issue their boxes one after another, about 100
+        // clocks each, and a tile costs some 600 besides.
+        const bool is_v = warp > W_COPY;
+        const int box = min(A.page_size, KEYS), boxes = BN / box, kb = lane % boxes, col = lane / boxes * 64;
+        const int shift = __ffs(A.page_size) - 1;  // a power of two
         const CUtensorMap *map = is_v ? &tv : &tk;
-        if (n > 0 && lane == 0) {
+        uint8_t *const ring = is_v ? v_sm : k_sm;
+        uint64_t *const full = is_v ? v_full : k_full, *const empty = is_v ? v_empty : k_empty;
+        const int slots = is_v ? VS : KS;
+        if (!C::Q_TMEM && !is_v && n > 0 && lane == 0) {
             mbar_arrive_expect_tx(&q_full, nq * (DP / 64) * per_tile * A.group * 128);
             for (int q = 0; q < nq; q++)
                 for (int c = 0; c < DP / 64; c++)
@@ -782,45 +791,39 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         }
         __syncwarp();
         const bool has = col < DP;
-        auto page_of = [&](int i) {  // of this lane's box of tile i (K or V)
+        const int *const table = A.b.table + (int64_t) seq * A.b.table_stride;
+        const int first_page = sp.lo >> shift;
+        // this lane's box of tile i holds keys that a row sees (the entry of a page without may be none)
+        auto seen = [&](int key) { return has && key < to && key >> shift >= first_page; };
+        auto entry = [&](int i) {
             const int key = from + i * BN + kb * box;
-            // a page that no row sees is outside the tensor: zeros (its entry may be none)
-            if (!has || i < 0 || i >= n || key >= to || (key / A.page_size + 1) * A.page_size <= sp.lo)
-                return (int) A.pages;
-            const int p = A.b.table[seq * A.b.table_stride + key / A.page_size];
-            if (p < 0 || p >= A.pages) {
-                atomicOr(A.err, ZEST_ERR_BAD_PAGE);
-                return (int) A.pages;
-            }
-            return p;
+            return seen(key) ? table[key >> shift] : -1;
         };
-        int page = page_of(-is_v), k_tiles = 0, v_tiles = 0;
-        bool ok = true;
-        for (int t = 0; ok && t <= n && n > 0; t++) {  // K(t), then V(t - 1)
-            const int next = page_of(t + 1 - is_v);
-            for (int v = 0; v < 2; v++) {
-                if (v ? t == 0 : t == n) continue;
-                const int i = t - v, at = v ? i % VS : i % KS, turn = v ? i / VS : i / KS;
-                uint64_t *const full = v ? &v_full[at] : &k_full[at], *const empty = v ? &v_empty[at] : &k_empty[at];
-                if (turn > 0 && !(ok = wait_soon(empty, (turn - 1) & 1, gone, A.err))) break;
-                if (lane == 0) mbar_arrive_expect_tx(full, C::KV_BYTES);
-                __syncwarp();
-                if (has && v == is_v) {
-                    const int key = from + i * BN + kb * box;
-                    tma_load_4d((v ? v_sm : k_sm) + at * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, full,
-                                col, key % A.page_size, kv_head, page);
+        int page = entry(0), i = 0, at = 0, phase = 1;  // phase: of the slot's last use
+        for (; i < n; i++) {
+            const int next = entry(i + 1);  // looked at a tile later
+            if (i >= slots && !wait_soon(&empty[at], phase, gone, A.err)) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[at], C::KV_BYTES);
+            __syncwarp();
+            if (has) {
+                const int key = from + i * BN + kb * box;
+                if (page < 0 || page >= A.pages) {
+                    if (seen(key)) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+                    page = (int) A.pages;  // outside the tensor: zeros
                 }
-                if (v) v_tiles = i + 1;
-                else k_tiles = i + 1;
+                tma_load_4d(ring + at * C::KV_BYTES + col / 64 * (BN * 128) + kb * box * 128, map, &full[at], col,
+                            key & (A.page_size - 1), kv_head, page);
             }
             page = next;
+            if (++at == slots) {
+                at = 0;
+                phase ^= 1;
+            }
         }
         // the last copies land before the block ends, whatever the others do
-        for (int i = max(0, k_tiles - KS); i < k_tiles; i++)
-            mbar_wait_bounded(&k_full[i % KS], (i / KS) & 1, nullptr, WAIT_LIMIT_NS);
-        for (int i = max(0, v_tiles - VS); i < v_tiles; i++)
-            mbar_wait_bounded(&v_full[i % VS], (i / VS) & 1, nullptr, WAIT_LIMIT_NS);
-        if (n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
+        for (int k = max(0, i - slots); k < i; k++)
+            mbar_wait_bounded(&full[k % slots], (k / slots) & 1, nullptr, WAIT_LIMIT_NS);
+        if (!C::Q_TMEM && !is_v && n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_QK || warp == W_PV) {
         // The scores' MMAs and the products' by a warp each: a wait or a commit
         // takes 100 to 250 clocks before the next MMA issues, and the tensor
@@ -851,9 +854,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     const uint64_t qt = q_desc + q * (C::Q_BYTES >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (int ks = 0; ks < DP / 16; ks++)
-                            tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4),
-                                        kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4), ID, ks > 0);
+                        for (int ks = 0; ks < DP / 16; ks++) {
+                            const uint64_t kd = kt + ((ks / 4 * (BN * 128) + ks % 4 * 32) >> 4);
+                            if (C::Q_TMEM) tc_mma_f16_ts(tmem + C::S_COL, tmem + C::Q_COL + ks * 8, kd, ID, ks > 0);
+                            else tc_mma_bf16(tmem + C::S_COL, qt + ((ks / 4 * (128 * 128) + ks % 4 * 32) >> 4), kd, ID, ks > 0);
+                        }
                         tc_commit(&s_full[q]);
                         if (q == nq - 1 && i + KS < n) tc_commit(&k_empty[at]);  // (else nobody waits for it)
                     }
@@ -901,6 +906,24 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const int lo = valid ? row_lo(A, s, t) : 0, hi = valid ? row_hi(A, s, t) : 0;
         // tiles [i0, i1) are seen whole by every row of the block
         const int i0 = max(0, sp.clo - from + BN - 1) / BN, i1 = max(0, min(sp.chi, to) - from) / BN;
+        if (C::Q_TMEM && n > 0) {  // the row of Q, two values a column
+            const uint16_t *src = valid ? A.q + (s.q0 + (int64_t) t) * A.ldq + (kv_head * A.group + row % A.group) * A.d : A.q;
+            const int d = valid ? A.d : 0;
+            uint32_t x[DP / 64][32];  // all the loads under way at once
+#pragma unroll
+            for (int c = 0; c < DP; c += 8) {
+                const uint4 w = c < d ? *reinterpret_cast<const uint4 *>(src + c) : make_uint4(0, 0, 0, 0);
+                uint32_t *const at = &x[c / 64][c % 64 / 2];
+                at[0] = w.x, at[1] = w.y, at[2] = w.z, at[3] = w.w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < DP / 64; c++) tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + c * 32, x[c]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
         float m = -INFINITY, l = 0.0f;
         bool ok = q < nq;
         for (int i = 0; ok && i < n; i++) {
@@ -1029,46 +1052,61 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 }
             }
             // Rolled, since every block comes through here once and pays for
-            // each line of code. 16-bit results go through the query tile's
-            // shared memory (its scores are all made), a row of DP a thread, 16
-            // bytes at unit ^ (row % 8), and out of it in whole rows.
-            uint8_t *const rows16 = q_sm + q * C::Q_BYTES + warp % 4 * 32 * (DP * 2);
+            // each line of code. 16-bit results go through shared memory (the
+            // query tile's, whose scores are all made, or the tiles', all used), a
+            // row of DP a thread, 16 bytes at unit ^ (row % 8), and out of it in
+            // whole rows.
+            uint8_t *const rows16 = (C::Q_TMEM ? k_sm : q_sm + q * C::Q_BYTES) + warp % 4 * 32 * (DP * 2);
             const bool whole = A.splits == 1;
 #pragma unroll 1
             for (int pass = 0; pass < (whole && A.a_next ? 2 : 1); pass++) {  // A.out and the rest; A.a_next
                 __syncwarp();
 #pragma unroll 1
-                for (int c = 0; c < DP; c += 32) {
-                    uint32_t o[32];
+                for (int c = 0; c < DP; c += 64) {
+                    uint32_t o[2][32];
                     __syncwarp();  // rows that hold nothing skip the stores, not the loads
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (n > 0) tmem_ld_32x32b_x32(o_at + c + 32 * h, o[h]);
+                        else
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[h][e] = 0;
                     if (n > 0) {
-                        tmem_ld_32x32b_x32(o_at + c, o);
-                        tmem_ld_wait(o);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = 0;
+                        tmem_ld_wait(o[0]);
+                        tmem_ld_wait(o[1]);
                     }
+                    auto eights = [&](auto store) {  // of eight columns' values each
+#pragma unroll
+                        for (int e = 0; e < 64; e += 8) {
+                            float r[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) r[k] = __uint_as_float(o[e / 32][e % 32 + k]) * inv;
+                            store(e, r);
+                        }
+                    };
+                    uint8_t *const at = rows16 + lane * (DP * 2) + c * 2;
                     if (!valid) continue;
+                    if (!whole) {  // unnormalised; the workspace's rows have room for DP values
+                        float4 *const dst = reinterpret_cast<float4 *>(A.part + slot * DP + c);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        float r[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) r[k] = __uint_as_float(o[e + k]);
-                        if (!whole) {  // (the workspace's rows have room for DP values)
-                            float4 *dst = reinterpret_cast<float4 *>(A.part + slot * DP + c + e);
-                            dst[0] = make_float4(r[0], r[1], r[2], r[3]);
-                            dst[1] = make_float4(r[4], r[5], r[6], r[7]);
-                            continue;
+                        for (int e = 0; e < 64; e += 4) {
+                            const uint32_t *const x = &o[e / 32][e % 32];
+                            dst[e / 4] = make_float4(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]),
+                                                     __uint_as_float(x[3]));
                         }
-#pragma unroll
-                        for (int k = 0; k < 8; k++) r[k] *= inv;
-                        uint4 *at =
-                            reinterpret_cast<uint4 *>(rows16 + lane * (DP * 2) + (((c + e) / 8 ^ (lane & 7)) << 4));
-                        if (pass == 1) *at = pack8(r);
-                        else {
-                            if (A.out) *at = round8<F16>(r);
-                            if (A.y && c + e < A.d) store8_f32(A, tok, head, c + e, r);
-                        }
+                    } else if (pass == 1) {
+                        eights([&](int e, const float (&r)[8]) {
+                            *reinterpret_cast<uint4 *>(at + ((e / 8 ^ (lane & 7)) << 4)) = pack8(r);
+                        });
+                    } else {
+                        if (A.out)
+                            eights([&](int e, const float (&r)[8]) {
+                                *reinterpret_cast<uint4 *>(at + ((e / 8 ^ (lane & 7)) << 4)) = round8<F16>(r);
+                            });
+                        if (A.y)
+                            eights([&](int e, const float (&r)[8]) {
+                                if (c + e < A.d) store8_f32(A, tok, head, c + e, r);
+                            });
                     }
                 }
                 uint16_t *const base = pass == 0 ? A.out : A.a_next;
@@ -1077,8 +1115,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 const int64_t ld = pass == 0 ? A.ldo : A.lda;
                 constexpr int UNITS = DP / 8, AT_ONCE = 32 / UNITS, N = 4;
                 const int u = lane % UNITS, rows = min(32, (tq1 - tq0) * A.group - warp % 4 * 32);
-                uint16_t *const col = base + kv_head * A.group * A.d + u * 8;
-                int g = (warp % 4 * 32 + lane / UNITS) % A.group, tk = (warp % 4 * 32 + lane / UNITS) / A.group;
+                const int r1 = warp % 4 * 32 + lane / UNITS;  // this lane's first row of the tile
+                int g = r1 % A.group;
+                uint16_t *dst = base + (s.q0 + (int64_t) (tq0 + r1 / A.group)) * ld + (kv_head * A.group + g) * A.d + u * 8;
+                const int64_t wrap = ld - (int64_t) A.group * A.d;  // from a token's last head to the next's first
+                const bool has = u * 8 < A.d;
 #pragma unroll 1
                 for (int r0 = lane / UNITS; r0 < rows; r0 += N * AT_ONCE) {
                     uint4 v[N];
@@ -1089,9 +1130,9 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     }
 #pragma unroll
                     for (int k = 0; k < N; k++) {
-                        if (r0 + k * AT_ONCE < rows && u * 8 < A.d)
-                            *reinterpret_cast<uint4 *>(col + (s.q0 + (int64_t) (tq0 + tk)) * ld + g * A.d) = v[k];
-                        for (g += AT_ONCE; g >= A.group; g -= A.group) tk++;
+                        if (has && r0 + k * AT_ONCE < rows) *reinterpret_cast<uint4 *>(dst) = v[k];
+                        dst += AT_ONCE * A.d;
+                        for (g += AT_ONCE; g >= A.group; g -= A.group) dst += wrap;
                     }
                 }
             }
