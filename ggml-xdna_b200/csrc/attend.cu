@@ -47,6 +47,7 @@ struct attend_args {
     int64_t chunk;      // many rows: keys a block takes, a multiple of 128
     int splits;         // parts of a row that go to the workspace (1: none does, the result is whole)
     int join;           // few rows: blocks of a cluster, each with an equal part of the keys (then splits is 1)
+    int by_rows;        // many rows: every head's last rows first, not one head's after another's
     int wide;           // few rows: a box has a head's columns whole
     float2 *ml;         // [splits][T * heads]: m and l
     float *part;        // [splits][T * heads][DP]: o
@@ -205,17 +206,16 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     __shared__ float m_sh[4][ROWS], l_sh[4][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = blockIdx.z, split = blockIdx.x;  // the part of the keys (in a cluster, the block's rank)
-    const int row_tiles = gridDim.y / (A.heads / A.group);
-    const int kv_head = blockIdx.y / row_tiles, tile = blockIdx.y % row_tiles;
+    const int kv_head = blockIdx.y;
 
     const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
     if (!s.ok) {
         if (threadIdx.x == 0) atomicOr(A.err, ZEST_ERR_BAD_SEQ);
         return;
     }
-    const int64_t rows = (int64_t) s.n * A.group, r0 = (int64_t) tile * ROWS;
-    if (r0 >= rows) return;
-    const key_span sp = span_of(A, s, (int) (r0 / A.group), (int) ((min(r0 + ROWS, rows) - 1) / A.group));
+    const int rows = s.n * A.group;  // at most ROWS
+    if (rows == 0) return;
+    const key_span sp = span_of(A, s, 0, s.n - 1);
     // this block's keys: from the first of the span's 64-key block on, by chunks
     const int64_t first = (int64_t) sp.lo / KEYS * KEYS, blocks = (max((int64_t) sp.hi - first, (int64_t) 0) + KEYS - 1) / KEYS;
     const int64_t chunk = (blocks + gridDim.x - 1) / gridDim.x * KEYS;
@@ -295,11 +295,11 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     const uint16_t *qp[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-        const int64_t r = r0 + g + 8 * e;
+        const int r = g + 8 * e;
         lo[e] = hi[e] = 0;
         qp[e] = nullptr;
         if (r < rows) {
-            const int t = (int) (r / A.group);
+            const int t = r / A.group;
             lo[e] = row_lo(A, s, t);
             hi[e] = row_hi(A, s, t);
             qp[e] = A.q + (s.q0 + (int64_t) t) * A.ldq + (int64_t) (kv_head * A.group + r % A.group) * A.d;
@@ -458,7 +458,6 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         }
     named_barrier(1, 128);
     const int row = threadIdx.x >> 3;
-    const int64_t r = r0 + row;
     float mx = -INFINITY, w[4], sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; k++) mx = fmaxf(mx, m_sh[k][row]);
@@ -467,10 +466,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         w[k] = m_sh[k][row] == -INFINITY ? 0.0f : exp2_fast(m_sh[k][row] - mx);
         sum += w[k] * l_sh[k][row];
     }
-    const int t = (int) (r / A.group), head = kv_head * A.group + (int) (r % A.group);
+    const int t = row / A.group, head = kv_head * A.group + row % A.group;
     const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const bool live = r < rows && !stop;  // a wait that ran out leaves the rows as they were
+    const bool live = row < rows && !stop;  // a wait that ran out leaves the rows as they were
 #pragma unroll
     for (int i = 0; i < DP / 64; i++) {
         const int c = (threadIdx.x & 7) * 8 + 64 * i;
@@ -508,8 +507,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
     if ((threadIdx.x & 7) == 0) ml_sh[row] = make_float2(stop ? NAN : mx, sum);
     __syncwarp();
     cluster_sync();
-    const int live_rows = (int) min((int64_t) ROWS, rows - r0);
-    for (int u = split * 128 + threadIdx.x; u < live_rows * (DP / 8); u += A.join * 128) {
+    for (int u = split * 128 + threadIdx.x; u < rows * (DP / 8); u += A.join * 128) {
         const int jr = u / (DP / 8), c = u % (DP / 8) * 8;
         if (c >= A.d) continue;
         float2 part[8];
@@ -544,8 +542,8 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(v[e], f, x[e]);
             }
-        const int64_t jrow = r0 + jr, jtok = s.q0 + jrow / A.group;
-        const int jhead = kv_head * A.group + (int) (jrow % A.group);
+        const int64_t jtok = s.q0 + (int64_t) (jr / A.group);
+        const int jhead = kv_head * A.group + jr % A.group;
         if (!whole) continue;
         const float scale = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
@@ -715,9 +713,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int seq = blockIdx.z;
-    const int kv_head = blockIdx.y / A.splits, split = blockIdx.y % A.splits;
-    const int tile = gridDim.x - 1 - blockIdx.x;  // the last rows see the most keys: first
+    // the last rows see the most keys: first
+    const int heads = A.heads / A.group, tiles = gridDim.x / (heads * A.splits), split = blockIdx.x % A.splits;
+    const int unit = blockIdx.x / A.splits, seq = blockIdx.y;
+    const int kv_head = A.by_rows ? unit % heads : unit / tiles;
+    const int tile = tiles - 1 - (A.by_rows ? unit / heads : unit % tiles);
 
     const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
     if (!s.ok) {
@@ -1264,7 +1264,7 @@ zest_kv_batch tightened(const zest_kv_cache *kv, const zest_kv_batch *b) {
 // How a call runs: its row tiles, and the chunks its keys are cut into.
 struct attend_plan {
     int dp, tile_rows, splits, join;
-    bool many, wide;
+    bool many, wide, by_rows;
     int64_t row_tiles, chunk, ws_ml, ws_part;
 };
 
@@ -1278,6 +1278,11 @@ struct attend_plan {
 // that have an SM each join as one cluster, without a second launch; more go
 // through the workspace (as clusters of 4 the 32 tokens took 128 us, and one
 // token over 131,072 keys 127 for 91: clusters wait for a GPC's SMs together).
+// Many rows: where rows differ much in the keys they see, the blocks with the
+// most run first, of all heads, so that the last to start are short (2,048
+// tokens of 2,048: 72 us one head after another, 58 so; over 8,192: 199 and
+// 190). With long keys all blocks are alike, and neighbours on one head's keys
+// find them in L2 (over 32,768: 910 and 928; heads of 256 over 8,192: 290 and 307).
 attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const zest_kv_attn *at) {
     attend_plan p;
     p.dp = kv->d <= 64 ? 64 : kv->d <= 128 ? 128 : 256;
@@ -1291,6 +1296,7 @@ attend_plan plan_attend(const zest_kv_cache *kv, const zest_kv_batch *b, const z
     int64_t span = b->max_kv;
     if (at->causal && at->window)  // which may start inside a block of keys
         span = std::min(span, std::min(at->window, span) + std::min<int64_t>(b->max_q, p.tile_rows) + KEYS - 1);
+    p.by_rows = p.dp < 256 && span < 8 * b->max_q;
     const int64_t once = std::max<int64_t>(1, 148 * per_sm / units), least = p.many ? 512 : 128;
     int64_t splits = once;
     if (b->n_seqs > 1) splits = std::max(once, std::min(148 * per_sm * 4 / units, up(span, 1024)));
@@ -1320,7 +1326,7 @@ const char *attend_fault(const zest_kv_cache *kv, const zest_kv_batch *b, const 
     if (!(at->scale > 0.0f) || std::isinf(at->scale * LOG2E)) return "scale is not positive and finite";
     if (at->window < 0 || (at->window > 0 && !at->causal)) return "a window is positive and causal";
     const attend_plan p = plan_attend(kv, b, at);
-    if (p.splits * (int64_t) kv->kv_heads > 65535 || b->max_q * (at->heads / kv->kv_heads) > 0x7fffffff)
+    if (p.row_tiles * kv->kv_heads * p.splits > 0x7fffffff || b->max_q * (at->heads / kv->kv_heads) > 0x7fffffff)
         return "too many rows, or too many heads for the keys";
     return nullptr;
 }
@@ -1360,13 +1366,13 @@ int launch_attend(const zest_kv_cache *kv, const CUtensorMap &tk, const CUtensor
         CUtensorMap tq;
         if (!query_tmap(&tq, a)) return kv_refuse(call, "the queries' strides make no tensor map");
         if (!allow_smem(kv_attend_many_kernel<DP, F16>, C::SMEM, many_ready)) return check_launch(call);
-        const dim3 grid((unsigned) p.row_tiles, (unsigned) (kv->kv_heads * p.splits), a.b.n_seqs);
+        const dim3 grid((unsigned) (p.row_tiles * kv->kv_heads * p.splits), a.b.n_seqs);
         kv_attend_many_kernel<DP, F16><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, a);
     } else {
         using C = few_rows<DP>;
         if (!allow_smem(kv_attend_few_kernel<DP, F16>, C::SMEM, few_ready)) return check_launch(call);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(p.splits * p.join, (unsigned) (p.row_tiles * kv->kv_heads), a.b.n_seqs);
+        cfg.gridDim = dim3(p.splits * p.join, kv->kv_heads, a.b.n_seqs);
         cfg.blockDim = dim3(FEW_THREADS);
         cfg.dynamicSmemBytes = C::SMEM;
         cfg.stream = st;
@@ -1458,6 +1464,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.splits = p.splits;
     a.join = p.join;
     a.wide = p.wide;
+    a.by_rows = p.by_rows;
     a.ml = (float2 *) workspace;
     a.part = (float *) ((uint8_t *) workspace + p.ws_ml);
     a.err = err;
