@@ -573,10 +573,11 @@ struct many_rows {
     // tiles more of keys and values, and the scores' MMAs, 64 keys wide, read half
     // as many bytes
     static constexpr bool Q_TMEM = NQ == 1;
-    static constexpr int Q_BYTES = Q_TMEM ? 0 : 128 * DP * 2;
+    static constexpr int Q_BYTES = 128 * DP * 2;
     static constexpr int KV_BYTES = BN * DP * 2;
     static constexpr int KS = DP == 128 ? 3 : 4, VS = DP == 64 ? 4 : DP == 128 ? 2 : 3;  // tiles of K and of V in flight or in use
-    static constexpr int SMEM = 1024 + NQ * Q_BYTES + (KS + VS) * KV_BYTES;
+    static constexpr int SMEM = 1024 + (Q_TMEM ? 0 : NQ * Q_BYTES) + (KS + VS) * KV_BYTES;
+    static_assert(!Q_TMEM || Q_BYTES == (VS - 1) * KV_BYTES, "Q comes in through V's slots but the first");
     static constexpr int SOFTMAX = NQ * 128;        // threads: one a row
     static constexpr int THREADS = SOFTMAX + 128;   // and a warp each for Q K^T, P V, K's copies and V's
     // Buffers of P: two where one query tile has the block to itself, since the
@@ -704,11 +705,12 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     using C = many_rows<DP>;
     constexpr int NQ = C::NQ, NP = C::NP, BN = C::BN, KS = C::KS, VS = C::VS, PARTS = C::PARTS;
     extern __shared__ uint8_t dyn[];
-    uint8_t *q_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
-    uint8_t *k_sm = q_sm + NQ * C::Q_BYTES, *v_sm = k_sm + KS * C::KV_BYTES;
+    uint8_t *const tiles_sm = reinterpret_cast<uint8_t *>(((uintptr_t) dyn + 1023) & ~(uintptr_t) 1023);
+    uint8_t *const k_sm = tiles_sm + (C::Q_TMEM ? 0 : NQ * C::Q_BYTES), *const v_sm = k_sm + KS * C::KV_BYTES;
+    uint8_t *const q_sm = C::Q_TMEM ? v_sm + C::KV_BYTES : tiles_sm;
     // Every barrier's phases are waited for one after another by whoever waits
     // for it: a parity tells a phase from the one before it, not from the next.
-    __shared__ uint64_t q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[NQ], s_free, p_full[NQ][NP][PARTS],
+    __shared__ uint64_t q_in, q_full, k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[NQ], s_free, p_full[NQ][NP][PARTS],
         pv_done[NQ][NP], drained[2];
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
@@ -735,7 +737,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 
     constexpr int W_QK = C::SOFTMAX / 32, W_PV = W_QK + 1, W_COPY = W_QK + 2;
     if (threadIdx.x == 0) {
-        mbar_init(&q_full, C::Q_TMEM ? 4 : 1);
+        mbar_init(&q_in, 1);
+        mbar_init(&q_full, 4);
         for (int i = 0; i < KS; i++) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
@@ -782,11 +785,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         uint8_t *const ring = is_v ? v_sm : k_sm;
         uint64_t *const full = is_v ? v_full : k_full, *const empty = is_v ? v_empty : k_empty;
         const int slots = is_v ? VS : KS;
-        if (!C::Q_TMEM && !is_v && n > 0 && lane == 0) {
-            mbar_arrive_expect_tx(&q_full, nq * (DP / 64) * per_tile * A.group * 128);
+        if (!is_v && n > 0 && lane == 0) {
+            mbar_arrive_expect_tx(&q_in, nq * (DP / 64) * per_tile * A.group * 128);
             for (int q = 0; q < nq; q++)
                 for (int c = 0; c < DP / 64; c++)
-                    tma_load_3d(q_sm + q * C::Q_BYTES + c * (128 * 128), &tq, &q_full, c * 64, kv_head * A.group,
+                    tma_load_3d(q_sm + q * C::Q_BYTES + c * (128 * 128), &tq, &q_in, c * 64, kv_head * A.group,
                                 s.q0 + t0 + q * per_tile);
         }
         __syncwarp();
@@ -803,6 +806,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         for (; i < n; i++) {
             const int next = entry(i + 1);  // looked at a tile later
             if (i >= slots && !wait_soon(&empty[at], phase, gone, A.err)) break;
+            if (C::Q_TMEM && is_v && i == 1 && !wait_soon(&q_full, 0, gone, A.err)) break;  // Q has left the slots
             if (lane == 0) mbar_arrive_expect_tx(&full[at], C::KV_BYTES);
             __syncwarp();
             if (has) {
@@ -823,7 +827,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         // the last copies land before the block ends, whatever the others do
         for (int k = max(0, i - slots); k < i; k++)
             mbar_wait_bounded(&full[k % slots], (k / slots) & 1, nullptr, WAIT_LIMIT_NS);
-        if (!C::Q_TMEM && !is_v && n > 0) mbar_wait_bounded(&q_full, 0, nullptr, WAIT_LIMIT_NS);
+        if (!is_v && n > 0) mbar_wait_bounded(&q_in, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_QK || warp == W_PV) {
         // The scores' MMAs and the products' by a warp each: a wait or a commit
         // takes 100 to 250 clocks before the next MMA issues, and the tensor
@@ -843,7 +847,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             constexpr uint32_t ID = (1u << 4) | TYPE | ((uint32_t) (BN >> 3) << 17) | (8u << 24);
             const uint64_t q_desc = sw128_desc(q_sm), k_desc = sw128_desc(k_sm);
             uint32_t used = 0;  // score tiles so far: the next waits until the last is in registers
-            ok = wait(&q_full, 0);
+            ok = wait(C::Q_TMEM ? &q_full : &q_in, 0);
             for (int i = 0; ok && i < n; i++) {
                 const int at = i % KS;
                 const uint64_t kt = k_desc + at * (C::KV_BYTES >> 4);
@@ -906,26 +910,28 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const int lo = valid ? row_lo(A, s, t) : 0, hi = valid ? row_hi(A, s, t) : 0;
         // tiles [i0, i1) are seen whole by every row of the block
         const int i0 = max(0, sp.clo - from + BN - 1) / BN, i1 = max(0, min(sp.chi, to) - from) / BN;
+        bool ok = q < nq;
         if (C::Q_TMEM && n > 0) {  // the row of Q, two values a column
-            const uint16_t *src = valid ? A.q + (s.q0 + (int64_t) t) * A.ldq + (kv_head * A.group + row % A.group) * A.d : A.q;
-            const int d = valid ? A.d : 0;
-            uint32_t x[DP / 64][32];  // all the loads under way at once
+            ok = wait_soon(&q_in, 0, gone, A.err);
+            if (ok) {
 #pragma unroll
-            for (int c = 0; c < DP; c += 8) {
-                const uint4 w = c < d ? *reinterpret_cast<const uint4 *>(src + c) : make_uint4(0, 0, 0, 0);
-                uint32_t *const at = &x[c / 64][c % 64 / 2];
-                at[0] = w.x, at[1] = w.y, at[2] = w.z, at[3] = w.w;
+                for (int c = 0; c < DP / 64; c++) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(q_sm + c * (128 * 128) + row * 128 + ((u ^ (row & 7)) << 4));
+                        x[4 * u] = w.x, x[4 * u + 1] = w.y, x[4 * u + 2] = w.z, x[4 * u + 3] = w.w;
+                    }
+                    tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + c * 32, x);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full);
             }
-            __syncwarp();
-#pragma unroll
-            for (int c = 0; c < DP / 64; c++) tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + c * 32, x[c]);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
         }
         float m = -INFINITY, l = 0.0f;
-        bool ok = q < nq;
         for (int i = 0; ok && i < n; i++) {
             if (!(ok = wait_soon(&s_full[q], i & 1, gone, A.err))) break;
             tc_fence_after();
@@ -1056,8 +1062,9 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             // query tile's, whose scores are all made, or the tiles', all used), a
             // row of DP a thread, 16 bytes at unit ^ (row % 8), and out of it in
             // whole rows.
-            uint8_t *const rows16 = (C::Q_TMEM ? k_sm : q_sm + q * C::Q_BYTES) + warp % 4 * 32 * (DP * 2);
+            uint8_t *const rows16 = q_sm + q * C::Q_BYTES + warp % 4 * 32 * (DP * 2);
             const bool whole = A.splits == 1;
+            const int rows = min(32, (tq1 - tq0) * A.group - warp % 4 * 32);  // of this warp's that hold something
 #pragma unroll 1
             for (int pass = 0; pass < (whole && A.a_next ? 2 : 1); pass++) {  // A.out and the rest; A.a_next
                 __syncwarp();
@@ -1085,15 +1092,33 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                         }
                     };
                     uint8_t *const at = rows16 + lane * (DP * 2) + c * 2;
-                    if (!valid) continue;
-                    if (!whole) {  // unnormalised; the workspace's rows have room for DP values
-                        float4 *const dst = reinterpret_cast<float4 *>(A.part + slot * DP + c);
+                    if (!whole) {
+                        // unnormalised to the workspace, whose rows have room for DP
+                        // values: 32 columns at a time, a line of a row by 8 lanes
+                        // (a row a lane took 8,700 clocks where this takes XXX)
 #pragma unroll
-                        for (int e = 0; e < 64; e += 4) {
-                            const uint32_t *const x = &o[e / 32][e % 32];
-                            dst[e / 4] = make_float4(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]),
-                                                     __uint_as_float(x[3]));
+                        for (int h = 0; h < 2; h++) {
+                            __syncwarp();
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                *reinterpret_cast<uint4 *>(rows16 + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                                    make_uint4(o[h][4 * e], o[h][4 * e + 1], o[h][4 * e + 2], o[h][4 * e + 3]);
+                            __syncwarp();
+                            const int r1 = warp % 4 * 32 + lane / 8, u = lane % 8;
+                            int g = r1 % A.group;
+                            float *dst = A.part + (split * (A.b.T * A.heads) + (s.q0 + (int64_t) (tq0 + r1 / A.group)) * A.heads +
+                                                   kv_head * A.group + g) * DP + c + 32 * h + u * 4;
+                            const int64_t wrap = (int64_t) (A.heads - A.group) * DP;
+#pragma unroll
+                            for (int r = lane / 8; r < 32; r += 4) {
+                                if (r < rows)
+                                    *reinterpret_cast<uint4 *>(dst) =
+                                        *reinterpret_cast<const uint4 *>(rows16 + r * 128 + ((u ^ (r & 7)) << 4));
+                                dst += 4 * DP;
+                                for (g += 4; g >= A.group; g -= A.group) dst += wrap;
+                            }
                         }
+                    } else if (!valid) {
                     } else if (pass == 1) {
                         eights([&](int e, const float (&r)[8]) {
                             *reinterpret_cast<uint4 *>(at + ((e / 8 ^ (lane & 7)) << 4)) = pack8(r);
@@ -1114,7 +1139,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 __syncwarp();
                 const int64_t ld = pass == 0 ? A.ldo : A.lda;
                 constexpr int UNITS = DP / 8, AT_ONCE = 32 / UNITS, N = 4;
-                const int u = lane % UNITS, rows = min(32, (tq1 - tq0) * A.group - warp % 4 * 32);
+                const int u = lane % UNITS;
                 const int r1 = warp % 4 * 32 + lane / UNITS;  // this lane's first row of the tile
                 int g = r1 % A.group;
                 uint16_t *dst = base + (s.q0 + (int64_t) (tq0 + r1 / A.group)) * ld + (kv_head * A.group + g) * A.d + u * 8;
