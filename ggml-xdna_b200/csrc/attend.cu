@@ -715,11 +715,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     __shared__ uint32_t tmem_sh;
     __shared__ int stop, not_finite;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the last rows see the most keys: first
-    const int heads = A.heads / A.group, tiles = gridDim.x / (heads * A.splits), split = blockIdx.x % A.splits;
-    const int unit = blockIdx.x / A.splits, seq = blockIdx.y;
-    const int kv_head = A.by_rows ? unit % heads : unit / tiles;
-    const int tile = tiles - 1 - (A.by_rows ? unit / heads : unit % tiles);
+    // the last rows see the most keys: first; and neighbours on the same keys
+    const int units = A.heads / A.group * A.splits, tiles = gridDim.x / units, seq = blockIdx.y;
+    const int unit = A.by_rows ? blockIdx.x % units : blockIdx.x / tiles;
+    const int tile = tiles - 1 - (A.by_rows ? blockIdx.x / units : blockIdx.x % tiles);
+    const int kv_head = unit / A.splits, split = unit % A.splits;
 
     const kv_seq s = kv_seq_of(A.b, A.page_size, seq);
     if (!s.ok) {
