@@ -770,6 +770,11 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
     volatile int *const gone = &stop;
+    // Q of 256 columns on its way to tensor memory: through shared memory, or (a
+    // row cut into parts, where all blocks run at once) each row's thread reads
+    // it. 2,048 tokens of 2,048, 24 heads: 64 us and 69; 128 tokens over 8,192, in
+    // five parts: 60 us and 45, the tiles then taking 2,200 clocks for 1,240.
+    const bool q_tma = !C::Q_TMEM || A.splits == 1;
 
     // A row of scores lives in registers: the softmax warps take the others'
     // share (384 threads of 168 at launch: 256 of 208 and 128 of 80 are no more).
@@ -785,7 +790,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         uint8_t *const ring = is_v ? v_sm : k_sm;
         uint64_t *const full = is_v ? v_full : k_full, *const empty = is_v ? v_empty : k_empty;
         const int slots = is_v ? VS : KS;
-        if (!is_v && n > 0 && lane == 0) {
+        if (!is_v && q_tma && n > 0 && lane == 0) {
             mbar_arrive_expect_tx(&q_in, nq * (DP / 64) * per_tile * A.group * 128);
             for (int q = 0; q < nq; q++)
                 for (int c = 0; c < DP / 64; c++)
@@ -806,7 +811,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         for (; i < n; i++) {
             const int next = entry(i + 1);  // looked at a tile later
             if (i >= slots && !wait_soon(&empty[at], phase, gone, A.err)) break;
-            if (C::Q_TMEM && is_v && i == 1 && !wait_soon(&q_full, 0, gone, A.err)) break;  // Q has left the slots
+            if (C::Q_TMEM && q_tma && is_v && i == 1 && !wait_soon(&q_full, 0, gone, A.err)) break;  // Q has left the slots
             if (lane == 0) mbar_arrive_expect_tx(&full[at], C::KV_BYTES);
             __syncwarp();
             if (has) {
@@ -827,7 +832,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         // the last copies land before the block ends, whatever the others do
         for (int k = max(0, i - slots); k < i; k++)
             mbar_wait_bounded(&full[k % slots], (k / slots) & 1, nullptr, WAIT_LIMIT_NS);
-        if (!is_v && n > 0) mbar_wait_bounded(&q_in, 0, nullptr, WAIT_LIMIT_NS);
+        if (!is_v && q_tma && n > 0) mbar_wait_bounded(&q_in, 0, nullptr, WAIT_LIMIT_NS);
     } else if (warp == W_QK || warp == W_PV) {
         // The scores' MMAs and the products' by a warp each: a wait or a commit
         // takes 100 to 250 clocks before the next MMA issues, and the tensor
@@ -912,18 +917,23 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         const int i0 = max(0, sp.clo - from + BN - 1) / BN, i1 = max(0, min(sp.chi, to) - from) / BN;
         bool ok = q < nq;
         if (C::Q_TMEM && n > 0) {  // the row of Q, two values a column
-            ok = wait_soon(&q_in, 0, gone, A.err);
+            if (q_tma) ok = wait_soon(&q_in, 0, gone, A.err);
             if (ok) {
+                const uint8_t *const staged = q_sm + row * 128;
+                const uint16_t *const src =
+                    A.q + (s.q0 + (int64_t) (valid ? t : 0)) * A.ldq + (kv_head * A.group + (valid ? row % A.group : 0)) * A.d;
+                uint32_t x[DP / 64][32];  // all loads under way at once
 #pragma unroll
-                for (int c = 0; c < DP / 64; c++) {
-                    uint32_t x[32];
-#pragma unroll
-                    for (int u = 0; u < 8; u++) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(q_sm + c * (128 * 128) + row * 128 + ((u ^ (row & 7)) << 4));
-                        x[4 * u] = w.x, x[4 * u + 1] = w.y, x[4 * u + 2] = w.z, x[4 * u + 3] = w.w;
-                    }
-                    tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + c * 32, x);
+                for (int c = 0; c < DP; c += 8) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (q_tma) w = *reinterpret_cast<const uint4 *>(staged + c / 64 * (128 * 128) + ((c / 8 ^ row) % 8 << 4));
+                    else if (c < A.d) w = *reinterpret_cast<const uint4 *>(src + c);
+                    uint32_t *const at = &x[c / 64][c % 64 / 2];
+                    at[0] = w.x, at[1] = w.y, at[2] = w.z, at[3] = w.w;
                 }
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < DP / 64; c++) tmem_st_32x32b_x32(tmem + lanes + C::Q_COL + c * 32, x[c]);
                 tmem_st_wait();
                 tc_fence_before();
                 fence_proxy_async_shared();
@@ -996,7 +1006,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                         top[k] = max3_nan(top[k], __uint_as_float(x[c][e + k]), __uint_as_float(x[c][e + 4 + k]));
             float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * A.scale_log2;
             float base = m == -INFINITY ? 0.0f : -m;
-            const bool rose = !(mx <= m + LAZY);  // or NaN
+            // or NaN; a row past the last holds what lay there and moves no other's
+            const bool rose = valid && !(mx <= m + LAZY);
             if (__any_sync(0xffffffffu, rose)) {
                 if (i > 0 && NP > 1) {  // and the last product into o
                     if (!(ok = wait_soon(&pv_done[q][(i - 1) % NP], ((i - 1) / NP) & 1, gone, A.err))) break;

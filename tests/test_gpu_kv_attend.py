@@ -326,6 +326,21 @@ def test_the_same_bits_every_time():
         assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, c.q), first)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_past_the_last_move_no_bits(d):
+    """A tile's rows past its tokens, or past its sequence's, hold what lay there: nothing of it shows."""
+    c = Case([(50, 900), (45, 400)], 12, 2, d, 64, BF, seed=d)  # 6 heads a kv head: 126 of a tile's 128 rows
+    first = Z.kv_attend(c.cache, 0, c.batch, c.q).clone()
+    c.check(first)
+    loud = Case([(128, 600)] * 8, 64, 4, d, 64, BF, seed=1)  # every row of every tile
+    for gain in (300.0, 3e4):
+        Z.kv_attend(loud.cache, 0, loud.batch, (loud.q.float() * gain).to(BF))
+        assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, c.q), first)
+        q = c.q.clone()
+        q[50:] = (q[50:].float() * gain).to(BF)
+        assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, q)[:50], first[:50])
+
+
 @pytest.mark.parametrize("n", [1, 200])
 def test_offsets_past_32_bits(n):
     """A pool of more than 2^32 values whose sequences lie at its end."""
