@@ -193,7 +193,9 @@ constexpr int FEW_THREADS = 160;  // four warps of products, one that copies
 // box where it is whole blocks: a box costs the TMA unit about 45 clocks
 // besides 2 a row, and 32 sequences in pages of 16 took 142 us with a box a
 // block); warps 0-3 take 16 keys of a stage each, with a running m, l and o of
-// their own, joined at the end.
+// their own, joined at the end. Bound by HBM: 32 tokens over up to 8,192 keys
+// (8 kv heads of 128, pages of 16) 119 us, 5.5 TB/s; one over 131,072 88 us, 6.0
+// TB/s; over 1,000 by its latencies, 10.5 us.
 template <int DP, bool F16>
 __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid_constant__ CUtensorMap tk,
                                                                     const __grid_constant__ CUtensorMap tv,
@@ -562,7 +564,14 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
 // while these take their exponentials, and the tensor cores and the
 // exponential units both work throughout. (A buffer of each tile's own, with P
 // over it as the first form had it, holds the next scores back until P has
-// been used: 229 us where this takes 199 for 2,048 tokens over 8,192.)
+// been used: 229 us where this took 199 for 2,048 tokens over 8,192.)
+// Measured: 2,048 tokens, 32 heads of 128 on 8, over 8,192 190 us (1,260
+// TFLOP/s), over 32,768 900 us (1,190, at the power limit: 1.6 GHz); 24 heads of
+// 256 on 4 over themselves 65-70 us; ragged prompts of up to 700 tokens, 32
+// heads of 64: 61 us. A tile takes 2,600 clocks at 128 columns, where its MMAs
+// take 2,048: the exponentials and their conversions (2,150 of two warps a
+// scheduler) and a tile's first loads from TMEM bound it; a block pays 6 to 8 us
+// besides for its set-up, its first tiles' way and its results.
 template <int DP>
 struct many_rows {
     static constexpr int NQ = DP == 256 ? 1 : 2;    // query tiles of a block
@@ -694,8 +703,8 @@ __device__ __forceinline__ void weights(const uint32_t *x, float scale, float ba
 
 // A block: NQ x 128 rows of one kv head of one sequence over one chunk of
 // keys. S = Q K^T into TMEM; each softmax thread owns a row: it takes the
-// row's scores from TMEM, keeps m and l, and leaves the weights P in TMEM over
-// the scores, from where O += P V takes them as its A operand. O stays in TMEM
+// row's scores from TMEM, keeps m and l, and leaves the weights P in TMEM, from
+// where O += P V takes them as its A operand. O stays in TMEM
 // and is touched by the threads only when a row's maximum rises by more than
 // 2^8, and at the end.
 template <int DP, bool F16>
@@ -1106,7 +1115,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     if (!whole) {
                         // unnormalised to the workspace, whose rows have room for DP
                         // values: 32 columns at a time, a line of a row by 8 lanes
-                        // (a row a lane took 8,700 clocks where this takes XXX)
+                        // (128 tokens over 8,192, heads of 128: 36 us with a row a lane, 32 so)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             __syncwarp();
