@@ -15,7 +15,6 @@ from pathlib import Path
 import torch
 
 own = False
-_zest = None
 
 EPS, ROPE_BASE = 1e-6, 1e6
 TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
@@ -218,15 +217,11 @@ def run(state):
 
 
 def _library():
-    """The library's binding, imported once as a program does."""
-    global _zest
-    if _zest is None:
-        path = str(Path(__file__).resolve().parents[1] / "ggml-xdna_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import zest_b200
-        _zest = zest_b200
-    return _zest
+    path = str(Path(__file__).resolve().parents[1] / "ggml-xdna_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import zest_b200
+    return zest_b200
 
 
 def _run_own(s):
