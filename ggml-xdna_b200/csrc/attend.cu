@@ -983,27 +983,32 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     for (int e = 0; e < 32; e++)
                         if (c * 32 + e >= z) x[c][e] = 0xff800000u;
                 // keys that not every row of the block sees: their NaN and
-                // infinities out of the tile of values (add_not_finite)
-                if (!(ok = wait_soon(&v_full[i % VS], (i / VS) & 1, gone, A.err))) break;
-                uint8_t *vt = v_sm + i % VS * C::KV_BYTES;
-                const int c0 = sp.clo - key0, c1 = min(sp.chi, to) - key0;
-                bool found = false;
+                // infinities out of the tile of values (add_not_finite). The
+                // first query tile's warps do it for both: its product goes
+                // before the second's, so every row's waits on its own product
+                // put the cleaned tile and the flag before what it reads
+                if (q == 0) {
+                    if (!(ok = wait_soon(&v_full[i % VS], (i / VS) & 1, gone, A.err))) break;
+                    uint8_t *vt = v_sm + i % VS * C::KV_BYTES;
+                    const int c0 = sp.clo - key0, c1 = min(sp.chi, to) - key0;
+                    bool found = false;
 #pragma unroll 4
-                for (int e = row; e < C::KV_BYTES / 16; e += 128) {
-                    const int key = e / 8 % BN;
-                    uint4 w = *reinterpret_cast<uint4 *>(vt + e * 16);
-                    if ((key >= c0 && key < c1) || !any_bad<F16>(w)) continue;
-                    uint32_t h[4] = { w.x, w.y, w.z, w.w };
+                    for (int e = row; e < C::KV_BYTES / 16; e += 128) {
+                        const int key = e / 8 % BN;
+                        uint4 w = *reinterpret_cast<uint4 *>(vt + e * 16);
+                        if ((key >= c0 && key < c1) || !any_bad<F16>(w)) continue;
+                        uint32_t h[4] = { w.x, w.y, w.z, w.w };
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (bad_half<F16>(h[k])) h[k] &= 0xffff0000u;
-                        if (bad_half<F16>(h[k] >> 16)) h[k] &= 0x0000ffffu;
+                        for (int k = 0; k < 4; k++) {
+                            if (bad_half<F16>(h[k])) h[k] &= 0xffff0000u;
+                            if (bad_half<F16>(h[k] >> 16)) h[k] &= 0x0000ffffu;
+                        }
+                        *reinterpret_cast<uint4 *>(vt + e * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                        found |= key0 + key < to;
                     }
-                    *reinterpret_cast<uint4 *>(vt + e * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-                    found |= key0 + key < to;
+                    if (found) not_finite = 1;
+                    fence_proxy_async_shared();
                 }
-                if (found) not_finite = 1;
-                fence_proxy_async_shared();
             }
             float top[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll

@@ -193,6 +193,23 @@ def test_values_a_row_does_not_see_do_not_reach_it(d, lens, window, bad):
     assert torch.isfinite(got[rest]).all()
 
 
+@pytest.mark.parametrize("d,lens,window", [(128, [(64, 64)], 0), (64, [(64, 640)], 0), (96, [(61, 200), (64, 70)], 30),
+                                           (128, [(64, 6000)], 0)])
+def test_not_finite_values_in_the_last_tile_of_two_query_tiles(d, lens, window):
+    """A block's two query tiles of 32 tokens over one tile of values with NaN and infinities that the first rows of
+    either, or all of one, do not see: every row gets what it sees, call after call."""
+    c = Case(lens, 8, 2, d, 16, BF, seed=17)
+    for s, (n, kv) in enumerate(lens):
+        for x, back in enumerate((1, 2, 17, 30, 33, 48, 60)):
+            p = kv - back
+            c.v[0, c.rows[s][p // 16], p % 16, x % 2, 5 * x] = (math.nan, math.inf, -math.inf)[x % 3]
+    first = Z.kv_attend(c.cache, 0, c.batch, c.q, window=window)
+    c.check(first, True, window)
+    for _ in range(50):
+        assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, c.q, window=window).view(torch.int16),
+                           first.view(torch.int16))
+
+
 @pytest.mark.parametrize("d", [64, 128, 96, 256])
 @pytest.mark.parametrize("n,window", [(1, 50), (3, 77), (40, 30), (150, 100)])
 def test_pages_behind_the_window_may_be_gone(n, window, d):
