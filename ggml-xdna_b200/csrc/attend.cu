@@ -154,6 +154,15 @@ __device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr));
 }
 
+// One lane arrives for a warp whose lanes have all come this far. They are
+// together again behind it: warp-wide (.aligned) instructions want that, and a
+// branch that one lane takes does not promise it by itself.
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    __syncwarp();
+}
+
 // 2^x by the hardware's approximation (relative error about 2^-22).
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -281,11 +290,10 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         // the last copies land before the block ends, whatever the others do
         for (int k = max(0, i - C::STAGES); k < i; k++)
             mbar_wait_bounded(&full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, WAIT_LIMIT_NS);
+        __syncwarp();
         __syncthreads();
         if (A.join > 1) {
-            __syncwarp();
             cluster_sync();
-            __syncwarp();
             cluster_sync();
         }
         return;
@@ -332,6 +340,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         if (!mbar_wait_bounded(&full[st], (i / C::STAGES) & 1, (volatile int *) &stop, WAIT_LIMIT_NS)) {
             timeout = true;
         }
+        __syncwarp();
         if (__any_sync(0xffffffffu, timeout)) {
             if (lane == 0) {
                 stop = 1;
@@ -367,6 +376,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
                     const int64_t key = key0 + n * 8 + tq * 2 + (e & 1);
                     if (key < lo[e >> 1] || key >= hi[e >> 1] || key >= to) sc[n][e] = -INFINITY;
                 }
+            __syncwarp();
         }
         float f[2];
         bool moved = false;
@@ -427,15 +437,16 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
                                 bad |= k < to;
                             }
                         }
+                    __syncwarp();
                 }
                 mma16816<F16>(o[j], p, b[0], b[1]);
                 mma16816<F16>(o[j + 1], p, b[2], b[3]);
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        warp_arrive(&empty[st]);
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) not_finite = 1;
+    __syncwarp();
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
@@ -458,6 +469,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
             m_sh[warp][g + 8 * e] = m[e];
             l_sh[warp][g + 8 * e] = l[e];
         }
+    __syncwarp();
     named_barrier(1, 128);
     const int row = threadIdx.x >> 3;
     float mx = -INFINITY, w[4], sum = 0.0f;
@@ -643,6 +655,7 @@ __device__ __forceinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile
         ok = mbar_try_wait(bar, parity);
         if (!ok && (it & 63u) == 0 && (*gone || global_ns() - t0 > WAIT_LIMIT_NS)) break;
     }
+    __syncwarp();
     if (__all_sync(0xffffffffu, ok)) return true;
     *gone = 1;
     atomicOr(err, ERR_TIMEOUT);
@@ -770,6 +783,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
         not_finite = 0;
         fence_barrier_init();
     }
+    __syncwarp();
     if (warp == W_QK) {
         tmem_alloc(&tmem_sh, C::COLS);
         tmem_relinquish();
@@ -946,8 +960,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 tmem_st_wait();
                 tc_fence_before();
                 fence_proxy_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full);
+                warp_arrive(&q_full);
             }
         }
         float m = -INFINITY, l = 0.0f;
@@ -960,8 +973,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 #pragma unroll
             for (int c = 0; c < BN / 32; c++) tmem_ld_wait(x[c]);
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free);
+            warp_arrive(&s_free);
             // the last product of P's buffer is done: P may go
             if (i >= NP) {
                 if (!(ok = wait_soon(&pv_done[q][i % NP], (i / NP - 1) & 1, gone, A.err))) break;
@@ -1009,6 +1021,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     if (found) not_finite = 1;
                     fence_proxy_async_shared();
                 }
+                __syncwarp();
             }
             float top[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
@@ -1054,8 +1067,7 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                 tmem_st_32x32b_x32(tmem + lanes + C::P_COL + (q * NP + i % NP) * (BN / 2) + h * 32, p);
                 tmem_st_wait();
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[q][i % NP][h]);
+                warp_arrive(&p_full[q][i % NP][h]);
             }
             float sa, sb;
             unpack2(add2(s0, s1), sa, sb);
