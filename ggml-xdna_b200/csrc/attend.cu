@@ -49,7 +49,7 @@ struct attend_args {
     int join;           // few rows: blocks of a cluster, each with an equal part of the keys (then splits is 1)
     int by_rows;        // many rows: every head's last rows first, not one head's after another's
     int wide;           // few rows: a box has a head's columns whole
-    float2 *ml;         // [splits][T * heads]: m and l
+    float2 *ml;         // [splits][T * heads]: m and l (m NaN: a wait ran out and the part is none)
     float *part;        // [splits][T * heads][DP]: o
     unsigned *err;
 };
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(FEW_THREADS) kv_attend_few_kernel(const __grid
         }
     }
     if (A.join == 1) {
-        if (live && A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(mx, sum);
+        if (row < rows && A.splits > 1 && (threadIdx.x & 7) == 0) A.ml[slot] = make_float2(stop ? NAN : mx, sum);
         return;
     }
     // the cluster's chunks joined in order, the rows' columns dealt to its blocks
@@ -1078,9 +1078,9 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
             ok = wait_soon(&pv_done[q][(n - 1) % NP], ((n - 1) / NP) & 1, gone, A.err);
             tc_fence_after();
         }
+        const int head = kv_head * A.group + row % A.group;
+        const int64_t tok = s.q0 + (int64_t) t;
         if (ok) {
-            const int head = kv_head * A.group + row % A.group;
-            const int64_t tok = s.q0 + (int64_t) t, slot = split * (A.b.T * A.heads) + tok * A.heads + head;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             if (not_finite) {
 #pragma unroll 1
@@ -1198,8 +1198,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
                     }
                 }
             }
-            if (A.splits > 1 && valid) A.ml[slot] = make_float2(m, l);
         }
+        if (A.splits > 1 && valid) A.ml[split * (A.b.T * A.heads) + tok * A.heads + head] = make_float2(ok ? m : NAN, l);
     }
     tc_fence_before();
     __syncthreads();
@@ -1211,7 +1211,8 @@ __global__ void __launch_bounds__(many_rows<DP>::THREADS, 1)
 
 // The parts of each row joined in order, eight columns a thread. Few rows: the
 // block's groups of threads take every GROUPS-th part of one row and meet in
-// shared memory, so that 37 parts cost five loads one after another.
+// shared memory, so that 37 parts cost five loads one after another. A row one
+// of whose parts is none (m is NaN, which no maximum is) stays as it was.
 template <int DP, bool F16, bool FEW>
 __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__ attend_args A, int tile_rows) {
     constexpr int PER_ROW = DP / 8, GROUPS = 128 / PER_ROW;
@@ -1233,7 +1234,12 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
     const int64_t tok = s.q0 + (int64_t) t, stride = A.b.T * A.heads, slot = tok * A.heads + head;
     float mx = -INFINITY, sum = 0.0f, x[8] = {};
     const int first = FEW ? group : 0, step = FEW ? GROUPS : 1;
-    for (int i = first; i < n; i += step) mx = fmaxf(mx, A.ml[i * stride + slot].x);
+    bool whole = true;
+    for (int i = first; i < n; i += step) {
+        const float m = A.ml[i * stride + slot].x;
+        whole = whole && m == m;
+        mx = fmaxf(mx, m);
+    }
 #pragma unroll 4
     for (int i = first; i < n; i += step) {
         const float2 ml = A.ml[i * stride + slot];
@@ -1248,13 +1254,17 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
     if (FEW) {
         __shared__ float sh[GROUPS][DP + 4];
         __shared__ float2 ml_sh[GROUPS];
-        if (c == 0) ml_sh[group] = make_float2(mx, sum);
+        if (c == 0) ml_sh[group] = make_float2(whole ? mx : NAN, sum);
 #pragma unroll
         for (int e = 0; e < 8; e++) sh[group][c + e] = x[e];
         __syncthreads();
         if (group > 0 || c >= A.d) return;
         float top = -INFINITY;
-        for (int g = 0; g < GROUPS; g++) top = fmaxf(top, ml_sh[g].x);
+        whole = true;
+        for (int g = 0; g < GROUPS; g++) {
+            whole = whole && ml_sh[g].x == ml_sh[g].x;
+            top = fmaxf(top, ml_sh[g].x);
+        }
         sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = 0.0f;
@@ -1265,6 +1275,7 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(const __grid_constant__
             for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(sh[g][c + e], w, x[e]);
         }
     }
+    if (!whole) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] *= inv;

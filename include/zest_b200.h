@@ -289,7 +289,9 @@ int zest_norm_rope(const float *x, int64_t T, int64_t heads, int64_t d, float ep
  *
  * err is a device word that the kernels OR ZEST_ERR_* bits into (the caller
  * clears it). A sequence or a page that is out of bounds is never read or
- * written: it raises a bit, and what was asked of it is not done.
+ * written: it raises a bit, and what was asked of it is not done. A wait inside
+ * the attention that runs out raises ZEST_ERR_TIMEOUT, and the rows that it
+ * kept from being made stay as they were.
  * ------------------------------------------------------------------------- */
 #define ZEST_TYPE_BF16 30        /* with ZEST_TYPE_F16: the types of a cache (ggml_type ids) */
 #define ZEST_ERR_BAD_PAGE 4u     /* a page number outside the cache where a page was needed */

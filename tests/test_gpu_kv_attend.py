@@ -336,6 +336,40 @@ def test_captured_replayed_and_beside_another_stream():
             c.check(out)
 
 
+@pytest.mark.parametrize("d,lens", [(128, [(1, 3000)]), (64, [(2, 5000), (1, 2000)]), (128, [(40, 6000)]),
+                                    (256, [(30, 5000)])])
+def test_a_row_with_a_part_that_never_came_stays(d, lens):
+    """A block whose wait runs out marks its part of a row with a maximum of NaN. Such marks set by hand between the
+    two kernels of a captured call, the first of them turned off: the join leaves those rows, and makes the others."""
+    from cuda.bindings import runtime as rt
+
+    c = Case(lens, 8, 2, d, 16, BF, seed=19)
+    out, err = torch.zeros_like(c.q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    Z.kv_attend(c.cache, 0, c.batch, c.q, out=out, err=err, workspace=ws)
+    good = out.clone()
+    c.check(good)
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        Z.kv_attend(c.cache, 0, c.batch, c.q, out=out, err=err, workspace=ws)
+    handle = rt.cudaGraph_t(g.raw_cuda_graph())
+    n = rt.cudaGraphGetNodes(handle, 0)[2]
+    assert n == 2, "the keys are cut: the attention, and the join of its parts"
+    e, roots, _ = rt.cudaGraphGetRootNodes(handle, 1)
+    assert int(e) == 0
+    g.instantiate()
+    assert int(rt.cudaGraphNodeSetEnabled(rt.cudaGraphExec_t(g.raw_cuda_graph_exec()), roots[0], 0)[0]) == 0
+    ml = ws.view(torch.float32)
+    rows, missing = c.T * c.heads, torch.zeros(c.T, c.heads, dtype=torch.bool, device="cuda")
+    for part, t, head in ((0, 0, 1), (1, c.T - 1, 6)):
+        ml[2 * (part * rows + t * c.heads + head)] = math.nan
+        missing[t, head] = True
+    out.fill_(5.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out[missing] == 5).all() and torch.equal(out[~missing], good[~missing]) and int(err) == 0
+
+
 def test_the_same_bits_every_time():
     c = Case([(1, 3000), (1, 50)], 8, 2, 128, 16, BF, seed=1)
     first = Z.kv_attend(c.cache, 0, c.batch, c.q)
