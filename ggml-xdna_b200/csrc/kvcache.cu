@@ -529,17 +529,48 @@ __global__ void __launch_bounds__(PG_THREADS) kv_fork_kernel(const __grid_consta
     if (i < A.n) A.out.len[sh.who[i]] = len;
 }
 
+// Whether one of the table's entries that thread `at` of `step` looks at is no
+// page of the pool (an entry below zero holds none).
+__device__ __forceinline__ bool no_page(const pages_args &A, int64_t at, int64_t step) {
+    const int64_t n = A.in.seqs * A.in.table_stride, n4 = ((uintptr_t) A.in.table & 15) ? 0 : n / 4;
+    bool bad = false;
+#pragma unroll 4
+    for (int64_t i = at; i < n4; i += step) {
+        const int4 p = reinterpret_cast<const int4 *>(A.in.table)[i];
+        bad |= max(max(p.x, p.y), max(p.z, p.w)) >= A.pages;
+    }
+    for (int64_t i = 4 * n4 + at; i < n; i += step) bad |= A.in.table[i] >= A.pages;
+    return bad;
+}
+
+// Tables that one block would take longer over than a launch costs are looked
+// over by many, ahead of the plan: what they find in ws[0], cleared before.
+constexpr int64_t CHECKED_APART = 1 << 16;
+
+__global__ void __launch_bounds__(256) kv_check_table_kernel(const __grid_constant__ pages_args A) {
+    if (no_page(A, blockIdx.x * (int64_t) blockDim.x + threadIdx.x, (int64_t) gridDim.x * blockDim.x)) A.ws[0] = 1;
+}
+
 // ws: count of moves, (from, to) pairs, and behind 1 + 2 * pages the new
 // number of each page. The table is rewritten by the copying kernel, whose
-// many blocks suit its size.
+// many blocks suit its size. An entry that is no page: nothing moves, and every
+// page keeps its number.
 __global__ void __launch_bounds__(PG_THREADS) kv_compact_kernel(const __grid_constant__ pages_args A) {
     __shared__ pages_shared sh;
+    const bool apart = A.in.seqs * A.in.table_stride > CHECKED_APART;
+    const bool bad = apart ? A.ws[0] != 0 : no_page(A, threadIdx.x, PG_THREADS);
     copy_values(A.out.refs, A.in.refs, A.pages);
     copy_values(A.out.len, A.in.len, A.in.seqs);
     int32_t *map = A.ws + 1 + 2 * A.pages;
     const int64_t all = A.pages;
     for (int64_t i = threadIdx.x; i < all; i += blockDim.x) map[i] = (int32_t) i;
-    __syncthreads();
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) {
+            atomicOr(A.err, ZEST_ERR_BAD_PAGE);
+            A.ws[0] = 0;
+        }
+        return;
+    }
     const int64_t live = each_page(A.out.refs, 0, all, true, all, sh, [](int64_t, int64_t) {});
     const int64_t holes = each_page(A.out.refs, 0, live, false, all, sh, [&](int64_t rank, int64_t page) {
         A.ws[2 + 2 * rank] = (int32_t) page;
@@ -565,7 +596,6 @@ struct move_args {
     const int32_t *table_in;      // compact: its entries renumbered by the map (null: none)
     int32_t *table_out;
     int64_t entries;
-    unsigned *err;
 };
 
 constexpr int MV_THREADS = 256, MV_PIECE = MV_THREADS * 4;  // 16-byte vectors: 16 KB
@@ -608,14 +638,13 @@ __global__ void __launch_bounds__(MV_THREADS) kv_move_kernel(const __grid_consta
         for (int64_t e = blockIdx.x * (int64_t) MV_THREADS + threadIdx.x; e < A.entries;
              e += (int64_t) gridDim.x * MV_THREADS) {
             const int p = A.table_in[e];
-            if (p >= A.pages) atomicOr(A.err, ZEST_ERR_BAD_PAGE);
             A.table_out[e] = p >= 0 && p < A.pages ? map[p] : p;
         }
     }
 }
 
 int launch_moves(const zest_kv_cache *kv, const int32_t *ws, int64_t most, const int32_t *table_in,
-                 int32_t *table_out, int64_t entries, unsigned *err, cudaStream_t st, const char *what) {
+                 int32_t *table_out, int64_t entries, cudaStream_t st, const char *what) {
     move_args m;
     m.ws = ws;
     m.pool[0] = (uint16_t *) kv->k;
@@ -636,7 +665,6 @@ int launch_moves(const zest_kv_cache *kv, const int32_t *ws, int64_t most, const
     m.table_in = table_in;
     m.table_out = table_out;
     m.entries = entries;
-    m.err = err;
     const int64_t units = std::max<int64_t>(most * m.layers * 2 * m.pieces, (entries + MV_THREADS - 1) / MV_THREADS);
     kv_move_kernel<<<(int) std::min<int64_t>(std::max<int64_t>(units, 1), 148 * 8), MV_THREADS, 0, st>>>(m);
     return check_launch(what);
@@ -774,8 +802,7 @@ int zest_kv_fork(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_k
     kv_fork_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(a);
     if (check_launch("zest_kv_fork")) return -1;
     if (n == 0) return 0;
-    return launch_moves(kv, (const int32_t *) workspace, n, nullptr, nullptr, 0, err, (cudaStream_t) stream,
-                        "zest_kv_fork");
+    return launch_moves(kv, (const int32_t *) workspace, n, nullptr, nullptr, 0, (cudaStream_t) stream, "zest_kv_fork");
 }
 
 int zest_kv_compact(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, void *workspace,
@@ -783,11 +810,18 @@ int zest_kv_compact(const zest_kv_cache *kv, const zest_kv_tables *in, const zes
     if (const char *why = tables_fault(kv, in, out)) return kv_refuse("zest_kv_compact", why);
     if (!err) return kv_refuse("zest_kv_compact", "no device error word");
     if (!workspace || ((uintptr_t) workspace & 15)) return kv_refuse("zest_kv_compact", "no 16-byte aligned workspace");
-    kv_compact_kernel<<<1, PG_THREADS, 0, (cudaStream_t) stream>>>(
-        args_of(kv, in, out, 0, nullptr, nullptr, workspace, err));
+    const pages_args a = args_of(kv, in, out, 0, nullptr, nullptr, workspace, err);
+    const int64_t entries = in->seqs * in->table_stride;
+    cudaStream_t st = (cudaStream_t) stream;
+    if (entries > CHECKED_APART) {
+        cudaMemsetAsync(workspace, 0, 4, st);
+        kv_check_table_kernel<<<(int) std::min<int64_t>((entries / 4 + 255) / 256, 148 * 8), 256, 0, st>>>(a);
+        if (check_launch("zest_kv_compact")) return -1;
+    }
+    kv_compact_kernel<<<1, PG_THREADS, 0, st>>>(a);
     if (check_launch("zest_kv_compact")) return -1;
-    return launch_moves(kv, (const int32_t *) workspace, kv->pages / 2, in->table, out->table,
-                        in->seqs * in->table_stride, err, (cudaStream_t) stream, "zest_kv_compact");
+    return launch_moves(kv, (const int32_t *) workspace, kv->pages / 2, in->table, out->table, entries, st,
+                        "zest_kv_compact");
 }
 
 }  // extern "C"

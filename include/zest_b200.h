@@ -401,8 +401,8 @@ typedef struct {
 /* The page operations: tables `in` to tables `out` (the same, or disjoint
  * arrays of the same sizes), n sequences at once (n <= ZEST_KV_MAX_SEQS,
  * device arrays). Free pages are taken lowest number first, for the sequences
- * in the order given. On an error bit of theirs nothing changes: `out` is
- * `in`. workspace: zest_kv_pages_workspace bytes, 16-byte aligned. */
+ * in the order given. On an error bit of theirs nothing changes, in the pools
+ * neither: `out` is `in`. workspace: zest_kv_pages_workspace bytes, 16-byte aligned. */
 #define ZEST_KV_MAX_SEQS 1024
 /* Room for add[i] more tokens of sequence seq[i] (each named once). */
 int zest_kv_grow(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,

@@ -223,6 +223,29 @@ def test_page_operations_that_fail_change_nothing(fresh):
     assert int(err) == Z.ERR_BAD_PAGE and t.t.tensors[2].tolist()[1] == 0
 
 
+@pytest.mark.parametrize("pages,seqs,width", [(40, 6, 9), (40, 7000, 10)])
+@pytest.mark.parametrize("fresh", [False, True])
+def test_a_compaction_that_fails_changes_nothing(pages, seqs, width, fresh):
+    """A table with an entry that is no page, small and large enough to be looked over apart: tables and pools stay,
+    and the same call without the entry goes through."""
+    t = Tables(pages, seqs, width, 16)
+    t.step("grow", [0, 1, 5], [100, 130, 60])
+    t.step("free", [0])
+    good = t.t.tensors[1].clone()
+    for at, entry in (((3, 2), pages), ((seqs - 1, width - 1), 0x7fffffff), ((0, 0), pages + 1)):
+        t.t.tensors[1][at] = entry
+        before, k, v = [x.clone() for x in t.t.tensors], t.k.clone(), t.v.clone()
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = Z.KvTables(*(torch.full_like(x, 77) for x in t.t.tensors)) if fresh else None
+        got = Z.kv_compact(t.cache, t.t, out=out, err=err)
+        assert int(err) == Z.ERR_BAD_PAGE
+        assert all(torch.equal(a, b) for a, b in zip(before, got.tensors))
+        assert all(torch.equal(a, b) for a, b in zip(before, t.t.tensors))
+        assert torch.equal(t.k, k) and torch.equal(t.v, v)
+        t.t.tensors[1].copy_(good)
+    assert t.step("compact", fresh=fresh)
+
+
 def test_the_same_sequence_twice():
     t = Tables(30, 8, 8, 16)
     t.step("grow", [0, 1], [40, 33])
