@@ -402,7 +402,8 @@ typedef struct {
  * arrays of the same sizes), n sequences at once (n <= ZEST_KV_MAX_SEQS,
  * device arrays). Free pages are taken lowest number first, for the sequences
  * in the order given. On an error bit of theirs nothing changes, in the pools
- * neither: `out` is `in`. workspace: zest_kv_pages_workspace bytes, 16-byte aligned. */
+ * neither: `out` is `in`. Of ZEST_ERR_BAD_PAGE from zest_kv_free this does not
+ * hold (there). workspace: zest_kv_pages_workspace bytes, 16-byte aligned. */
 #define ZEST_KV_MAX_SEQS 1024
 /* Room for add[i] more tokens of sequence seq[i] (each named once). */
 int zest_kv_grow(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
@@ -412,7 +413,10 @@ int zest_kv_grow(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_k
 int zest_kv_fork(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
                  const int32_t *src, const int32_t *dst, void *workspace, unsigned *err, void *stream);
 /* Sequences seq[i] give their pages back and are empty (naming one twice
- * frees it once). */
+ * frees it once). An entry that is no page, or a page that nobody holds, is
+ * dropped and raises ZEST_ERR_BAD_PAGE; the sequences' other pages are given
+ * back and they are empty all the same, so that a row gone bad can be had rid
+ * of. */
 int zest_kv_free(const zest_kv_cache *kv, const zest_kv_tables *in, const zest_kv_tables *out, int n,
                  const int32_t *seq, unsigned *err, void *stream);
 /* The pages in use moved to the front, in every layer: with c pages in use,

@@ -246,6 +246,25 @@ def test_a_compaction_that_fails_changes_nothing(pages, seqs, width, fresh):
     assert t.step("compact", fresh=fresh)
 
 
+@pytest.mark.parametrize("fresh", [False, True])
+def test_a_row_gone_bad_is_freed(fresh):
+    """Entries that are no page, and a page nobody holds: dropped with an error bit; the rest of the row, and the
+    other sequences named, are given back."""
+    t = Tables(30, 6, 9, 16)
+    t.step("grow", [0, 1, 2], [100, 70, 40])
+    t.step("fork", [0], [4])
+    refs, table, lens = t.t.tensors
+    table[1, 1], table[1, 6], table[0, 8] = 30, 0x7fffffff, 29  # page 29 is free
+    held = t.host.table[1][1]
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = Z.KvTables(*(torch.full_like(x, 77) for x in t.t.tensors)) if fresh else None
+    got = Z.kv_free(t.cache, t.t, i32([1, 0]), out=out, err=err)
+    assert int(err) == Z.ERR_BAD_PAGE
+    t.host.free([0, 1])
+    t.host.refs[held] += 1  # its row no longer said so
+    t.agree(got)
+
+
 def test_the_same_sequence_twice():
     t = Tables(30, 8, 8, 16)
     t.step("grow", [0, 1], [40, 33])
