@@ -1458,8 +1458,8 @@ int launch_attend(const zest_kv_cache *kv, const CUtensorMap &tk, const CUtensor
         cudaLaunchKernelEx(&cfg, kv_attend_few_kernel<DP, F16>, tk, tv, a);
     }
     if (check_launch(call)) return -1;
-    if (p.splits == 1) return 0;
     const int64_t rows = a.b.max_q * a.group;
+    if (p.splits == 1 || rows == 0) return 0;  // (of no rows, the kernel above has looked for sequences that have some)
     if (p.many)
         kv_combine_kernel<DP, F16, false><<<dim3((unsigned) up(rows, 128 / (DP / 8)), kv->kv_heads, a.b.n_seqs), 128, 0, st>>>(
             a, p.tile_rows);
@@ -1494,6 +1494,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     const zest_kv_batch b = tightened(kv, batch);
     if (const char *why = attend_fault(kv, &b, at)) return kv_refuse(call, why);
     if (!err) return kv_refuse(call, "no device error word");
+    if (b.T == 0 || b.n_seqs == 0) return 0;  // nothing to read or write: whatever the pointers
     const int64_t wide = (int64_t) at->heads * kv->d;
     auto rows = [&](const void *p, int64_t ld, int64_t unit) { return ld >= wide && ld % unit == 0 && !((uintptr_t) p & 15); };
     if (!at->q || !rows(at->q, at->ldq, 8)) return kv_refuse(call, "q rows cover the heads and are 16-byte aligned");
@@ -1505,7 +1506,6 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     const int64_t need = p.ws_ml + p.ws_part;
     if (need > 0 && (!workspace || ((uintptr_t) workspace & 15) || (int64_t) workspace_bytes < need))
         return kv_refuse(call, "the workspace is smaller than zest_kv_attend_workspace says, or not 16-byte aligned");
-    if (b.T == 0 || b.n_seqs == 0 || b.max_q == 0) return 0;
     const int64_t off = kv->layers > 1 ? layer * kv->layer_stride : 0;
     CUtensorMap tk, tv;
     if (!pool_tmap(&tk, kv, (const uint16_t *) kv->k + off, p.wide) ||

@@ -235,6 +235,22 @@ def test_bounds_as_wide_as_they_go():
         c.check(Z.kv_attend(c.cache, 0, b, c.q, window=(1 << 62)))
 
 
+def test_a_step_of_no_rows():
+    """Empty tensors through the binding; and a bound of no rows that a sequence passes."""
+    c = Case([(0, 200), (0, 0), (0, 70)], 8, 2, 128, 16, BF, seed=23)
+    assert c.q.shape == (0, 8, 128) and Z.kv_attend(c.cache, 0, c.batch, c.q).shape == c.q.shape
+    y = torch.empty(0, 8 * 128, device="cuda")
+    assert Z.kv_attend(c.cache, 0, c.batch, c.q, y=y) is y
+    rows = torch.empty(0, 2, 128, device="cuda")
+    Z.kv_append(c.cache, 0, c.batch, rows, rows)
+    for lens in ([(1, 200)], [(0, 3000), (1, 3000)]):
+        c = Case(lens, 8, 2, 128, 16, BF, seed=24)
+        out, err = torch.full_like(c.q, 5.0), torch.zeros(1, dtype=torch.int32, device="cuda")
+        b = Z.KvBatch(c.q_start, c.kv_len, c.table, T=c.T, max_q=0, max_kv=c.max_kv)
+        Z.kv_attend(c.cache, 0, b, c.q, out=out, err=err)
+        assert int(err) == Z.ERR_BAD_SEQ and (out == 5).all()
+
+
 def test_a_first_call_that_is_captured():
     """A process whose first calls are captured: nothing is set up that a capture forbids."""
     code = """

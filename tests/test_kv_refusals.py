@@ -146,3 +146,11 @@ def test_page_operations():
     refused(calls["fork"](b=0), "no sequence numbers")
     assert L.zest_kv_pages_workspace(ref(c)) >= 4 * (1 + 3 * 10)
     refused(L.zest_kv_pages_workspace(None), "no cache")
+
+
+def test_a_step_of_no_rows_is_no_call():
+    """As an empty tensor comes: no pointers, and nothing to do."""
+    for b in (batch(T=0, max_q=0), batch(T=0), batch(n=0, T=0, q_start=0, kv_len=0, table=0, stride=0)):
+        assert attend(b=b, a=attn(q=0, ldq=0, out=0, ldo=0)) == 0
+        assert append(b=b, i=new(k=0, v=0, ldk=0, ldv=0, q=0, q_out=0)) == 0
+        refused(attend(b=b, a=attn(heads=12)), "multiple of the kv heads")
