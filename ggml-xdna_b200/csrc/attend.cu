@@ -1525,7 +1525,7 @@ int zest_kv_attend(const zest_kv_cache *kv, int64_t layer, const zest_kv_batch *
     a.d = kv->d;
     a.page_size = kv->page_size;
     a.causal = at->causal != 0;
-    a.window = at->window;
+    a.window = std::min(at->window, int64_t(1) << 32);  // wider than any sequence is as wide as it gets
     a.scale_log2 = at->scale * LOG2E;
     a.out = (uint16_t *) at->out;
     a.ldo = at->ldo;

@@ -77,9 +77,10 @@ inline const char *kv_cache_fault(const zest_kv_cache *c, int64_t layer) {
 inline const char *kv_batch_fault(const zest_kv_batch *b) {
     if (!b) return "no batch";
     if (b->n_seqs < 0 || b->n_seqs > 65535) return "0 to 65535 sequences";
-    if (b->T < 0 || b->T > 0x7fffffff || b->max_q < 0 || b->max_q > 0x7fffffff || b->max_kv < 0 ||
-        b->max_kv > 0x7fffffff - 4096)
-        return "row and token counts below 2^31";
+    // the kernels count rows and keys in 32 bits, up to a tile past the last
+    const int64_t most = 0x7fffffff - 4096;
+    if (b->T < 0 || b->T > most || b->max_q < 0 || b->max_q > 0x7fffffff || b->max_kv < 0 || b->max_kv > most)
+        return "row and token counts below 2^31 - 4096";
     if (b->n_seqs > 0 && (!b->q_start || !b->kv_len)) return "no q_start or kv_len";
     if (b->table_stride < 0 || b->table_stride > 0x7fffffff || (b->n_seqs > 0 && b->table_stride > 0 && !b->table))
         return "no page table";

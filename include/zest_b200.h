@@ -321,7 +321,7 @@ typedef struct {
     const int32_t *kv_len;      /* [n_seqs] */
     const int32_t *table;       /* [n_seqs][table_stride] */
     int64_t table_stride;
-    int64_t T;
+    int64_t T;                  /* below 2^31 - 4096, as max_kv */
     int64_t max_q, max_kv;      /* no sequence has more new tokens, or holds more (host-side bounds that the
                                    launch is shaped by; a longer sequence raises ZEST_ERR_BAD_SEQ) */
     int n_seqs;                 /* at most 65535 */

@@ -235,6 +235,13 @@ def test_bounds_as_wide_as_they_go():
         c.check(Z.kv_attend(c.cache, 0, b, c.q, window=(1 << 62)))
 
 
+@pytest.mark.parametrize("lens", [[(6, 3), (2, 60)], [(90, 20), (30, 200)]])
+def test_the_widest_window(lens):
+    """2^63 - 1, over rows before the first key too: the causal mask alone."""
+    c = Case(lens, 8, 2, 128, 16, BF, seed=25)
+    c.check(Z.kv_attend(c.cache, 0, c.batch, c.q, window=(1 << 63) - 1))
+
+
 def test_a_step_of_no_rows():
     """Empty tensors through the binding; and a bound of no rows that a sequence passes."""
     c = Case([(0, 200), (0, 0), (0, 70)], 8, 2, 128, 16, BF, seed=23)

@@ -154,3 +154,10 @@ def test_a_step_of_no_rows_is_no_call():
         assert attend(b=b, a=attn(q=0, ldq=0, out=0, ldo=0)) == 0
         assert append(b=b, i=new(k=0, v=0, ldk=0, ldv=0, q=0, q_out=0)) == 0
         refused(attend(b=b, a=attn(heads=12)), "multiple of the kv heads")
+
+
+@pytest.mark.parametrize("call", [attend, append])
+def test_counts_whose_tiles_pass_32_bits(call):
+    """A sequence of 2^31 - 1 rows: its last tile's rows would be counted past 2^31."""
+    for kw in (dict(T=0x7fffffff, max_q=0x7fffffff), dict(T=0x7fffffff - 4095), dict(max_kv=0x7fffffff - 4095)):
+        refused(call(b=batch(**kw)), "2^31")
