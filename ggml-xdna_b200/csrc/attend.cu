@@ -185,7 +185,8 @@ __device__ __forceinline__ bool any_bad(const uint4 &w) {
     return (((w.x & m) + one) | ((w.y & m) + one) | ((w.z & m) + one) | ((w.w & m) + one)) & 0x80008000u;
 }
 
-// A stage's bytes, and as many stages as keep about 64 KB in flight on an SM.
+// A stage's bytes, and as many stages as fill an SM with its 3, 2 or 1 blocks
+// (by padded head size): 192 KB of keys and values in flight or in use.
 template <int DP>
 struct few_rows {
     static constexpr int HALF = KEYS * DP * 2;  // K or V of a stage
@@ -689,7 +690,11 @@ __device__ __forceinline__ void exp2_poly(float &u, float &w) {
 }
 
 // The weights of 64 keys: x in as bits of scores, 2^(x scale + base) rounded to
-// the cache's type into p, their f32 sums into s0 and s1. One pair of eight by
+// the cache's type into p, their f32 sums into s0 and s1. Rounded because the
+// MMA takes both operands in 16 bits of one type: half a step of each weight,
+// 1.4 times the distance from 64-bit arithmetic that one rounding of the result
+// has (bf16 2.35e-3 against 1.66e-3); l sums the weights before that rounding,
+// whose errors have no bias for it to share. One pair of eight by
 // polynomial: the exponential unit (16 a clock and SM) is what the rows wait
 // for. Clocks for 128 keys of a warp alone and of two warps a scheduler, with
 // the maximum before: 1,676 and 2,334 with none, 1,536 and 2,146 with one of

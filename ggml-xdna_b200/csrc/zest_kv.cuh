@@ -33,14 +33,8 @@ __device__ __forceinline__ kv_seq kv_seq_of(const zest_kv_batch &b, int page_siz
     return kv_seq_from(b, page_size, b.q_start[s], b.q_start[s + 1], b.kv_len[s]);
 }
 
-// The bits of x rounded once (nearest even) to the cache's type. fp16 values
-// past 65504 become infinite, as the format's rounding has it.
-template <bool F16>
-__device__ __forceinline__ uint16_t kv_bits(float x) {
-    if (F16) return __half_as_ushort(__float2half_rn(x));
-    return bf16_bits_rne(x);
-}
-
+// The bits of lo and hi, each rounded once (nearest even) to the cache's type.
+// fp16 values past 65504 become infinite, as the format's rounding has it.
 template <bool F16>
 __device__ __forceinline__ uint32_t kv_bits2(float lo, float hi) {
     uint32_t p;
