@@ -152,6 +152,37 @@ def test_long_keys_are_cut_and_joined(lens, heads_first):
     c.check(Z.kv_attend(c.cache, 0, wide, c.q))
 
 
+@pytest.mark.parametrize("dt,d,kv_heads,page,lens,causal,window", [
+    (BF, 128, 2, 64, [(1, 8192)], True, 0), (HF, 128, 2, 16, [(1, 8192), (1, 8192), (1, 700)], True, 0),
+    (BF, 64, 4, 32, [(2, 8192)], True, 0), (HF, 256, 1, 128, [(1, 8000), (1, 90)], True, 0),
+    (BF, 128, 2, 64, [(40, 8192)], False, 0), (HF, 64, 4, 16, [(70, 8192)], True, 0),
+    (BF, 256, 2, 64, [(30, 16000)], True, 0), (HF, 128, 2, 64, [(200, 8000), (33, 5000)], True, 0),
+    (BF, 128, 2, 64, [(2100, 8192)], True, 0), (BF, 128, 2, 16, [(1, 8100)], True, 5000),
+    (HF, 128, 2, 16, [(60, 8100)], True, 5001)])
+def test_no_key_is_lost_or_doubled_at_a_cut(dt, d, kv_heads, page, lens, causal, window):
+    """Queries of zero weigh every key a row sees alike: with one value of 4096 in a column and zeros in the rest, the
+    column is 4096 / (the keys it sees), or zero where that key is not seen. A column each for the keys on both sides
+    of every multiple of 64, where keys may be cut into parts, rings and tiles end. The weights are 1 to 2^-20 and
+    round to 1, the sum of them is within 2^-18, the result is rounded once: eps / 2 + 2^-16 of the value."""
+    c = Case(lens, 4 * kv_heads, kv_heads, d, page, dt, seed=31)
+    c.q.zero_()
+    c.v[0][torch.isfinite(c.v[0])] = 0.0
+    want = torch.zeros(c.T, kv_heads, d, dtype=torch.float64, device="cuda")
+    for s, (n, kv) in enumerate(lens):
+        pos = torch.arange(kv - n, kv, device="cuda") if causal else torch.full((n,), kv - 1, device="cuda")
+        low = (pos - window + 1).clamp(min=0) if window else torch.zeros_like(pos)
+        keys = [x for m in range(0, kv + 64, 64) for x in (m - 1, m) if 0 <= x < kv]
+        first = max(0, len(keys) - kv_heads * d)  # more than there are columns: the last of them
+        for i, key in enumerate(keys[first:]):
+            head, col = i // d, i % d
+            c.v[0, c.rows[s][key // page], key % page, head, col] = 4096.0
+            sees = (key <= pos) & (key >= low)
+            want[c.starts[s]:c.starts[s + 1], head, col] = torch.where(sees, 4096.0 / (pos - low + 1), 0.0)
+    want = want.repeat_interleave(4, 1)
+    got = Z.kv_attend(c.cache, 0, c.batch, c.q, causal=causal, window=window).double()
+    assert bool(((got - want).abs() <= (torch.finfo(dt).eps / 2 + 2.0 ** -16) * want).all())
+
+
 @pytest.mark.parametrize("lens", [[(1, 200)], [(1, 3000)], [(150, 400)]])
 def test_outputs_and_strides(lens):
     c = Case(lens, 8, 2, 128, 64, BF, seed=9, layers=3)

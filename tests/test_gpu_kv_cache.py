@@ -280,6 +280,70 @@ def test_the_same_sequence_twice():
     t.step("grow", [], [])
 
 
+def test_captured_page_operations():
+    """Each of them in one graph, replayed over other sequences and counts."""
+    t = Tables(80, 8, 12, 16)
+    t.step("grow", [0, 1, 2], [60, 77, 33])
+    arrays = {name: torch.zeros(2, dtype=torch.int32, device="cuda") for name in ("seq", "add", "src", "dst", "gone")}
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(Z.lib().zest_kv_pages_workspace(t.cache.ref), dtype=torch.uint8, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        Z.kv_grow(t.cache, t.t, arrays["seq"], arrays["add"], err=err)
+        Z.kv_fork(t.cache, t.t, arrays["src"], arrays["dst"], workspace=ws, err=err)
+        Z.kv_free(t.cache, t.t, arrays["gone"], err=err)
+        Z.kv_compact(t.cache, t.t, workspace=ws, err=err)
+    t.agree()  # nothing has run
+    for seq, add, src, dst, gone in [([0, 2], [5, 20], [0, 1], [3, 4], [0, 1]), ([3, 4], [40, 1], [2, 3], [0, 1], [2, 4]),
+                                     ([0, 1], [1, 1], [1, 1], [5, 6], [3, 1])]:
+        for name, v in dict(seq=seq, add=add, src=src, dst=dst, gone=gone).items():
+            arrays[name].copy_(i32(v))
+        k, v = t.k.clone(), t.v.clone()
+        for moves in (t.host.grow(seq, add), t.host.fork(src, dst), t.host.free(gone), t.host.compact()):
+            for a, b in moves:
+                k[:, b], v[:, b] = k[:, a], v[:, a]
+        g.replay()
+        t.agree()
+        assert int(err) == 0 and torch.equal(t.k, k) and torch.equal(t.v, v)
+
+
+def test_offsets_past_32_bits():
+    """Pools of two layers whose last pages lie past 2^32 values: written, copied and moved there, and nowhere else."""
+    layers, page, kv_heads, d = 2, 64, 8, 128
+    pages = (1 << 31) // (page * kv_heads * d) + 40
+    k, v = (torch.zeros(layers, pages, page, kv_heads, d, dtype=BF, device="cuda") for _ in range(2))
+    cache, last = Z.KvCache(k, v), pages - 1
+    assert (k[1, last - 2].data_ptr() - k.data_ptr()) // 2 > 1 << 32
+    g = torch.Generator("cuda").manual_seed(2)
+    kn, vn = (torch.randn(100, kv_heads, d, device="cuda", generator=g) for _ in range(2))
+    batch = Z.KvBatch(i32([0, 100]), i32([100]), i32([[last, last - 2]]), T=100, max_q=100, max_kv=100)
+    for layer in range(layers):
+        Z.kv_append(cache, layer, batch, kn, vn)
+        for x, new in ((k, kn), (v, vn)):
+            assert torch.equal(x[layer, last], new[:64].to(BF)) and torch.equal(x[layer, last - 2, :36], new[64:].to(BF))
+    used = lambda x: x.view(layers, pages, -1).view(torch.int64).ne(0).any(-1)
+    where = torch.zeros(layers, pages, dtype=torch.bool)
+    where[:, [last, last - 2]] = True
+    assert torch.equal(used(k).cpu(), where) and torch.equal(used(v).cpu(), where)
+    # a fork whose one free page is the last but one: the part page is copied to it
+    refs = torch.ones(pages, dtype=torch.int32, device="cuda")
+    refs[last - 1] = 0
+    t = Z.KvTables(refs, i32([[last, last - 2], [-1, -1]]), i32([100, 0]))
+    Z.kv_fork(cache, t, i32([0]), i32([1]))
+    assert t.tensors[1].tolist() == [[last, last - 2], [last, last - 1]] and t.tensors[2].tolist() == [100, 100]
+    assert torch.equal(k[:, last - 1], k[:, last - 2]) and torch.equal(v[:, last - 1], v[:, last - 2])
+    # only these three in use: they move to the front
+    refs.zero_()
+    refs[last - 2], refs[last - 1], refs[last] = 1, 1, 2
+    kept = k[:, last - 2:].clone(), v[:, last - 2:].clone()
+    Z.kv_compact(cache, t)
+    assert t.tensors[1].tolist() == [[2, 0], [2, 1]] and refs[:4].tolist() == [1, 1, 2, 0] and int(refs.sum()) == 4
+    assert torch.equal(k[:, :3], kept[0]) and torch.equal(v[:, :3], kept[1])
+    where[:, :3] = True
+    where[:, last - 1] = True
+    assert torch.equal(used(k).cpu(), where) and torch.equal(used(v).cpu(), where)
+
+
 def test_a_serving_loop():
     """Prompts in chunks, forks, single tokens, ended sequences, compaction: every step's attention against the
     attention of what the sequences hold, with the operators run together, the tables never read by the host."""
