@@ -446,6 +446,31 @@ def test_rows_past_the_last_move_no_bits(d):
         assert torch.equal(Z.kv_attend(c.cache, 0, c.batch, q)[:50], first[:50])
 
 
+@pytest.mark.parametrize("n_seqs,group", [(65535, 2), (4000, 24)])
+def test_the_most_sequences(n_seqs, group):
+    """65,535 of one token each, of 1 to 3 tokens in all; and as many tiles of a token's 24 heads."""
+    d, g = 16, torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(1, n_seqs, 16, 1, d, device="cuda", generator=g).to(BF) for _ in range(2))
+    q = torch.randn(n_seqs, group, d, device="cuda", generator=g).to(BF)
+    kv = (torch.arange(n_seqs, device="cuda") % 3 + 1).int()
+    pages = torch.arange(n_seqs - 1, -1, -1, dtype=torch.int32, device="cuda")
+    b = Z.KvBatch(torch.arange(n_seqs + 1, dtype=torch.int32, device="cuda"), kv, pages[:, None].contiguous(), T=n_seqs,
+                  max_q=1, max_kv=3)
+    kn, vn = (torch.randn(n_seqs, 1, d, device="cuda", generator=g) for _ in range(2))
+    cache = Z.KvCache(k, v)
+    Z.kv_append(cache, 0, b, kn, vn)
+    at = (kv - 1).long()
+    ks, vs = (x[0, pages.long(), :, 0] for x in (k, v))  # [n_seqs][16][d]
+    rows = torch.arange(n_seqs, device="cuda")
+    assert torch.equal(ks[rows, at], kn[:, 0].to(BF)) and torch.equal(vs[rows, at], vn[:, 0].to(BF))
+    got = Z.kv_attend(cache, 0, b, q).double()
+    z = torch.einsum("shd,sjd->shj", q.double(), ks[:, :3].double()) / 4
+    z.masked_fill_(torch.arange(3, device="cuda") >= kv[:, None, None], -math.inf)
+    p = torch.softmax(z, -1)
+    want, mean = (torch.einsum("shj,sjd->shd", p, x) for x in (vs[:, :3].double(), vs[:, :3].double().abs()))
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * mean).all())
+
+
 @pytest.mark.parametrize("n", [1, 200])
 def test_offsets_past_32_bits(n):
     """A pool of more than 2^32 values whose sequences lie at its end."""

@@ -192,6 +192,38 @@ def test_large_tables_out_of_place():
 
 
 @pytest.mark.parametrize("fresh", [False, True])
+def test_the_most_sequences_of_a_call(fresh):
+    """1,024 at once, each of which takes pages, is copied with a part page, and is freed."""
+    n = Z.KV_MAX_SEQS
+    t = Tables(5 * n, 2 * n + 3, 4, 16, layers=1, kv_heads=1, d=8)
+    r = random.Random(7)
+    order = r.sample(range(2 * n), 2 * n)
+    t.step("grow", order[:n], [r.randint(1, 40) for _ in range(n)], fresh=fresh)
+    assert len(t.step("fork", order[:n], order[n:], fresh=fresh)) > n // 2
+    t.step("free", order[:n], fresh=fresh)
+    assert t.step("compact", fresh=fresh)
+    with pytest.raises(Z.ZestError, match="0 to 1024"):
+        Z.kv_free(t.cache, t.t, i32(list(range(n + 1))))
+
+
+@pytest.mark.parametrize("fresh", [False, True])
+def test_tables_that_start_anywhere(fresh):
+    """Arrays 4 bytes past a 16-byte boundary, and of lengths that are no multiple of four."""
+    def shifted(x):
+        at = torch.full((x.numel() + 1,), 55, dtype=torch.int32, device="cuda")
+        at[1:] = x.flatten()
+        return at[1:].view(x.shape)
+
+    t = Tables(131, 11, 13, 16)
+    t.t = Z.KvTables(*(shifted(x) for x in t.t.tensors))
+    t.step("grow", [0, 3, 7], [100, 200, 33], fresh=fresh)
+    t.step("fork", [3, 7, 3], [1, 2, 4], fresh=fresh)
+    t.step("free", [0, 3], fresh=fresh)
+    t.step("compact", fresh=fresh)
+    assert fresh or all(int(x.flatten().as_strided((1,), (1,), 0)) == 55 for x in t.t.tensors)
+
+
+@pytest.mark.parametrize("fresh", [False, True])
 def test_page_operations_that_fail_change_nothing(fresh):
     t = Tables(10, 6, 8, 16)
     t.step("grow", [0, 1], [100, 20])  # 7 + 2 pages of 10
