@@ -158,8 +158,9 @@ __device__ __forceinline__ void append_row(float (&v)[NC][4], const append_args 
 // loads run beside. 2,048 tokens of 32 + 8 + 8 heads of 128 take 27.5 us, 2.8
 // TB/s: two thirds of the issue slots are taken, by the norm's sums over lanes
 // and the rotation's exchange (24.6 us without the norm), and four blocks' 32
-// warps an SM are what the rows in registers leave room for. 32 tokens: 3.8 us,
-// those loads' latency.
+// warps an SM are what the rows in registers leave room for: at 64 registers a
+// thread, 40 bytes of which spill (27.0 us; three blocks of 80 registers, which
+// spill none, 28.8). 32 tokens: 3.9 us, those loads' latency.
 template <int NC, bool F16>
 __global__ void __launch_bounds__(AP_WARPS * 32, NC == 1 ? 4 : 2) kv_append_kernel(const __grid_constant__ append_args A) {
     constexpr int N = AP_ROWS<NC>;
